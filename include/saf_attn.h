@@ -71,7 +71,7 @@ enum {
   SAF_EWORKSPACE = -5     /* workspace missing or too small */
 };
 
-enum { SAF_F32 = 0, SAF_F16 = 1, SAF_BF16 = 2, SAF_I32 = 3 };
+enum { SAF_F32 = 0, SAF_F16 = 1, SAF_BF16 = 2, SAF_I32 = 3, SAF_I64 = 4 };
 
 /* Head states (kernel/fused_attn.py:12-19, nanogpt/model.py:869-874). */
 enum { SAF_LIVE = 0, SAF_FROZEN_DENSE = 1, SAF_FROZEN_DECOMP = 2 };
@@ -85,7 +85,7 @@ enum { SAF_CLOSED_NONE = 0, SAF_CLOSED_MEAN = 1, SAF_CLOSED_DECAY = 2, SAF_CLOSE
 
 typedef struct saf_tensor {
   void* data;         /* device pointer (NULL = absent) */
-  int32_t dtype;      /* SAF_F32 / SAF_F16 / SAF_BF16 / SAF_I32 */
+  int32_t dtype;      /* SAF_F32 / SAF_F16 / SAF_BF16 / SAF_I32 / SAF_I64 */
   int32_t ndim;       /* number of used sizes/strides (<= 4) */
   int64_t size[4];
   int64_t stride[4];  /* in elements */
@@ -354,6 +354,110 @@ int64_t saf_mixed_attn_workspace_bytes(const saf_mixed_attn_args* args);
  * up leaves NaN in its chunk's rows and in every later chunk of that
  * (batch, head) sequence, never a silently incomplete sum. */
 int saf_workspace_error(const void* workspace, void* stream, int32_t* error_out);
+
+/* ---- after the prefill: a paged cache and its single-token attention --------
+ *
+ * K and V of past tokens live in caches of pages: k_cache (P, UK, PS, HD) and
+ * v_cache (P, HV, PS, HD), P pages of PS token slots (a power of two, at least
+ * 16).  page_table (B, N) int32 gives the page of each run of PS positions of
+ * each sequence, so position s of sequence b is slot s % PS of page
+ * page_table[b][s / PS].  As in the prefill, UK counts the live heads' compact
+ * slots and HV = H; with kvidx both are the HKV raw key / value heads (frozen
+ * heads never read K).  Page ids, positions and lengths are device data: an id
+ * outside 0..P-1 or a position past the table is never followed (see each
+ * entry point). */
+
+typedef struct saf_paged_append_args {
+  saf_tensor_t q;          /* optional (B, UQ, T, HD) */
+  saf_tensor_t k;          /* (B, UK, T, HD); absent when no head is live */
+  saf_tensor_t v;          /* (B, HV, T, HD) */
+  saf_tensor_t q_out;      /* with q: like q */
+  saf_tensor_t k_cache, v_cache;
+  saf_tensor_t page_table; /* (B, N) int32 */
+  saf_tensor_t positions;  /* (B,) int32: position of each sequence's first new token */
+  saf_tensor_t counts;     /* optional (B,) int32: new tokens per sequence (at most T), default T */
+  saf_tensor_t cos, sin;   /* optional (T', RD) fp32 / bf16 / fp16 caches, RD <= HD a multiple of 16 */
+  saf_tensor_t q_weight, k_weight;  /* optional (HD,) RMSNorm weights, both or none */
+  float eps;
+} saf_paged_append_args;
+
+/* Rotary embedding of T new tokens per sequence and their write into the
+ * cache: token t of sequence b, t < counts[b], stands at position
+ * s = positions[b] + t.  q_out and the cached key are rope_s(norm(x)), norm
+ * the RMSNorm over HD with the weights (when given), rope_s the Llama half
+ * rotation of the first RD elements with row s of cos / sin (when given); all
+ * in fp32 and rounded once.  v is copied.  Rows of q_out with t >= counts[b]
+ * are zero.  A token whose position lies outside the table or the caches of
+ * cos / sin, or whose page id is not a page, is not written and its q_out rows
+ * are NaN.  Two tokens on one slot: either may win.  bf16, fp16 and fp32, one
+ * dtype for q, k, v and the caches. */
+int saf_paged_append(const saf_paged_append_args* args, void* stream);
+
+typedef struct saf_paged_attn_args {
+  saf_tensor_t q;          /* (B, U, 1, HD) live-head queries */
+  saf_tensor_t k_cache, v_cache;
+  saf_tensor_t out;        /* (B, H, 1, HD) */
+  saf_tensor_t lse;        /* optional (B, H, 1) fp32, base-2 log-sum-exp of live heads */
+  saf_tensor_t patt;       /* (P, S, S) dense patterns (heads of state 1) */
+  saf_tensor_t alpha, rho, z;  /* (H, S) decomposed buffers (heads of state 2) */
+  saf_tensor_t page_table; /* (B, N) int32 */
+  saf_tensor_t lengths;    /* (B,) int32: cached tokens, the new one included */
+  int32_t n_heads;
+  const int32_t* frozen;   /* host tables as in saf_mixed_attn_args */
+  const int32_t* hidx;
+  const int32_t* pidx;
+  const int32_t* kvidx;
+  float sm_scale;
+  void* workspace;         /* saf_paged_attn_workspace_bytes() bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+} saf_paged_attn_args;
+
+/* Attention of the newest token of each sequence, i = lengths[b] - 1, over its
+ * cached tokens j = 0..i:
+ *   live         out = softmax_j(q . k_j * sm_scale) v_j
+ *   dense        out = sum_j patt[pidx(h), i, j] v_j
+ *   decomposed   out = sum_j exp(alpha[j] + rho[i - j] - z[i]) v_j
+ * (closed-form heads through their alpha / rho / z).  A sequence of length 0
+ * gets zero rows (lse -inf); a length past the table, or a page id outside the
+ * cache, gives NaN rows, as does a frozen head whose pattern is shorter than
+ * the sequence.  Slots past a sequence's length are not read into the result.
+ * bf16, fp16 and fp32; HD as in the prefill. */
+int saf_paged_attn_fwd(const saf_paged_attn_args* args, void* stream);
+
+/* Workspace of saf_paged_attn_fwd (0: none needed), -1 on invalid arguments. */
+int64_t saf_paged_attn_workspace_bytes(const saf_paged_attn_args* args);
+
+typedef struct saf_token_logprobs_args {
+  saf_tensor_t logits;     /* (R, V) fp32 / bf16 / fp16, unit column stride */
+  saf_tensor_t tokens;     /* (R,) int32 or int64 */
+  saf_tensor_t logp;       /* (R,) fp32 */
+  saf_tensor_t entropy;    /* optional (R,) fp32 */
+  saf_tensor_t stats;      /* (R, 2) fp32, contiguous: the largest logit, log2 of the sum relative to it */
+  saf_tensor_t top_index;  /* with top > 0: (R, top) int64 */
+  saf_tensor_t top_logp;   /* with top > 0: (R, top) fp32 */
+  int32_t top;             /* alternatives per row, 0..32 and at most V */
+  int64_t ignore_index;    /* token value of rows whose logp is 0 and has no gradient */
+  float scale;             /* x = scale * logits, scale > 0 (1 / temperature) */
+  void* workspace;         /* saf_token_logprobs_workspace_bytes() bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+} saf_token_logprobs_args;
+
+/* Log probabilities of given tokens, in one pass over the logits: with
+ * x = scale * logits, logp = x[token] - logsumexp(x) in fp32, the entropy
+ * -sum p log p, and the `top` largest entries of each row (equal ones by
+ * lower index) with their log probabilities.  A token outside 0..V-1 that is
+ * not ignore_index gives a NaN logp.  A row that holds NaN or +inf, or nothing
+ * above -inf, gives NaN (its top indices are some indices of the row). */
+int saf_token_logprobs(const saf_token_logprobs_args* args, void* stream);
+int64_t saf_token_logprobs_workspace_bytes(const saf_token_logprobs_args* args);
+
+/* Gradient of saf_token_logprobs with respect to the logits, for upstream
+ * gradients dlogp (R,) and, when present, dentropy (R,) (fp32):
+ *   dlogits_j = scale (dlogp ([j = token] - p_j) - dentropy p_j (log p_j + entropy))
+ * args is the forward's block (stats and, with dentropy, entropy as the
+ * forward wrote them); dlogits (R, V) in the logits' dtype is written. */
+int saf_token_logprobs_bwd(const saf_token_logprobs_args* args, const saf_tensor_t* dlogp,
+                           const saf_tensor_t* dentropy, const saf_tensor_t* dlogits, void* stream);
 
 /* Kernel timing: the next main kernel this host thread launches through an
  * attention entry point (the flash, dense P.V, decomposed P.V or scan kernel;

@@ -1,0 +1,485 @@
+// Attention of one new token per sequence over a paged key / value cache
+// (gfx950): live, dense-frozen and decomposed-frozen heads in one launch.
+//
+// For sequence b with n cached tokens (the new one, i = n - 1, included):
+//   live         o = sum_j softmax_j(q . k_j scale) v_j
+//   dense        o = sum_j patt[i, j] v_j
+//   decomposed   o = sum_j exp(alpha_j + rho_{i-j} - z_i) v_j
+// Every key and value is read once and used for at most a handful of queries,
+// so the bound is HBM: the layout serves wide loads in flight, and the matrix
+// pipe (which a single query column leaves almost idle) does the arithmetic
+// without LDS traffic.
+//
+// Unit: the query heads (columns, at most 16) that share one K and one V
+// head: a KV group with kvidx, a single head without.  A wave takes steps of
+// 32 keys:
+//   S^T[key][col] = K . Q^T      (A = K rows straight from memory)
+//   O^T[d][col]  += V^T . P^T    (B = P in the registers that S^T left it in)
+// with 16x16 MFMA tiles: lane (c = l % 16, g = l / 16) of an S^T tile holds
+// column c, keys 4g..4g+3, and with the key order {4g + r, 16 + 4g + r} the
+// eight weights of a lane over the step's two tiles are its B operand of the
+// P.V product as they stand.  The A operand of P.V needs eight keys of one d
+// per lane: lane (c, g) loads E consecutive d of the eight keys of its group
+// and transposes them in registers (one v_perm_b32 per two elements), with
+// output row 4g + r of tile e standing for d = E (4g + r) + e.
+//
+// P is rounded to 16 bits for the product as two terms, P = hi + lo, so the
+// rounding of the result is the output's own; fp16 weights are scaled by 2^8
+// first (their small ones would be subnormal: weights above 255 overflow).
+#include "saf_kernels.h"
+
+namespace saf {
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x3_a4_t __attribute__((ext_vector_type(3), aligned(4)));
+
+__device__ inline f32x4_t zero4() { return f32x4_t{0.f, 0.f, 0.f, 0.f}; }
+
+// Maximum / sum over the four lanes c, c + 16, c + 32, c + 48.
+__device__ inline float column_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_swap_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ inline float column_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+__device__ inline f32x4_t mfma16(__bf16, uint4 a, uint4 b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
+                                                 0, 0);
+}
+__device__ inline f32x4_t mfma16(_Float16, uint4 a, uint4 b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0,
+                                                0);
+}
+
+// One step's K and V in registers and its products, 16-bit storage.
+template <typename T, int HD> struct PagedTile {
+  static constexpr int E = HD <= 128 ? HD / 16 : 8;  // consecutive d per lane
+  static constexpr int NBLK = HD / (16 * E);
+  static constexpr int KS = HD / 32;
+  static constexpr float kShift = Elem<T>::is_bf16 ? 0.f : 8.f;  // log2 of the scale of P
+  typedef uint4 Query[KS];
+  uint4 k[2][KS];
+  uint32_t v[NBLK][2][4][E / 2];
+
+  __device__ static inline void load_q(Query& q, const T* row, bool live, int g) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      q[ks] = live ? *reinterpret_cast<const uint4*>(row + 32 * ks + 8 * g) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ inline void load_k(const T* page, uint32_t row_off, int t, int g) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k[t][ks] = *reinterpret_cast<const uint4*>(page + (row_off + 32 * ks + 8 * g));
+  }
+  __device__ inline void load_v(const T* page, uint32_t row_off, int t, int r, int c) {
+#pragma unroll
+    for (int b = 0; b < NBLK; ++b) {
+      const T* p = page + (row_off + 16 * E * b + E * c);
+      uint32_t(&w)[E / 2] = v[b][t][r];
+      if constexpr (E == 2) {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+      } else if constexpr (E == 4) {
+        const u32x2_t x = *reinterpret_cast<const u32x2_t*>(p);
+        w[0] = x[0]; w[1] = x[1];
+      } else if constexpr (E == 6) {
+        const u32x3_a4_t x = *reinterpret_cast<const u32x3_a4_t*>(p);
+        w[0] = x[0]; w[1] = x[1]; w[2] = x[2];
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+      }
+    }
+  }
+  __device__ inline f32x4_t scores(const Query& q, int t) const {
+    f32x4_t s = zero4();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mfma16(T{}, k[t][ks], q[ks], s);
+    return s;
+  }
+  __device__ inline void pv(f32x4_t (&o)[NBLK][E], const float (&p)[2][4]) const {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float a = p[t][2 * h], b = p[t][2 * h + 1];
+        const uint32_t w = Elem<T>::pack2(a, b);
+        hi[2 * t + h] = w;
+        lo[2 * t + h] = Elem<T>::pack2(a - Elem<T>::lo(w), b - Elem<T>::hi(w));
+      }
+    const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]), pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+    for (int b = 0; b < NBLK; ++b)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+        uint32_t a[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            a[2 * t + h] = __builtin_amdgcn_perm(v[b][t][2 * h + 1][e / 2], v[b][t][2 * h][e / 2], sel);
+        const uint4 av = make_uint4(a[0], a[1], a[2], a[3]);
+        o[b][e] = mfma16(T{}, av, ph, o[b][e]);
+        o[b][e] = mfma16(T{}, av, pl, o[b][e]);
+      }
+  }
+};
+
+// float32: v_mfma_f32_16x16x4_f32 (one key or d per lane and operand), the
+// same tiles with K's 16 d of a slice in the order 4g + e and P.V one key per
+// lane group and product.
+template <int HD> struct PagedTile<float, HD> {
+  static constexpr int E = HD % 64 == 0 ? 4 : 2;
+  static constexpr int NBLK = HD / (16 * E);
+  static constexpr int KS = HD / 16;
+  static constexpr float kShift = 0.f;
+  typedef float4 Query[KS];
+  float4 k[2][KS];
+  float v[NBLK][2][4][E];
+
+  __device__ static inline void load_q(Query& q, const float* row, bool live, int g) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      q[ks] = live ? *reinterpret_cast<const float4*>(row + 16 * ks + 4 * g) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ inline void load_k(const float* page, uint32_t row_off, int t, int g) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k[t][ks] = *reinterpret_cast<const float4*>(page + (row_off + 16 * ks + 4 * g));
+  }
+  __device__ inline void load_v(const float* page, uint32_t row_off, int t, int r, int c) {
+#pragma unroll
+    for (int b = 0; b < NBLK; ++b) {
+      const float* p = page + (row_off + 16 * E * b + E * c);
+      if constexpr (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[b][t][r][0] = x.x; v[b][t][r][1] = x.y; v[b][t][r][2] = x.z; v[b][t][r][3] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        v[b][t][r][0] = x.x; v[b][t][r][1] = x.y;
+      }
+    }
+  }
+  __device__ inline f32x4_t scores(const Query& q, int t) const {
+    f32x4_t s = zero4();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][ks].x, q[ks].x, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][ks].y, q[ks].y, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][ks].z, q[ks].z, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][ks].w, q[ks].w, s, 0, 0, 0);
+    }
+    return s;
+  }
+  __device__ inline void pv(f32x4_t (&o)[NBLK][E], const float (&p)[2][4]) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int b = 0; b < NBLK; ++b)
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            o[b][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[b][t][r][e], p[t][r], o[b][e], 0, 0, 0);
+  }
+};
+
+template <typename T> __device__ inline void store4(T* p, float4 x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(Elem<T>::pack2(x.x, x.y), Elem<T>::pack2(x.z, x.w));
+}
+template <> __device__ inline void store4<float>(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
+
+constexpr int kWPitch = 36;   // floats per column of a wave's frozen weights (32 keys)
+constexpr int kOPad = 4;      // floats after each column's HD partial sums
+
+// Grid: one workgroup per (sequence, unit, key range of p.chunk keys).
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void paged_attn_kernel(const PagedAttnParams p) {
+  using Tile = PagedTile<T, HD>;
+  constexpr int E = Tile::E, NBLK = Tile::NBLK;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = blockDim.x >> 6;
+  const int c = lane & 15, g = lane >> 4;
+  int wg = blockIdx.x;
+  const int split = wg % p.n_splits;
+  wg /= p.n_splits;
+  const int u = wg % p.n_units, b = wg / p.n_units;
+  const int c0 = p.unit_c0[u], nc = p.unit_c0[u + 1] - c0, nl = p.unit_live[u];
+
+  const int n_in = p.lengths[b];
+  const int n = n_in < 0 ? 0 : (n_in > p.capacity ? p.capacity : n_in);
+  bool bad = n_in > p.capacity;
+  const int j0 = split * p.chunk, j1 = min(n, j0 + p.chunk);
+  if (split > 0 && j0 >= n) return;  // the merge knows the live ranges from the lengths
+
+  extern __shared__ __align__(16) float lds[];
+  float* sm_ml = lds;                                       // [W][16][2]
+  float* sm_w = lds + W * 32 + wave * 16 * kWPitch;         // [16][kWPitch] of this wave
+  float* sm_o = lds + W * 32 + W * 16 * kWPitch;            // [W][nc][HD + kOPad]
+
+  const bool live_col = c < nl;
+  const T* qrow = reinterpret_cast<const T*>(p.q);
+  if (live_col) qrow += b * p.q_sb + p.col_q[c0 + c] * p.q_sh;
+  typename Tile::Query q;
+  Tile::load_q(q, qrow, live_col, g);
+
+  // frozen columns: lane c holds z of column c
+  float zc = 0.f;
+  if (c >= nl && c < nc && p.col_state[c0 + c] == 2 && n > 0 && n <= p.d_S)
+    zc = load_as_f32(p.z, p.col_pat[c0 + c] * p.z_sh + (n - 1) * p.z_ss, p.z_dtype);
+
+  f32x4_t o[NBLK][E];
+#pragma unroll
+  for (int k = 0; k < NBLK; ++k)
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[k][e] = zero4();
+  float m = live_col || c >= nc ? -INFINITY : 0.f, l = 0.f;
+
+  const T* kc = reinterpret_cast<const T*>(p.kc) + p.unit_k[u] * p.k_sh;
+  const T* vc = reinterpret_cast<const T*>(p.vc) + p.unit_v[u] * p.v_sh;
+  const int32_t* table = p.table + b * p.t_sb;
+  const int page_mask = (1 << p.page_shift) - 1;
+
+  int ids = 0;
+  for (int s = wave, it = 0; j0 + 32 * s < j1; s += W, ++it) {
+    const int key0 = j0 + 32 * s;
+    if ((it & 31) == 0) {
+      // page ids of the next 32 steps, two 16-key tiles each (a page holds
+      // whole tiles); a step whose second tile lies past the end uses its
+      // first tile's page and rows twice, with weight 0
+      const int kk = key0 + 32 * W * (lane >> 1);
+      ids = 0;
+      if (kk < j1) {
+        const int kt = (lane & 1) && kk + 16 < j1 ? kk + 16 : kk;
+        ids = table[kt >> p.page_shift];
+        if (ids < 0 || ids >= p.n_pages) {
+          bad = true;
+          ids = 0;
+        }
+      }
+    }
+    Tile tile;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int page = __builtin_amdgcn_readlane(ids, 2 * (it & 31) + t);
+      const int kt = t && key0 + 16 < j1 ? key0 + 16 : key0;
+      const int row0 = kt & page_mask, last = min(16, j1 - kt) - 1;
+      if (nl > 0)
+        tile.load_k(kc + page * p.k_sp, (uint32_t)(row0 + min(c, last)) * (uint32_t)p.k_st, t, g);
+      const T* vp = vc + page * p.v_sp;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        tile.load_v(vp, (uint32_t)(row0 + min(4 * g + r, last)) * (uint32_t)p.v_st, t, r, c);
+    }
+    float w[2][4];
+    if (nl > 0) {
+      f32x4_t sc[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) sc[t] = tile.scores(q, t);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          w[t][r] = key0 + 16 * t + 4 * g + r < j1 ? sc[t][r] * p.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, w[t][r]);
+        }
+      const float m_new = fmaxf(m, column_max(mx));
+      const float mu = m_new == -INFINITY ? 0.f : m_new;  // nothing above -inf yet: weights 0
+      float corr = fast_exp2(m - mu);
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          w[t][r] = fast_exp2(w[t][r] - (mu - Tile::kShift));
+          sum += w[t][r];
+        }
+      if (live_col) {
+        l = l * corr + sum;
+        m = m_new;
+      } else {
+        corr = 1.f;
+      }
+      if (__any(corr != 1.f)) {
+#pragma unroll
+        for (int k = 0; k < NBLK; ++k)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[k][e] *= corr;
+      }
+    }
+    if (nl < nc) {
+      // weights of the frozen columns, 32 keys by two columns at a time
+      const int key = key0 + (lane & 31);
+      for (int f0 = nl; f0 < nc; f0 += 2) {
+        const int f = f0 + (lane >> 5), col = c0 + min(f, nc - 1);
+        const int st = p.col_state[col], row = p.col_pat[col];
+        const float z = __shfl(zc, min(f, nc - 1), 64);
+        float x = 0.f;
+        if (f < nc && key < j1) {
+          if (st == 1) {
+            x = n <= p.p_S ? load_as_f32(p.patt, row * p.p_sh + (n - 1) * p.p_si + key * p.p_sj, p.patt_dtype)
+                           : __builtin_nanf("");
+          } else if (n <= p.d_S) {
+            const float a = load_as_f32(p.alpha, row * p.a_sh + key * p.a_ss, p.a_dtype);
+            const float d = load_as_f32(p.rho, row * p.r_sh + (n - 1 - key) * p.r_ss, p.r_dtype);
+            x = fast_exp2((a + d - z) * kLog2e);
+          } else {
+            x = __builtin_nanf("");
+          }
+        }
+        if (f < nc) sm_w[f * kWPitch + (lane & 31)] = x * (Tile::kShift != 0.f ? 256.f : 1.f);
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (!live_col) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float4 x = c < nc ? *reinterpret_cast<const float4*>(sm_w + c * kWPitch + 16 * t + 4 * g)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+          w[t][0] = x.x; w[t][1] = x.y; w[t][2] = x.z; w[t][3] = x.w;
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    tile.pv(o, w);
+  }
+
+  // merge of the workgroup's waves: every wave's column maxima and sums and
+  // its partial O in LDS, then each thread four d of one column
+  l = column_sum(l);
+  if (__any(bad)) {
+    l = __builtin_nanf("");
+#pragma unroll
+    for (int k = 0; k < NBLK; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        o[k][e] = f32x4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+  }
+  if (g == 0) {
+    sm_ml[(wave * 16 + c) * 2] = m;
+    sm_ml[(wave * 16 + c) * 2 + 1] = l;
+  }
+  if (c < nc) {
+    float* dst = sm_o + (wave * nc + c) * (HD + kOPad);
+#pragma unroll
+    for (int k = 0; k < NBLK; ++k)
+#pragma unroll
+      for (int x = 0; x < E; ++x) {  // elements 4x..4x+3 of the lane's 4E consecutive d
+        float4 f;
+        f.x = o[k][(4 * x + 0) % E][(4 * x + 0) / E];
+        f.y = o[k][(4 * x + 1) % E][(4 * x + 1) / E];
+        f.z = o[k][(4 * x + 2) % E][(4 * x + 2) / E];
+        f.w = o[k][(4 * x + 3) % E][(4 * x + 3) / E];
+        *reinterpret_cast<float4*>(dst + 16 * E * k + 4 * E * g + 4 * x) = f;
+      }
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < nc * (HD / 4); idx += blockDim.x) {
+    const int col = idx / (HD / 4), d = 4 * (idx % (HD / 4));
+    float mm = -INFINITY;
+    for (int w = 0; w < W; ++w) mm = fmaxf(mm, sm_ml[(w * 16 + col) * 2]);
+    const float mu = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < W; ++w) {
+      const float f = fast_exp2(sm_ml[(w * 16 + col) * 2] - mu);
+      const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * nc + col) * (HD + kOPad) + d);
+      ll += f * sm_ml[(w * 16 + col) * 2 + 1];
+      acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+    }
+    if (p.n_splits > 1) {
+      const int64_t slot = ((int64_t)b * p.n_heads + c0 + col) * p.n_splits + split;
+      *reinterpret_cast<float4*>(p.part_o + slot * HD + d) = acc;
+      if (d == 0) {
+        p.part_ml[2 * slot] = mm;
+        p.part_ml[2 * slot + 1] = ll;
+      }
+      continue;
+    }
+    const int h = p.col_head[c0 + col];
+    const float inv = n == 0 && !bad ? 0.f : (col < nl ? 1.f / ll : (Tile::kShift != 0.f ? 1.f / 256.f : 1.f));
+    acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+    store4(reinterpret_cast<T*>(p.out) + b * p.o_sb + h * p.o_sh + d, acc);
+    if (p.lse && d == 0 && col < nl) p.lse[b * p.l_sb + h * p.l_sh] = n == 0 && !bad ? -INFINITY : mm + log2f(ll) - Tile::kShift;
+  }
+}
+
+// Join of the key ranges of one (sequence, column): 256 threads, HD / 4
+// lanes per range, ranges in a fixed order.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p) {
+  constexpr int L = HD / 4, G = 256 / L;  // hd 96: 10 groups of 24, the rest idle
+  __shared__ float4 sm[G][L];
+  const int col = blockIdx.x % p.n_heads, b = blockIdx.x / p.n_heads;
+  const int h = p.col_head[col];
+  const bool live = p.col_state[col] == 0;
+  const int n_in = p.lengths[b];
+  const bool bad = n_in > p.capacity;
+  const int n = n_in < 0 ? 0 : (bad ? p.capacity : n_in);
+  const int ns = n == 0 ? 0 : (n - 1) / p.chunk + 1;
+  const int64_t slot = ((int64_t)b * p.n_heads + col) * p.n_splits;
+  const float* ml = p.part_ml + 2 * slot;
+  float mm = -INFINITY;
+  for (int s = 0; s < ns; ++s) mm = fmaxf(mm, ml[2 * s]);
+  const float mu = mm == -INFINITY ? 0.f : mm;
+  const int grp = threadIdx.x / L, d4 = threadIdx.x % L;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (grp < G) {
+    for (int s = grp; s < ns; s += G) {
+      const float f = fast_exp2(ml[2 * s] - mu);
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot + s) * HD + 4 * d4);
+      acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+    }
+    sm[grp][d4] = acc;
+  }
+  __syncthreads();
+  if (threadIdx.x >= L) return;
+  float ll = 0.f;
+  for (int s = 0; s < ns; ++s) ll += fast_exp2(ml[2 * s] - mu) * ml[2 * s + 1];
+  acc = sm[0][d4];
+  for (int k = 1; k < G; ++k) {
+    const float4 x = sm[k][d4];
+    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+  }
+  constexpr float shift = PagedTile<T, HD>::kShift;
+  float inv = live ? 1.f / ll : (shift != 0.f ? 1.f / 256.f : 1.f);
+  if (n == 0) inv = 0.f;
+  if (bad) inv = __builtin_nanf("");
+  acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+  store4(reinterpret_cast<T*>(p.out) + b * p.o_sb + h * p.o_sh + 4 * d4, acc);
+  if (p.lse && d4 == 0 && live)
+    p.lse[b * p.l_sb + h * p.l_sh] = bad ? __builtin_nanf("") : (n == 0 ? -INFINITY : mm + log2f(ll) - shift);
+}
+
+template <typename T, int HD>
+static hipError_t launch_paged_t(const PagedAttnParams& p, hipStream_t s) {
+  const size_t lds = sizeof(float) * p.waves * (32 + 16 * kWPitch + p.max_cols * (HD + kOPad));
+  hipLaunchKernelGGL((paged_attn_kernel<T, HD>), dim3((unsigned)((int64_t)p.B * p.n_units * p.n_splits)),
+                     dim3(64 * p.waves), lds, s, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.n_splits == 1) return e;
+  hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3((unsigned)(p.B * p.n_heads)), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+template <typename T>
+static hipError_t launch_paged_dt(const PagedAttnParams& p, int hd, hipStream_t s) {
+  switch (hd) {
+    case 32: return launch_paged_t<T, 32>(p, s);
+    case 64: return launch_paged_t<T, 64>(p, s);
+    case 96: return launch_paged_t<T, 96>(p, s);
+    case 128: return launch_paged_t<T, 128>(p, s);
+    case 256: return launch_paged_t<T, 256>(p, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int hd, hipStream_t s) {
+  if (dtype == kBF16) return launch_paged_dt<__bf16>(p, hd, s);
+  if (dtype == kF16) return launch_paged_dt<_Float16>(p, hd, s);
+  if (dtype == kF32) return launch_paged_dt<float>(p, hd, s);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace saf

@@ -16,14 +16,15 @@
 #include <string>
 #include <vector>
 
-#include "saf_attn.h"
-#include "saf_kernels.h"
+#include "saf_host.h"
 
 using namespace saf;
 
 namespace {
-
 thread_local std::string g_last_error;
+}
+
+namespace saf {
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -37,7 +38,7 @@ int fail(int code, const char* fmt, ...) {
 
 bool present(const saf_tensor_t& t) { return t.data != nullptr; }
 
-int elem_size(int dtype) { return dtype == SAF_F32 || dtype == SAF_I32 ? 4 : 2; }
+int elem_size(int dtype) { return dtype == SAF_I64 ? 8 : (dtype == SAF_F32 || dtype == SAF_I32 ? 4 : 2); }
 
 const char* dtype_name(int d) {
   switch (d) {
@@ -45,9 +46,38 @@ const char* dtype_name(int d) {
     case SAF_F16: return "float16";
     case SAF_BF16: return "bfloat16";
     case SAF_I32: return "int32";
+    case SAF_I64: return "int64";
     default: return "unknown";
   }
 }
+
+// Head dims of the forward kernels; the backward kernels and the fused
+// RoPE / q-k norm prologue stop at 128.
+bool supported_hd(int64_t hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256; }
+
+// Compute units of the current device, cached per device per thread.
+int cu_count() {
+  thread_local int cached_dev = -1, cached_cus = 0;
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  if (dev != cached_dev) {
+    int cus = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
+      cus = 256;
+    cached_dev = dev;
+    cached_cus = cus;
+  }
+  return cached_cus;
+}
+
+int launched(hipError_t e, const char* what) {
+  if (e != hipSuccess) return fail(SAF_ELAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+  return SAF_OK;
+}
+
+}  // namespace saf
+
+namespace {
 
 // Row-aligned 4-D activation: stride[3] == 1, base and row strides aligned to
 // `align` bytes.
@@ -94,9 +124,6 @@ saf_mixed_attn_args one_row(const saf_mixed_attn_args& a) {
   return r;
 }
 
-// Head dims of the forward kernels; the backward kernels and the fused
-// RoPE / q-k norm prologue stop at 128.
-bool supported_hd(int64_t hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 bool supported_bwd_hd(int64_t hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128; }
 
 int n_scan_chunks(int T, int hd) { return (T + scan_chunk_rows(hd) - 1) / scan_chunk_rows(hd); }
@@ -264,21 +291,6 @@ int plan_and_validate(const saf_mixed_attn_args* a, unsigned which, Plan& pl, bo
 }
 
 // ---- causal load balancing of the live-head kernel ------------------------
-// Compute units of the current device, cached per device per thread.
-int cu_count() {
-  thread_local int cached_dev = -1, cached_cus = 0;
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return 256;
-  if (dev != cached_dev) {
-    int cus = 0;
-    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
-      cus = 256;
-    cached_dev = dev;
-    cached_cus = cus;
-  }
-  return cached_cus;
-}
-
 struct FlashPlan {
   int n_items = 0, seg_len = 0, n_part_per_head = 0, n_split = 0;
   std::vector<int32_t> items;
@@ -399,11 +411,6 @@ int flash_qtiles_for(const saf_mixed_attn_args* a, int HD) {
 int64_t scan_ws_bytes(const Plan& pl) {
   const int64_t t = ws_layout(pl.B, pl.T, pl.HD, (int64_t)pl.scan.size()).total;
   return (t + 255) / 256 * 256;
-}
-
-int launched(hipError_t e, const char* what) {
-  if (e != hipSuccess) return fail(SAF_ELAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
-  return SAF_OK;
 }
 
 // Pending events of saf_time_next_kernel (per host thread, consumed by the

@@ -11,7 +11,7 @@ namespace saf {
 constexpr int kMaxHeads = 128;
 
 // dtype codes shared with the C-ABI (saf_attn.h)
-enum : int { kF32 = 0, kF16 = 1, kBF16 = 2, kI32 = 3 };
+enum : int { kF32 = 0, kF16 = 1, kBF16 = 2, kI32 = 3, kI64 = 4 };
 
 // Causal load balancing of the live-head kernel: the per-head work list
 // holds (query block, key segment) items, heaviest first; query blocks whose
@@ -208,6 +208,114 @@ struct ProjGemmParams {
   int64_t cs_st, sn_st;
 };
 
+// Single-token attention over a paged cache (paged_attn.hip).  Columns are the
+// query heads in unit order: unit u covers columns unit_c0[u]..unit_c0[u+1]-1
+// (at most 16, its unit_live[u] live heads first), which share key head
+// unit_k[u] and value head unit_v[u].
+struct PagedAttnParams {
+  const void* q;
+  const void* kc;
+  const void* vc;
+  void* out;
+  float* lse;  // may be null
+  int64_t q_sb, q_sh;
+  int64_t k_sp, k_sh, v_sp, v_sh;  // page and head strides of the caches
+  int k_st, v_st;                  // slot strides
+  int64_t o_sb, o_sh, l_sb, l_sh;
+  const int32_t* table;
+  int64_t t_sb;
+  const int32_t* lengths;
+  int page_shift, n_pages, capacity;  // capacity = page_table columns x page size
+  int B, n_heads, n_units, n_splits, chunk, waves, max_cols;
+  float scale_log2;
+  float* part_o;   // [B][n_heads][n_splits][HD] (by column), n_splits > 1
+  float* part_ml;  // [B][n_heads][n_splits][2]
+  const void* patt;
+  int patt_dtype, p_S;
+  int64_t p_sh, p_si, p_sj;
+  const void* alpha;
+  const void* rho;
+  const void* z;
+  int a_dtype, r_dtype, z_dtype, d_S;
+  int64_t a_sh, a_ss, r_sh, r_ss, z_sh, z_ss;
+  int16_t unit_c0[kMaxHeads + 2];
+  int16_t unit_live[kMaxHeads];
+  int16_t unit_k[kMaxHeads];
+  int16_t unit_v[kMaxHeads];
+  int16_t col_head[kMaxHeads];
+  int16_t col_q[kMaxHeads];
+  int16_t col_pat[kMaxHeads];   // dense: pattern row; decomposed: buffer row
+  int16_t col_state[kMaxHeads];
+};
+static_assert(sizeof(PagedAttnParams) <= 4096, "PagedAttnParams must fit the kernel argument segment");
+
+// New tokens into a paged cache (paged_append.hip).
+struct PagedAppendParams {
+  const void* q;  // null: none
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* kc;
+  void* vc;
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+  int64_t qo_sb, qo_sh, qo_st;
+  int64_t kc_sp, kc_sh, kc_st, vc_sp, vc_sh, vc_st;
+  const int32_t* table;
+  int64_t t_sb;
+  const int32_t* positions;
+  const int32_t* counts;  // null: T for every sequence
+  int page_shift, n_pages, capacity;
+  int B, T, Uq, Uk, Hv, hd;
+  const void* cos;  // null: no rotation
+  const void* sin;
+  int64_t cs_st, sn_st;
+  int cs_dtype, cs_rows, rd;
+  const void* q_w;  // null: no norm
+  const void* k_w;
+  int w_dtype;
+  float eps;
+};
+
+// Log probabilities of given tokens (token_logprobs.hip).
+struct LogprobParams {
+  const void* logits;
+  int64_t x_rs;
+  int64_t R;
+  int V;
+  const void* tokens;
+  int tok_i64;
+  int64_t tok_st;
+  int64_t ignore;
+  float scale;
+  float* logp;
+  float* entropy;   // null: none
+  float* stats;     // (R, 2)
+  int64_t* top_index;
+  float* top_logp;
+  int top;
+  int n_seg, seg_len;  // row segments (n_seg > 1: partials in the workspace)
+  float* part;         // [R][n_seg][4]: max, sum, sum e (x - m)
+  uint64_t* part_top;  // [R][n_seg][top]
+  int n_cu;
+};
+struct LogprobBwdParams {
+  const void* logits;
+  void* dx;
+  int64_t x_rs, d_rs;
+  int64_t R;
+  int V;
+  const void* tokens;
+  int tok_i64;
+  int64_t tok_st;
+  int64_t ignore;
+  float scale;
+  const float* stats;
+  const float* entropy;
+  const float* dlogp;
+  const float* dent;  // null: none
+  int64_t g_st, ge_st;
+};
+
 // Rows of one scan chunk for a head dimension (must match ScanShape in the
 // kernel): 8 rows per thread, 32 KB of V per chunk for hd 64 / 128.
 inline int scan_chunk_rows(int hd) { return hd == 32 ? 512 : (hd == 64 ? 256 : 128); }
@@ -223,6 +331,10 @@ hipError_t launch_scan(const ScanParams& p, int dtype, int hd, hipStream_t s);
 hipError_t launch_zero_u32(uint32_t* ptr, int64_t n, hipStream_t s);
 hipError_t launch_rope(const RopeParams& p, int dtype, hipStream_t s);
 hipError_t launch_add_layernorm(const AddLnParams& p, int dtype, hipStream_t s);
+hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int hd, hipStream_t s);
+hipError_t launch_paged_append(const PagedAppendParams& p, int dtype, hipStream_t s);
+hipError_t launch_token_logprobs(const LogprobParams& p, int dtype, hipStream_t s);
+hipError_t launch_token_logprobs_bwd(const LogprobBwdParams& p, int dtype, hipStream_t s);
 bool proj_gemm_shape_ok(int64_t M, int64_t N, int64_t K);
 // exact GELU in place over n elements (n % 8 == 0, 16-byte aligned)
 hipError_t launch_gelu_inplace(void* x, int64_t n, int dtype, int n_cu, hipStream_t s);

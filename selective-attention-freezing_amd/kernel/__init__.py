@@ -17,6 +17,8 @@ from .rope import rope_qk_, qk_rmsnorm_rope_
 from .layernorm import add_layernorm_, add_rmsnorm_
 from .projection import (gelu_, gelu_usable, linear_gelu, linear_gelu_usable, linear_rope, linear_rope_usable, linear_swiglu,
                          linear_swiglu_usable, swiglu_weight)
+from .paged import paged_append_, paged_mixed_attn
+from .logprobs import TokenLogprobs, token_logprobs
 from .fused_attn import (fused_mixed_attn, fused_attn_usable, decomposed_logz,
                          decomp_log_normalizers, decomp_log_normalizers_fft,
                          decomp_logits, make_rho_band, BAND_ROWS,
@@ -31,4 +33,5 @@ __all__ = ["frozen_pv", "frozen_pv_usable", "HAVE_TRITON",
            "classify_closed_form", "CLOSED_NONE", "CLOSED_MEAN",
            "CLOSED_DECAY", "CLOSED_WINDOW", "KernelTimer", "set_kernel_timer",
            "rope_qk_", "qk_rmsnorm_rope_", "add_layernorm_", "add_rmsnorm_", "gelu_", "gelu_usable", "linear_gelu", "linear_gelu_usable",
-           "linear_rope", "linear_rope_usable", "linear_swiglu", "linear_swiglu_usable", "swiglu_weight"]
+           "linear_rope", "linear_rope_usable", "linear_swiglu", "linear_swiglu_usable", "swiglu_weight",
+           "paged_append_", "paged_mixed_attn", "TokenLogprobs", "token_logprobs"]

@@ -15,11 +15,11 @@ LIB_NAME = "libsafattn.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 
 SAF_OK, SAF_EINVAL, SAF_EUNSUPPORTED, SAF_EALIGN, SAF_ELAUNCH, SAF_EWORKSPACE = 0, -1, -2, -3, -4, -5
-SAF_F32, SAF_F16, SAF_BF16, SAF_I32 = 0, 1, 2, 3
+SAF_F32, SAF_F16, SAF_BF16, SAF_I32, SAF_I64 = 0, 1, 2, 3, 4
 SAF_MAX_HEADS = 128
 
 _DTYPE_CODE = {torch.float32: SAF_F32, torch.float16: SAF_F16,
-               torch.bfloat16: SAF_BF16, torch.int32: SAF_I32}
+               torch.bfloat16: SAF_BF16, torch.int32: SAF_I32, torch.int64: SAF_I64}
 
 # Exported symbols, in header order (checked by the CPU test suite).
 EXPORTS = ("saf_mixed_attn_fwd", "saf_mixed_attn_side_kernels", "saf_mixed_attn_fwd_noalloc", "saf_flash_fwd",
@@ -29,6 +29,8 @@ EXPORTS = ("saf_mixed_attn_fwd", "saf_mixed_attn_side_kernels", "saf_mixed_attn_
            "saf_rope_qk_inplace", "saf_qk_rmsnorm_rope_inplace", "saf_add_layernorm",
            "saf_add_rmsnorm", "saf_linear_gelu", "saf_gelu_inplace", "saf_linear_swiglu", "saf_linear_rope", "saf_decomposed_logz",
            "saf_decomposed_logz_bwd", "saf_workspace_bytes", "saf_mixed_attn_workspace_bytes", "saf_workspace_error",
+           "saf_paged_append", "saf_paged_attn_fwd", "saf_paged_attn_workspace_bytes", "saf_token_logprobs",
+           "saf_token_logprobs_workspace_bytes", "saf_token_logprobs_bwd",
            "saf_time_next_kernel", "saf_last_error", "saf_version")
 
 
@@ -55,6 +57,34 @@ class SafMixedAttnArgs(ctypes.Structure):
                 ("flash_qtiles", ctypes.c_int32),
                 ("scan_spin_limit", ctypes.c_int32),
                 ("decomp_unsplit", ctypes.c_int32)]
+
+
+class SafPagedAppendArgs(ctypes.Structure):
+    _fields_ = [(n, SafTensor) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "page_table", "positions",
+                                         "counts", "cos", "sin", "q_weight", "k_weight")] + \
+        [("eps", ctypes.c_float)]
+
+
+class SafPagedAttnArgs(ctypes.Structure):
+    _fields_ = [(n, SafTensor) for n in ("q", "k_cache", "v_cache", "out", "lse", "patt", "alpha", "rho", "z",
+                                         "page_table", "lengths")] + \
+        [("n_heads", ctypes.c_int32),
+         ("frozen", ctypes.POINTER(ctypes.c_int32)),
+         ("hidx", ctypes.POINTER(ctypes.c_int32)),
+         ("pidx", ctypes.POINTER(ctypes.c_int32)),
+         ("kvidx", ctypes.POINTER(ctypes.c_int32)),
+         ("sm_scale", ctypes.c_float),
+         ("workspace", ctypes.c_void_p),
+         ("workspace_bytes", ctypes.c_int64)]
+
+
+class SafTokenLogprobsArgs(ctypes.Structure):
+    _fields_ = [(n, SafTensor) for n in ("logits", "tokens", "logp", "entropy", "stats", "top_index", "top_logp")] + \
+        [("top", ctypes.c_int32),
+         ("ignore_index", ctypes.c_int64),
+         ("scale", ctypes.c_float),
+         ("workspace", ctypes.c_void_p),
+         ("workspace_bytes", ctypes.c_int64)]
 
 
 _lib = None
@@ -124,6 +154,18 @@ def lib():
         L.saf_mixed_attn_workspace_bytes.restype = ctypes.c_int64
         L.saf_workspace_error.argtypes = [ctypes.c_void_p, ctypes.c_void_p, P(ctypes.c_int32)]
         L.saf_workspace_error.restype = ctypes.c_int
+        for name, block in (("saf_paged_append", SafPagedAppendArgs), ("saf_paged_attn_fwd", SafPagedAttnArgs),
+                            ("saf_token_logprobs", SafTokenLogprobsArgs)):
+            fn = getattr(L, name)
+            fn.argtypes = [P(block), ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+        for name, block in (("saf_paged_attn_workspace_bytes", SafPagedAttnArgs),
+                            ("saf_token_logprobs_workspace_bytes", SafTokenLogprobsArgs)):
+            fn = getattr(L, name)
+            fn.argtypes = [P(block)]
+            fn.restype = ctypes.c_int64
+        L.saf_token_logprobs_bwd.argtypes = [P(SafTokenLogprobsArgs)] + [P(SafTensor)] * 3 + [ctypes.c_void_p]
+        L.saf_token_logprobs_bwd.restype = ctypes.c_int
         L.saf_time_next_kernel.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         L.saf_time_next_kernel.restype = ctypes.c_int
         L.saf_last_error.argtypes = []
@@ -173,6 +215,47 @@ def rows_desc(t):
 def set_desc(args, offset, t):
     """tensor_desc(t) written at a byte offset of an argument block."""
     _DESC.pack_into(args, offset, *_desc_values(t))
+
+
+def fill(block, **tensors):
+    """Write the descriptors of the given tensors (None: left absent) into
+    their fields of an argument block."""
+    offset = _OFFSETS[type(block)]
+    for name, t in tensors.items():
+        if t is not None:
+            _DESC.pack_into(block, offset[name], *_desc_values(t))
+
+
+_OFFSETS = {c: {n: getattr(c, n).offset for n, kind in c._fields_ if kind is SafTensor}
+            for c in (SafPagedAppendArgs, SafPagedAttnArgs, SafTokenLogprobsArgs)}
+
+
+def same_device(what, device, **tensors):
+    """Raise unless every given tensor lives on `device`, a HIP device."""
+    if device.type != "cuda":
+        raise RuntimeError(f"{what} runs on HIP devices only (got a CPU tensor)")
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def on_device(device):
+    """Context that makes `device` the current one (launches and cached device
+    properties follow it); nothing to do where it is."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(device)
 
 
 # saf_mixed_attn_args: offsets of the tensor descriptors, and the fields from

@@ -1,0 +1,113 @@
+"""Log probabilities of given tokens: what a model answers with, and its loss.
+
+``token_logprobs`` reads each row of logits once and gives the log probability
+of the row's token, the entropy of the distribution and its most likely
+alternatives (libsafattn.so ``saf_token_logprobs``); its backward writes the
+logits' gradient in one pass (``saf_token_logprobs_bwd``), so
+``-token_logprobs(logits, tokens).logp.mean()`` is the cross-entropy loss.  It
+serves the evaluation that the reference does with log_softmax and gather
+(/root/reference/nanogpt/eval_nanogpt_logprobs.py) and sampling loops that
+report alternatives.
+"""
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _ext
+
+
+class TokenLogprobs(NamedTuple):
+    logp: torch.Tensor                  # (...) fp32
+    entropy: Optional[torch.Tensor]     # (...) fp32, nats
+    top_index: Optional[torch.Tensor]   # (..., top) int64
+    top_logp: Optional[torch.Tensor]    # (..., top) fp32
+
+
+def _forward(logits, tokens, top, entropy, scale, ignore_index):
+    R, dev = logits.size(0), logits.device
+    f32 = dict(device=dev, dtype=torch.float32)
+    logp, stats = torch.empty(R, **f32), torch.empty(R, 2, **f32)
+    ent = torch.empty(R, **f32) if entropy else None
+    idx = torch.empty(R, top, device=dev, dtype=torch.int64) if top else None
+    tlp = torch.empty(R, top, **f32) if top else None
+    args = _ext.SafTokenLogprobsArgs()
+    _ext.fill(args, logits=logits, tokens=tokens, logp=logp, entropy=ent, stats=stats, top_index=idx, top_logp=tlp)
+    args.top, args.ignore_index, args.scale = top, ignore_index, scale
+    L = _ext.lib()
+    with _ext.on_device(dev):
+        nbytes = L.saf_token_logprobs_workspace_bytes(args)
+        if nbytes > 0:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+        rc = L.saf_token_logprobs(args, _ext.current_stream_ptr(dev))
+    if rc:
+        _ext.check(rc)
+    return logp, ent, idx, tlp, stats
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, logits, tokens, top, entropy, scale, ignore_index):
+        logp, ent, idx, tlp, stats = _forward(logits, tokens, top, entropy, scale, ignore_index)
+        ctx.save_for_backward(logits, tokens, stats, ent)
+        ctx.scale, ctx.ignore_index = scale, ignore_index
+        ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(idx, tlp)
+        return logp, ent, idx, tlp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, glogp, gent, _gi, _gt):
+        logits, tokens, stats, ent = ctx.saved_tensors
+        if glogp is None and gent is None:
+            return (None,) * 6
+        glogp = torch.zeros_like(stats[:, 0]) if glogp is None else glogp.float()
+        gent = None if gent is None else gent.float()
+        R, V = logits.shape
+        dx = torch.empty(R, V, device=logits.device, dtype=logits.dtype)
+        args = _ext.SafTokenLogprobsArgs()
+        _ext.fill(args, logits=logits, tokens=tokens, stats=stats, entropy=ent)
+        args.ignore_index, args.scale = ctx.ignore_index, ctx.scale
+        with _ext.on_device(logits.device):
+            rc = _ext.lib().saf_token_logprobs_bwd(
+                args, _ext.tensor_desc(glogp), _ext.tensor_desc(gent), _ext.tensor_desc(dx),
+                _ext.current_stream_ptr(logits.device))
+        if rc:
+            _ext.check(rc)
+        return dx, None, None, None, None, None
+
+
+def token_logprobs(logits, tokens, top=0, entropy=False, scale=1.0, ignore_index=-100):
+    """Log probabilities of ``tokens`` (...) under softmax(scale * logits)
+    for logits (..., V) in float32, bfloat16 or float16.
+
+      tokens   int64 or int32 indices; ``ignore_index`` marks rows whose logp
+               is 0 and which get no gradient through it; any other index
+               outside 0..V-1 gives NaN
+      top      alternatives per row (0..32): the indices and log probabilities
+               of the largest logits, equal ones by lower index.  Not
+               differentiable
+      entropy  also return -sum p log p (nats)
+      scale    1 / temperature, > 0
+    fp32 arithmetic throughout; the gradient of logp and entropy with respect
+    to the logits is rounded once to their dtype.  As with log_softmax, a row
+    holding NaN or +inf, or nothing above -inf, gives NaN (its top indices are
+    then some indices of the row)."""
+    if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"tokens must have the logits' leading shape (got {tuple(tokens.shape)} for "
+                         f"{tuple(logits.shape)})")
+    _ext.same_device("token_logprobs", logits.device, tokens=tokens)
+    top, scale = int(top), float(scale)
+    lead, V = tokens.shape, logits.size(-1)
+    x = logits.reshape(-1, V)
+    if V > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    t = tokens.reshape(-1)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        logp, ent, idx, tlp = _TokenLogprobsFn.apply(x, t, top, bool(entropy), scale, int(ignore_index))
+    else:
+        logp, ent, idx, tlp, _ = _forward(x, t, top, bool(entropy), scale, int(ignore_index))
+    return TokenLogprobs(logp.view(lead), None if ent is None else ent.view(lead),
+                         None if idx is None else idx.view(*lead, top), None if tlp is None else tlp.view(*lead, top))

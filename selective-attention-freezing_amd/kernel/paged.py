@@ -1,0 +1,173 @@
+"""The token after the prefill: a paged key / value cache and its attention.
+
+``fused_mixed_attn`` runs whole sequences.  These two operators continue them
+one token at a time, with the same head states (live, dense-frozen,
+decomposed-frozen), compact live slots and GQA map:
+
+    q = paged_append_(k, v, k_cache, v_cache, page_table, positions, q=q, cos=cos, sin=sin)
+    y = paged_mixed_attn(q, k_cache, v_cache, page_table, lengths, patt, frozen, hidx, ...)
+
+A cache is a pool of pages: ``k_cache`` (P, U, PS, HD) for the live heads' U
+compact slots and ``v_cache`` (P, H, PS, HD) for every head (with ``kvidx``
+both hold the HKV raw heads; frozen heads never read keys), PS token slots a
+page (a power of two, at least 16).  ``page_table`` (B, N) int32 lists each
+sequence's pages: its position s is slot s % PS of page
+``page_table[b, s // PS]``.  Page ids, positions and lengths are device data
+that no call reads back; what they get wrong shows as NaN, never as a stray
+access (libsafattn.so ``saf_paged_append``, ``saf_paged_attn_fwd``).  Forward
+only.
+"""
+import torch
+
+from . import _ext
+from .fused_attn import _table, decomposed_logz
+
+
+def _no_grad_only(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError(f"{what} has no backward: call it under torch.no_grad()")
+
+
+def paged_append_(k, v, k_cache, v_cache, page_table, positions, counts=None, q=None, cos=None, sin=None,
+                  q_weight=None, k_weight=None, eps=1e-6):
+    """Write T new tokens per sequence into the caches, in place, rotating
+    them to their positions; returns the rotated q (None without q).
+
+      k        (B, U, T, HD) keys of the live slots (the HKV heads with GQA),
+               None when no head is live (k_cache None as well)
+      v        (B, H, T, HD) values of every head (the HKV heads with GQA)
+      positions (B,) int32, the position of each sequence's first new token
+      counts   (B,) int32, new tokens per sequence (right-padded batches);
+               default T.  The rest of a sequence writes nothing and its rows
+               of the returned q are zero
+      q        (B, UQ, T, HD) queries, not modified
+      cos, sin (T', RD) caches (leading singleton dims are dropped), row s for
+               position s: Llama half rotation of the first RD <= HD elements
+               (a multiple of 16); None: no rotation
+      q_weight, k_weight  (HD,) per-head RMSNorm weights, applied before the
+               rotation: w x / sqrt(mean(x^2) + eps)
+    fp32 arithmetic, one rounding.  A token whose position lies outside the
+    page table or the cos / sin caches, or whose page id is not a page of the
+    caches, is not written, and its rows of q are NaN."""
+    _no_grad_only("paged_append_", q, k, v, k_cache, v_cache)
+    if (k is None) != (k_cache is None):
+        raise ValueError("k and k_cache go together")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    dev = v.device
+    if cos is not None:
+        cos = cos.reshape(-1, cos.size(-1))
+        sin = sin.reshape(-1, sin.size(-1))
+    _ext.same_device("paged_append_", dev, k=k, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
+                     positions=positions, counts=counts, q=q, cos=cos, sin=sin, q_weight=q_weight, k_weight=k_weight)
+    if k is not None and k.size(1) == 0:
+        k = k_cache = None
+    q_in, k_in, v_in = (_rows16(t) for t in (q, k, v))
+    out = None
+    if q is not None:
+        # token-major like the projection it came from, so that a token's rows
+        # follow each other
+        B, U, T, HD = q.shape
+        out = torch.empty((B, T, U, HD), device=dev, dtype=q.dtype).transpose(1, 2)
+    if v.numel() == 0:
+        return out
+    args = _ext.SafPagedAppendArgs()
+    _ext.fill(args, q=q_in, k=k_in, v=v_in, q_out=out, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
+              positions=positions, counts=counts, cos=cos, sin=sin,
+              q_weight=None if q_weight is None else q_weight.detach(),
+              k_weight=None if k_weight is None else k_weight.detach())
+    if q is not None and q.numel() == 0:
+        args.q.data = None
+    args.eps = float(eps)
+    with _ext.on_device(dev):
+        rc = _ext.lib().saf_paged_append(args, _ext.current_stream_ptr(dev))
+    if rc:
+        _ext.check(rc)
+    return out
+
+
+def _rows16(t):
+    """t, or a copy whose (B, U, T, HD) rows are 16-byte aligned (rows may
+    overlap or repeat: they are only read)."""
+    if t is None:
+        return None
+    es = t.element_size()
+    ok = t.data_ptr() % 16 == 0 and (t.size(-1) == 1 or t.stride(-1) == 1) and all(
+        n <= 1 or (s * es) % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def paged_mixed_attn(q, k_cache, v_cache, page_table, lengths, patt, frozen, hidx=None, pidx=None, sm_scale=None,
+                     alpha=None, rho=None, z=None, validate=True, kvidx=None, lse=None):
+    """Attention of the newest token of each sequence over its cached tokens,
+    all heads in one call.
+
+      q        (B, U, 1, HD) compact live-head queries
+      k_cache, v_cache, page_table   see the module's docstring
+      lengths  (B,) int32 cached tokens, the newest included: the query stands
+               at position i = lengths - 1.  0 gives zero rows (an idle slot
+               of a batch)
+      patt, frozen, hidx, pidx, sm_scale, alpha, rho, z, kvidx, lse
+               as in fused_mixed_attn: row i of the patterns (closed-form
+               heads through their alpha / rho / z); lse (B, H, 1) fp32
+    Returns (B, H, 1, HD).  A length past the page table, a page id outside
+    the caches, and for a frozen head a length past its pattern give NaN rows.
+    validate also checks shapes with the reference operator's messages."""
+    H = frozen.numel() if isinstance(frozen, torch.Tensor) else len(frozen)
+    _no_grad_only("paged_mixed_attn", q, k_cache, v_cache, alpha, rho, z, patt)
+    dev = v_cache.device
+    _ext.same_device("paged_mixed_attn", dev, q=q, k_cache=k_cache, page_table=page_table, lengths=lengths, patt=patt,
+                     alpha=alpha, rho=rho, z=z, lse=lse)
+    if sm_scale is None:
+        sm_scale = 1.0 / (v_cache.size(-1) ** 0.5)
+    if alpha is not None and z is None:
+        z = decomposed_logz(alpha.float(), rho.float())
+    frozen_h, frozen_c = _table(frozen)
+    if validate:
+        _validate(q, k_cache, v_cache, page_table, lengths, patt, frozen_h, alpha, rho, z, kvidx)
+    tables = [_table(t)[1] for t in (hidx, pidx, kvidx)]
+    for name, t in zip(("hidx", "pidx", "kvidx"), tables):
+        if t is not None and len(t) < H:
+            raise ValueError(f"{name} must have one entry per output head")
+    B, HD = page_table.size(0), v_cache.size(-1)
+    out = torch.empty((B, H, 1, HD), device=dev, dtype=v_cache.dtype)
+    if B == 0:
+        return out
+    q = _rows16(q)
+    args = _ext.SafPagedAttnArgs()
+    live = q is not None and q.numel() > 0
+    _ext.fill(args, q=q if live else None, k_cache=k_cache if live else None, v_cache=v_cache, out=out, lse=lse, patt=patt,
+              alpha=alpha, rho=rho, z=z, page_table=page_table, lengths=lengths)
+    args.n_heads = H
+    args.frozen = frozen_c
+    args.hidx, args.pidx, args.kvidx = tables
+    args.sm_scale = float(sm_scale)
+    L = _ext.lib()
+    with _ext.on_device(dev):
+        nbytes = L.saf_paged_attn_workspace_bytes(args)
+        if nbytes > 0:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+        rc = L.saf_paged_attn_fwd(args, _ext.current_stream_ptr(dev))
+    if rc:
+        _ext.check(rc)
+    return out
+
+
+def _validate(q, k_cache, v_cache, page_table, lengths, patt, frozen, alpha, rho, z, kvidx):
+    assert v_cache.ndim == 4 and page_table.ndim == 2 and lengths.ndim == 1, \
+        "v_cache must be (P, H, PS, HD), page_table (B, N) and lengths (B,)"
+    assert page_table.dtype == lengths.dtype == torch.int32, "page_table and lengths must be int32"
+    B = page_table.size(0)
+    assert lengths.size(0) == B, "lengths must have one entry per sequence"
+    if kvidx is None:
+        assert v_cache.size(1) == len(frozen), "v_cache must hold one head per output head (or pass kvidx)"
+    if (frozen == 0).any():
+        assert q is not None and k_cache is not None, "live heads require q and k_cache"
+        assert q.ndim == 4 and q.shape[0] == B and q.shape[2] == 1 and q.shape[3] == v_cache.size(3), \
+            "q must be (B, U, 1, HD): one new token per sequence"
+    assert patt is not None or not (frozen == 1).any(), "dense-frozen heads require patt"
+    if (frozen == 2).any():
+        assert alpha is not None and rho is not None and alpha.shape == rho.shape == z.shape, \
+            "alpha, rho, and z must have matching (H, S) shapes"
+        assert alpha.shape[0] == len(frozen), "decomposed buffers must have shape (H, S)"
