@@ -35,7 +35,8 @@ HIPCC_FLAGS = [
 # instructions removes the copies and lowers register use.  The float32
 # kernels hold their accumulators across loops the same way.
 SOURCE_FLAGS = {"attn_bwd.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
-                "attn_f32.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form")}
+                "attn_f32.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
+                "paged_attn.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form")}
 
 
 def _hipcc():

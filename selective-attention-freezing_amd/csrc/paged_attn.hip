@@ -69,14 +69,17 @@ template <typename T, int HD> struct PagedTile {
     for (int ks = 0; ks < KS; ++ks)
       q[ks] = live ? *reinterpret_cast<const uint4*>(row + 32 * ks + 8 * g) : make_uint4(0, 0, 0, 0);
   }
-  __device__ inline void load_k(const T* page, uint32_t row_off, int t, int g) {
+  // byte offsets of a lane within a row
+  __device__ static inline uint32_t k_lane(int g) { return 16 * g; }
+  __device__ static inline uint32_t v_lane(int c) { return 2 * E * c; }
+  __device__ inline void load_k(const char* page, uint32_t off, int t) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) k[t][ks] = *reinterpret_cast<const uint4*>(page + (row_off + 32 * ks + 8 * g));
+    for (int ks = 0; ks < KS; ++ks) k[t][ks] = *reinterpret_cast<const uint4*>(page + off + 64 * ks);
   }
-  __device__ inline void load_v(const T* page, uint32_t row_off, int t, int r, int c) {
+  __device__ inline void load_v(const char* page, uint32_t off, int t, int r) {
 #pragma unroll
     for (int b = 0; b < NBLK; ++b) {
-      const T* p = page + (row_off + 16 * E * b + E * c);
+      const char* p = page + off + 32 * E * b;
       uint32_t(&w)[E / 2] = v[b][t][r];
       if constexpr (E == 2) {
         w[0] = *reinterpret_cast<const uint32_t*>(p);
@@ -145,14 +148,16 @@ template <int HD> struct PagedTile<float, HD> {
     for (int ks = 0; ks < KS; ++ks)
       q[ks] = live ? *reinterpret_cast<const float4*>(row + 16 * ks + 4 * g) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ inline void load_k(const float* page, uint32_t row_off, int t, int g) {
+  __device__ static inline uint32_t k_lane(int g) { return 16 * g; }
+  __device__ static inline uint32_t v_lane(int c) { return 4 * E * c; }
+  __device__ inline void load_k(const char* page, uint32_t off, int t) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) k[t][ks] = *reinterpret_cast<const float4*>(page + (row_off + 16 * ks + 4 * g));
+    for (int ks = 0; ks < KS; ++ks) k[t][ks] = *reinterpret_cast<const float4*>(page + off + 64 * ks);
   }
-  __device__ inline void load_v(const float* page, uint32_t row_off, int t, int r, int c) {
+  __device__ inline void load_v(const char* page, uint32_t off, int t, int r) {
 #pragma unroll
     for (int b = 0; b < NBLK; ++b) {
-      const float* p = page + (row_off + 16 * E * b + E * c);
+      const char* p = page + off + 64 * E * b;
       if constexpr (E == 4) {
         const float4 x = *reinterpret_cast<const float4*>(p);
         v[b][t][r][0] = x.x; v[b][t][r][1] = x.y; v[b][t][r][2] = x.z; v[b][t][r][3] = x.w;
@@ -191,114 +196,155 @@ template <typename T> __device__ inline void store4(T* p, float4 x) {
 }
 template <> __device__ inline void store4<float>(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
 
-constexpr int kWPitch = 36;   // floats per column of a wave's frozen weights (32 keys)
-constexpr int kOPad = 4;      // floats after each column's HD partial sums
+constexpr int kOPad = 4;  // floats after each column's HD partial sums
 
-// Grid: one workgroup per (sequence, unit, key range of p.chunk keys).
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void paged_attn_kernel(const PagedAttnParams p) {
+// What one wave keeps of its unit while it walks the keys.
+template <typename T, int HD> struct PagedWave {
+  using Tile = PagedTile<T, HD>;
+  static constexpr int E = Tile::E, NBLK = Tile::NBLK;
+  typename Tile::Query q;
+  f32x4_t o[NBLK][E];
+  float m, l;
+  bool bad;
+};
+
+// Weights of the frozen columns for the keys kb0..kb1-1, into w[f][key - kb0]
+// (f = column - nl), before the walk: the waves take runs of 256 keys of one
+// column in turn, four keys per lane, whose loads are in flight together.
+// Whole steps are written: weight 0 behind the last key.
+__device__ inline void frozen_weights(const PagedAttnParams& p, float* w, int pitch, int c0, int nl, int nc, int n, int kb0,
+                                      int kb1, int wave, int W, int lane, float scale) {
+  const int F = nc - nl, end = kb0 + ((kb1 - kb0 + 31) & ~31);
+  const int items = F * ((kb1 - kb0 + 255) >> 8);
+  for (int item = wave; item < items; item += W) {
+    const int run = item / F, f = item - run * F;
+    const int64_t word = p.col[c0 + nl + f];
+    const int state = col_state(word), row = col_pat(word);
+    const bool fits = n <= (state == 1 ? p.p_S : p.d_S);  // else the row is NaN
+    const int key0 = kb0 + 256 * run + lane;
+    float x[4];
+    if (!fits) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = __builtin_nanf("");
+    } else if (state == 1) {
+      uint32_t v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = load_bits(p.patt, row * p.p_sh + (n - 1) * p.p_si + min(key0 + 64 * k, kb1 - 1) * p.p_sj, p.patt_dtype);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = bits_to_f32(v[k], p.patt_dtype) * scale;
+    } else {
+      uint32_t a[4], d[4];
+      const uint32_t z = load_bits(p.z, row * p.z_sh + (n - 1) * p.z_ss, p.z_dtype);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int key = min(key0 + 64 * k, kb1 - 1);
+        a[k] = load_bits(p.alpha, row * p.a_sh + key * p.a_ss, p.a_dtype);
+        d[k] = load_bits(p.rho, row * p.r_sh + (n - 1 - key) * p.r_ss, p.r_dtype);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        x[k] = fast_exp2((bits_to_f32(a[k], p.a_dtype) + bits_to_f32(d[k], p.r_dtype) - bits_to_f32(z, p.z_dtype)) *
+                         kLog2e) * scale;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int key = key0 + 64 * k;
+      if (key < end) w[f * pitch + key - kb0] = key < kb1 ? x[k] : 0.f;
+    }
+  }
+}
+
+// The keys kb0..kb1-1 of one workgroup, steps of 32 dealt to its waves in
+// turn.  LIVE: the unit has live columns (K is read); FROZEN: it has frozen
+// ones (weights in w, kb0-based).
+template <typename T, int HD, bool LIVE, bool FROZEN>
+__device__ inline void walk(const PagedAttnParams& p, PagedWave<T, HD>& st, const char* kc, const char* vc,
+                            const int32_t* table, float* w, int pitch, int c0, int nl, int nc, int n, int kb0, int kb1,
+                            int wave, int W, int lane) {
   using Tile = PagedTile<T, HD>;
   constexpr int E = Tile::E, NBLK = Tile::NBLK;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = blockDim.x >> 6;
   const int c = lane & 15, g = lane >> 4;
-  int wg = blockIdx.x;
-  const int split = wg % p.n_splits;
-  wg /= p.n_splits;
-  const int u = wg % p.n_units, b = wg / p.n_units;
-  const int c0 = p.unit_c0[u], nc = p.unit_c0[u + 1] - c0, nl = p.unit_live[u];
-
-  const int n_in = p.lengths[b];
-  const int n = n_in < 0 ? 0 : (n_in > p.capacity ? p.capacity : n_in);
-  bool bad = n_in > p.capacity;
-  const int j0 = split * p.chunk, j1 = min(n, j0 + p.chunk);
-  if (split > 0 && j0 >= n) return;  // the merge knows the live ranges from the lengths
-
-  extern __shared__ __align__(16) float lds[];
-  float* sm_ml = lds;                                       // [W][16][2]
-  float* sm_w = lds + W * 32 + wave * 16 * kWPitch;         // [16][kWPitch] of this wave
-  float* sm_o = lds + W * 32 + W * 16 * kWPitch;            // [W][nc][HD + kOPad]
-
   const bool live_col = c < nl;
-  const T* qrow = reinterpret_cast<const T*>(p.q);
-  if (live_col) qrow += b * p.q_sb + p.col_q[c0 + c] * p.q_sh;
-  typename Tile::Query q;
-  Tile::load_q(q, qrow, live_col, g);
-
-  // frozen columns: lane c holds z of column c
-  float zc = 0.f;
-  if (c >= nl && c < nc && p.col_state[c0 + c] == 2 && n > 0 && n <= p.d_S)
-    zc = load_as_f32(p.z, p.col_pat[c0 + c] * p.z_sh + (n - 1) * p.z_ss, p.z_dtype);
-
-  f32x4_t o[NBLK][E];
-#pragma unroll
-  for (int k = 0; k < NBLK; ++k)
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[k][e] = zero4();
-  float m = live_col || c >= nc ? -INFINITY : 0.f, l = 0.f;
-
-  const T* kc = reinterpret_cast<const T*>(p.kc) + p.unit_k[u] * p.k_sh;
-  const T* vc = reinterpret_cast<const T*>(p.vc) + p.unit_v[u] * p.v_sh;
-  const int32_t* table = p.table + b * p.t_sb;
   const int page_mask = (1 << p.page_shift) - 1;
+  const uint32_t k_row = (uint32_t)p.k_st * sizeof(T), v_row = (uint32_t)p.v_st * sizeof(T);
+  const uint32_t k_lane = Tile::k_lane(g), v_lane = Tile::v_lane(c);
+  const uint32_t k_full = c * k_row + k_lane, v_full = 4 * g * v_row + v_lane;
+  const int64_t k_page = p.k_sp * (int64_t)sizeof(T), v_page = p.v_sp * (int64_t)sizeof(T);
+  const int n_it = kb1 - kb0 > 32 * wave ? (kb1 - kb0 - 32 * wave + 32 * W - 1) / (32 * W) : 0;
 
+  // page ids of the wave's next 32 steps, two 16-key tiles each (a page holds
+  // whole tiles), in one load; a step whose second tile lies past the end uses
+  // its first tile's page and rows twice, with weight 0
   int ids = 0;
-  for (int s = wave, it = 0; j0 + 32 * s < j1; s += W, ++it) {
-    const int key0 = j0 + 32 * s;
+  auto load = [&](Tile& tile, int it) {
+    const int key0 = kb0 + 32 * (wave + it * W);
     if ((it & 31) == 0) {
-      // page ids of the next 32 steps, two 16-key tiles each (a page holds
-      // whole tiles); a step whose second tile lies past the end uses its
-      // first tile's page and rows twice, with weight 0
       const int kk = key0 + 32 * W * (lane >> 1);
       ids = 0;
-      if (kk < j1) {
-        const int kt = (lane & 1) && kk + 16 < j1 ? kk + 16 : kk;
+      if (kk < kb1) {
+        const int kt = (lane & 1) && kk + 16 < kb1 ? kk + 16 : kk;
         ids = table[kt >> p.page_shift];
         if (ids < 0 || ids >= p.n_pages) {
-          bad = true;
+          st.bad = true;
           ids = 0;
         }
       }
     }
-    Tile tile;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int page = __builtin_amdgcn_readlane(ids, 2 * (it & 31) + t);
-      const int kt = t && key0 + 16 < j1 ? key0 + 16 : key0;
-      const int row0 = kt & page_mask, last = min(16, j1 - kt) - 1;
-      if (nl > 0)
-        tile.load_k(kc + page * p.k_sp, (uint32_t)(row0 + min(c, last)) * (uint32_t)p.k_st, t, g);
-      const T* vp = vc + page * p.v_sp;
+      const int kt = t && key0 + 16 < kb1 ? key0 + 16 : key0;
+      const int row0 = kt & page_mask, last = min(16, kb1 - kt) - 1;
+      uint32_t k_off = k_full, v_off[4] = {v_full, v_full + v_row, v_full + 2 * v_row, v_full + 3 * v_row};
+      if (last < 15) {  // rows past the end repeat the last one
+        k_off = min(c, last) * k_row + k_lane;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        tile.load_v(vp, (uint32_t)(row0 + min(4 * g + r, last)) * (uint32_t)p.v_st, t, r, c);
+        for (int r = 0; r < 4; ++r) v_off[r] = min(4 * g + r, last) * v_row + v_lane;
+      }
+      if (LIVE) tile.load_k(kc + page * k_page + row0 * k_row, k_off, t);
+      const char* vp = vc + page * v_page + row0 * v_row;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) tile.load_v(vp, v_off[r], t, r);
     }
-    float w[2][4];
-    if (nl > 0) {
+  };
+  auto compute = [&](const Tile& tile, int it) {
+    const int key0 = kb0 + 32 * (wave + it * W);
+    float x[2][4];
+    if (LIVE) {
       f32x4_t sc[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) sc[t] = tile.scores(q, t);
-      float mx = -INFINITY;
+      for (int t = 0; t < 2; ++t) sc[t] = tile.scores(st.q, t);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          w[t][r] = key0 + 16 * t + 4 * g + r < j1 ? sc[t][r] * p.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, w[t][r]);
-        }
-      const float m_new = fmaxf(m, column_max(mx));
+        for (int r = 0; r < 4; ++r) x[t][r] = sc[t][r] * p.scale_log2;
+      if (key0 + 32 > kb1) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (key0 + 16 * t + 4 * g + r >= kb1) x[t][r] = -INFINITY;
+      }
+      float mx = x[0][0];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, x[t][r]);
+      const float m_new = fmaxf(st.m, column_max(mx));
       const float mu = m_new == -INFINITY ? 0.f : m_new;  // nothing above -inf yet: weights 0
-      float corr = fast_exp2(m - mu);
+      float corr = fast_exp2(st.m - mu);
       float sum = 0.f;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          w[t][r] = fast_exp2(w[t][r] - (mu - Tile::kShift));
-          sum += w[t][r];
+          x[t][r] = fast_exp2(x[t][r] - (mu - Tile::kShift));
+          sum += x[t][r];
         }
-      if (live_col) {
-        l = l * corr + sum;
-        m = m_new;
+      if (!FROZEN || live_col) {
+        st.l = st.l * corr + sum;
+        st.m = m_new;
       } else {
         corr = 1.f;
       }
@@ -306,59 +352,138 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedAttnParams p
 #pragma unroll
         for (int k = 0; k < NBLK; ++k)
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[k][e] *= corr;
+          for (int e = 0; e < E; ++e) st.o[k][e] *= corr;
       }
     }
-    if (nl < nc) {
-      // weights of the frozen columns, 32 keys by two columns at a time
-      const int key = key0 + (lane & 31);
-      for (int f0 = nl; f0 < nc; f0 += 2) {
-        const int f = f0 + (lane >> 5), col = c0 + min(f, nc - 1);
-        const int st = p.col_state[col], row = p.col_pat[col];
-        const float z = __shfl(zc, min(f, nc - 1), 64);
-        float x = 0.f;
-        if (f < nc && key < j1) {
-          if (st == 1) {
-            x = n <= p.p_S ? load_as_f32(p.patt, row * p.p_sh + (n - 1) * p.p_si + key * p.p_sj, p.patt_dtype)
-                           : __builtin_nanf("");
-          } else if (n <= p.d_S) {
-            const float a = load_as_f32(p.alpha, row * p.a_sh + key * p.a_ss, p.a_dtype);
-            const float d = load_as_f32(p.rho, row * p.r_sh + (n - 1 - key) * p.r_ss, p.r_dtype);
-            x = fast_exp2((a + d - z) * kLog2e);
-          } else {
-            x = __builtin_nanf("");
-          }
-        }
-        if (f < nc) sm_w[f * kWPitch + (lane & 31)] = x * (Tile::kShift != 0.f ? 256.f : 1.f);
-      }
-      __builtin_amdgcn_wave_barrier();
-      if (!live_col) {
+    if (FROZEN && !live_col) {
+      // columns past the unit's repeat its last one (never written)
+      const float* wr = w + (min(c, nc - 1) - nl) * pitch + (key0 - kb0) + 4 * g;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const float4 x = c < nc ? *reinterpret_cast<const float4*>(sm_w + c * kWPitch + 16 * t + 4 * g)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-          w[t][0] = x.x; w[t][1] = x.y; w[t][2] = x.z; w[t][3] = x.w;
-        }
+      for (int t = 0; t < 2; ++t) {
+        const float4 f = *reinterpret_cast<const float4*>(wr + 16 * t);
+        x[t][0] = f.x; x[t][1] = f.y; x[t][2] = f.z; x[t][3] = f.w;
       }
-      __builtin_amdgcn_wave_barrier();
     }
-    tile.pv(o, w);
+    tile.pv(st.o, x);
+  };
+  // the frozen weights behind the first tile's loads, unless that keeps too many
+  // registers alive; the first barrier also ends the last block's reads
+  constexpr bool kEarly = sizeof(Tile) < 512;
+  Tile ta;
+  if (kEarly && n_it > 0) load(ta, 0);
+  if (FROZEN) {
+    __syncthreads();
+    frozen_weights(p, w, pitch, c0, nl, nc, n, kb0, kb1, wave, W, lane, Tile::kShift != 0.f ? 256.f : 1.f);
+    __syncthreads();
+  }
+  if (n_it == 0) return;
+  if (!kEarly) load(ta, 0);
+  if constexpr (sizeof(Tile) <= 512) {
+    // two tiles in registers: the next step's loads are in flight while a step
+    // is computed.  They are issued without a condition (past the end the last
+    // step again), so that the wait for a tile leaves the next one's loads out.
+    Tile tb;
+    for (int it = 0;;) {
+      load(tb, min(it + 1, n_it - 1));
+      compute(ta, it);
+      if (++it >= n_it) break;
+      load(ta, min(it + 1, n_it - 1));
+      compute(tb, it);
+      if (++it >= n_it) break;
+    }
+  } else {
+    // float32 at hd 256: one tile is half of the registers
+    for (int it = 0;;) {
+      compute(ta, it);
+      if (++it >= n_it) break;
+      load(ta, it);
+    }
+  }
+}
+
+// Keys per range where sequences are cut into n_splits ranges: the longest
+// sequence's share, so that a page table wider than the sequences costs
+// nothing (whole wave, uniform result).
+__device__ inline int range_keys(const PagedAttnParams& p, int lane) {
+  int most = 0;
+  for (int b = lane; b < p.B; b += 64) most = max(most, p.lengths[b]);
+  // in runs of 64 keys, which float32 holds exactly (capacity is at most 2^30)
+  most = min(64 * (int)wave_max((float)((most + 63) >> 6)), p.capacity);
+  const int keys = (most + p.n_splits - 1) / p.n_splits;
+  return max((keys + 127) & ~127, p.chunk);
+}
+
+// Grid: one workgroup per (sequence, unit, key range).
+template <typename T, int HD>
+__global__ __launch_bounds__(64 * paged_max_waves(sizeof(T), HD), paged_simd_waves(sizeof(T), HD)) void paged_attn_kernel(
+    const PagedAttnParams p) {
+  using Tile = PagedTile<T, HD>;
+  constexpr int E = Tile::E, NBLK = Tile::NBLK;
+  const int lane = threadIdx.x & 63, W = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  int wg = blockIdx.x;
+  const int split = wg % p.n_splits;
+  wg /= p.n_splits;
+  const int u = wg % p.n_units, b = wg / p.n_units;
+  const PagedUnit un = p.unit[u];
+  const int c0 = un.c0, nc = un.cols, nl = un.live;
+
+  const int n_in = p.lengths[b];
+  const int n = n_in < 0 ? 0 : (n_in > p.capacity ? p.capacity : n_in);
+  const int chunk = p.n_splits > 1 ? range_keys(p, lane) : p.chunk;
+  const int j0 = split * chunk, j1 = min(n, j0 + chunk);
+  if (split > 0 && j0 >= n) return;  // the join knows the live ranges from the lengths
+
+  extern __shared__ __align__(16) float lds[];
+  float* sm_ml = lds;           // [W][16][2]
+  float* sm_o = lds + W * 32;   // [W][nc][HD + kOPad], before it the frozen weights
+
+  const bool live_col = c < nl;
+  PagedWave<T, HD> st;
+  {
+    const T* qrow = reinterpret_cast<const T*>(p.q);
+    if (live_col) qrow += b * p.q_sb + col_q(p.col[c0 + c]) * p.q_sh;
+    Tile::load_q(st.q, qrow, live_col, g);
+  }
+#pragma unroll
+  for (int k = 0; k < NBLK; ++k)
+#pragma unroll
+    for (int e = 0; e < E; ++e) st.o[k][e] = zero4();
+  st.m = live_col || c >= nc ? -INFINITY : 0.f;
+  st.l = 0.f;
+  st.bad = n_in > p.capacity;
+
+  const char* kc = reinterpret_cast<const char*>(p.kc) + un.k * p.k_sh * (int64_t)sizeof(T);
+  const char* vc = reinterpret_cast<const char*>(p.vc) + un.v * p.v_sh * (int64_t)sizeof(T);
+  const int32_t* table = p.table + b * p.t_sb;
+  if (nl == nc) {
+    walk<T, HD, true, false>(p, st, kc, vc, table, nullptr, 0, c0, nl, nc, n, j0, j1, wave, W, lane);
+  } else {
+    // frozen weights in LDS, for as many keys at a time as fit
+    const int pitch = min(p.w_floats / (nc - nl), chunk) & ~31;
+    for (int kb0 = j0; kb0 < j1; kb0 += pitch) {
+      const int kb1 = min(j1, kb0 + pitch);
+      if (nl > 0) walk<T, HD, true, true>(p, st, kc, vc, table, sm_o, pitch, c0, nl, nc, n, kb0, kb1, wave, W, lane);
+      else walk<T, HD, false, true>(p, st, kc, vc, table, sm_o, pitch, c0, nl, nc, n, kb0, kb1, wave, W, lane);
+    }
+    __syncthreads();
   }
 
   // merge of the workgroup's waves: every wave's column maxima and sums and
   // its partial O in LDS, then each thread four d of one column
-  l = column_sum(l);
-  if (__any(bad)) {
-    l = __builtin_nanf("");
+  st.l = column_sum(st.l);
+  if (__any(st.bad)) {
+    st.l = __builtin_nanf("");
 #pragma unroll
     for (int k = 0; k < NBLK; ++k)
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        o[k][e] = f32x4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        st.o[k][e] = f32x4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
   }
   if (g == 0) {
-    sm_ml[(wave * 16 + c) * 2] = m;
-    sm_ml[(wave * 16 + c) * 2 + 1] = l;
+    sm_ml[(wave * 16 + c) * 2] = st.m;
+    sm_ml[(wave * 16 + c) * 2 + 1] = st.l;
   }
   if (c < nc) {
     float* dst = sm_o + (wave * nc + c) * (HD + kOPad);
@@ -367,10 +492,10 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedAttnParams p
 #pragma unroll
       for (int x = 0; x < E; ++x) {  // elements 4x..4x+3 of the lane's 4E consecutive d
         float4 f;
-        f.x = o[k][(4 * x + 0) % E][(4 * x + 0) / E];
-        f.y = o[k][(4 * x + 1) % E][(4 * x + 1) / E];
-        f.z = o[k][(4 * x + 2) % E][(4 * x + 2) / E];
-        f.w = o[k][(4 * x + 3) % E][(4 * x + 3) / E];
+        f.x = st.o[k][(4 * x + 0) % E][(4 * x + 0) / E];
+        f.y = st.o[k][(4 * x + 1) % E][(4 * x + 1) / E];
+        f.z = st.o[k][(4 * x + 2) % E][(4 * x + 2) / E];
+        f.w = st.o[k][(4 * x + 3) % E][(4 * x + 3) / E];
         *reinterpret_cast<float4*>(dst + 16 * E * k + 4 * E * g + 4 * x) = f;
       }
   }
@@ -397,11 +522,12 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedAttnParams p
       }
       continue;
     }
-    const int h = p.col_head[c0 + col];
-    const float inv = n == 0 && !bad ? 0.f : (col < nl ? 1.f / ll : (Tile::kShift != 0.f ? 1.f / 256.f : 1.f));
+    const int h = col_head(p.col[c0 + col]);
+    const bool empty = n_in <= 0;
+    const float inv = empty ? 0.f : (col < nl ? 1.f / ll : (Tile::kShift != 0.f ? 1.f / 256.f : 1.f));
     acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
     store4(reinterpret_cast<T*>(p.out) + b * p.o_sb + h * p.o_sh + d, acc);
-    if (p.lse && d == 0 && col < nl) p.lse[b * p.l_sb + h * p.l_sh] = n == 0 && !bad ? -INFINITY : mm + log2f(ll) - Tile::kShift;
+    if (p.lse && d == 0 && col < nl) p.lse[b * p.l_sb + h * p.l_sh] = empty ? -INFINITY : mm + log2f(ll) - Tile::kShift;
   }
 }
 
@@ -412,17 +538,25 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   constexpr int L = HD / 4, G = 256 / L;  // hd 96: 10 groups of 24, the rest idle
   __shared__ float4 sm[G][L];
   const int col = blockIdx.x % p.n_heads, b = blockIdx.x / p.n_heads;
-  const int h = p.col_head[col];
-  const bool live = p.col_state[col] == 0;
+  const int64_t word = p.col[col];
+  const int h = col_head(word);
+  const bool live = col_state(word) == 0;
   const int n_in = p.lengths[b];
   const bool bad = n_in > p.capacity;
   const int n = n_in < 0 ? 0 : (bad ? p.capacity : n_in);
-  const int ns = n == 0 ? 0 : (n - 1) / p.chunk + 1;
+  const int lane = threadIdx.x & 63;
+  const int chunk = range_keys(p, lane);
+  const int ns = n == 0 ? 0 : (n - 1) / chunk + 1;
   const int64_t slot = ((int64_t)b * p.n_heads + col) * p.n_splits;
   const float* ml = p.part_ml + 2 * slot;
   float mm = -INFINITY;
-  for (int s = 0; s < ns; ++s) mm = fmaxf(mm, ml[2 * s]);
+  for (int s = lane; s < ns; s += 64) mm = fmaxf(mm, ml[2 * s]);
+  mm = wave_max(mm);
   const float mu = mm == -INFINITY ? 0.f : mm;
+  float ll = 0.f;
+  for (int s = lane; s < ns; s += 64) ll += fast_exp2(ml[2 * s] - mu) * ml[2 * s + 1];
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) ll += __shfl_xor(ll, k, 64);
   const int grp = threadIdx.x / L, d4 = threadIdx.x % L;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (grp < G) {
@@ -435,8 +569,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   }
   __syncthreads();
   if (threadIdx.x >= L) return;
-  float ll = 0.f;
-  for (int s = 0; s < ns; ++s) ll += fast_exp2(ml[2 * s] - mu) * ml[2 * s + 1];
   acc = sm[0][d4];
   for (int k = 1; k < G; ++k) {
     const float4 x = sm[k][d4];
@@ -454,7 +586,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
 
 template <typename T, int HD>
 static hipError_t launch_paged_t(const PagedAttnParams& p, hipStream_t s) {
-  const size_t lds = sizeof(float) * p.waves * (32 + 16 * kWPitch + p.max_cols * (HD + kOPad));
+  const size_t o_floats = (size_t)p.waves * p.max_cols * (HD + kOPad);
+  const size_t lds = sizeof(float) * (p.waves * 32 + (o_floats > (size_t)p.w_floats ? o_floats : (size_t)p.w_floats));
   hipLaunchKernelGGL((paged_attn_kernel<T, HD>), dim3((unsigned)((int64_t)p.B * p.n_units * p.n_splits)),
                      dim3(64 * p.waves), lds, s, p);
   hipError_t e = hipGetLastError();

@@ -72,9 +72,19 @@ int check_vec(const saf_tensor_t& t, const char* name, int64_t n) {
 
 // ---- paged attention ----------------------------------------------------------
 
-// Key ranges: enough workgroups of kWaves waves to fill the device, at least
-// kMinKeys keys each.
-constexpr int kWaves = 4, kMinKeys = 256;
+// Key ranges.  A sequence is cut only where its units leave resident
+// workgroups idle, into as many ranges as fill them (whole rounds cost more
+// than a ragged tail: 64 sequences of up to 4096 keys, 768 units for 768
+// workgroups, 86 us whole, 94 us in two ranges, 106 us in eight), of at least
+// kMinKeys keys, and not below kSplitFrom positions, where the second launch
+// costs what the shorter walk saves (one sequence of 1024 keys: 9.2 us either
+// way and 4.6 us more host time; of 2000 keys in a group of seven: 21 us whole,
+// 11 us cut).  Uncut sequences from kWideFrom positions on run eight waves
+// where the registers allow (64 x 4096 keys: 79 us against 86; 128 x 8192 keys
+// at hd 128: 422 against 442); short ones four (64 x 128 keys: 7.4 us against
+// 12.6, idle waves cost their launch).
+constexpr int kMinKeys = 256, kSplitFrom = 1536, kWideFrom = 2048;
+constexpr int kWeightFloats = 8192;  // 32 KB: four workgroups of a CU still fit its LDS
 
 int plan_paged(const saf_paged_attn_args* a, PagedAttnParams& p, int& dtype, int& hd) {
   if (a == nullptr) return fail(SAF_EINVAL, "args is NULL");
@@ -174,64 +184,60 @@ int plan_paged(const saf_paged_attn_args* a, PagedAttnParams& p, int& dtype, int
 
   // units: without kvidx one head each; with it a KV head's query heads, live
   // ones first, at most 16 columns per unit
-  int nu = 0, col = 0;
+  int nu = 0, col = 0, max_frozen = 0;
   p.max_cols = 1;
-  auto add_col = [&](int h) {
-    p.col_head[col] = (int16_t)h;
-    p.col_state[col] = (int16_t)a->frozen[h];
-    p.col_q[col] = (int16_t)(a->frozen[h] == 0 ? (a->hidx ? a->hidx[h] : h) : 0);
-    p.col_pat[col] = (int16_t)(a->frozen[h] == 1 ? (a->pidx ? a->pidx[h] : h) : h);
-    ++col;
-  };
-  auto open_unit = [&](int k, int v) {
-    p.unit_c0[nu] = (int16_t)col;
-    p.unit_k[nu] = (int16_t)k;
-    p.unit_v[nu] = (int16_t)v;
-    p.unit_live[nu] = 0;
-    ++nu;
+  auto add = [&](int h, bool open, int k, int v) {
+    if (open) p.unit[nu++] = PagedUnit{(int16_t)k, (int16_t)v, (uint8_t)col, 0, 0, 0};
+    PagedUnit& u = p.unit[nu - 1];
+    const int st = a->frozen[h];
+    ++u.cols;
+    u.live += st == 0;
+    if (u.cols > p.max_cols) p.max_cols = u.cols;
+    if (u.cols - u.live > max_frozen) max_frozen = u.cols - u.live;
+    p.col[col++] = col_word(h, st, st == 0 ? (a->hidx ? a->hidx[h] : h) : 0, st == 1 && a->pidx ? a->pidx[h] : h);
   };
   if (a->kvidx == nullptr) {
-    for (int h = 0; h < H; ++h) {
-      open_unit(a->frozen[h] == 0 ? (a->hidx ? a->hidx[h] : h) : 0, h);
-      p.unit_live[nu - 1] = a->frozen[h] == 0;
-      add_col(h);
-    }
+    for (int h = 0; h < H; ++h) add(h, true, a->frozen[h] == 0 ? (a->hidx ? a->hidx[h] : h) : 0, h);
   } else {
     bool done[SAF_MAX_HEADS] = {};
     for (int h0 = 0; h0 < H; ++h0) {
       if (done[h0]) continue;
       const int kv = a->kvidx[h0];
-      int open = 0;
+      bool open = true;
       for (int pass = 0; pass < 2; ++pass)  // live heads, then frozen ones
         for (int h = h0; h < H; ++h) {
           if (a->kvidx[h] != kv || (a->frozen[h] == 0) != (pass == 0)) continue;
           done[h] = true;
-          if (open == 0 || open == 16) {
-            open_unit(kv, kv);
-            open = 0;
-          }
-          ++open;
-          if (open > p.max_cols) p.max_cols = open;
-          p.unit_live[nu - 1] += pass == 0;
-          add_col(h);
+          add(h, open, kv, kv);
+          open = p.unit[nu - 1].cols == 16;
         }
     }
   }
-  p.unit_c0[nu] = (int16_t)col;
   p.n_units = nu;
 
-  p.waves = kWaves;
   if (B > kMaxGrid / SAF_MAX_HEADS / 64) return fail(SAF_EUNSUPPORTED, "batch %lld is too large", (long long)B);
   p.B = (int)B;
+  // key ranges: as many as the resident workgroups leave for each unit
   const int64_t tasks = B * nu;
+  const int64_t slots = (int64_t)cu_count() * paged_simd_waves(elem_size(dtype), hd);
+  int64_t want = tasks > 0 ? slots / tasks : 1;
   const int64_t most = ((int64_t)p.capacity + kMinKeys - 1) / kMinKeys;
-  int64_t want = tasks > 0 ? (4 * (int64_t)cu_count() + tasks - 1) / tasks : 1;
   if (want > most) want = most;
-  if (want < 1) want = 1;
-  const int64_t step = 32 * p.waves;
-  const int64_t chunk = ((p.capacity + want - 1) / want + step - 1) / step * step;
-  p.chunk = (int)(chunk > 0 ? chunk : step);
-  p.n_splits = p.capacity > 0 ? (int)((p.capacity + p.chunk - 1) / p.chunk) : 1;
+  if (p.capacity < kSplitFrom) want = 1;
+  p.n_splits = want > 1 ? (int)want : 1;
+  p.chunk = p.n_splits > 1 ? kMinKeys : (p.capacity + 31) / 32 * 32;
+  if (p.chunk < 32) p.chunk = 32;
+  p.waves = p.n_splits == 1 && p.capacity >= kWideFrom ? paged_max_waves(elem_size(dtype), hd) : 4;
+  // key range of a workgroup at its largest
+  int64_t range = p.n_splits > 1 ? ((p.capacity + p.n_splits - 1) / p.n_splits + 127) / 128 * 128 : p.chunk;
+  if (range < p.chunk) range = p.chunk;
+  // LDS of the frozen columns' weights: a whole key range where that is within
+  // kWeightFloats, at least one step per column
+  if (max_frozen > 0) {
+    int64_t keys = kWeightFloats / max_frozen / 32 * 32;
+    if (keys > range) keys = range;
+    p.w_floats = (int)keys * max_frozen;
+  }
   return SAF_OK;
 }
 
@@ -388,6 +394,10 @@ int saf_paged_append(const saf_paged_append_args* a, void* stream) {
       return fail(SAF_EUNSUPPORTED, "rotary dimension %lld is not a multiple of 16 up to the head dimension", (long long)rd);
     p.cos = a->cos.data; p.sin = a->sin.data; p.cs_st = a->cos.stride[0]; p.sn_st = a->sin.stride[0];
     p.cs_dtype = a->cos.dtype; p.cs_rows = (int)a->cos.size[0]; p.rd = (int)rd;
+    auto al = [](const saf_tensor_t& t) {
+      return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && (t.size[0] <= 1 || t.stride[0] * elem_size(t.dtype) % 16 == 0);
+    };
+    p.cs_vec = al(a->cos) && al(a->sin);
   }
   if (present(a->q_weight) != present(a->k_weight)) return fail(SAF_EINVAL, "q_weight and k_weight go together");
   if (present(a->q_weight)) {
@@ -396,6 +406,7 @@ int saf_paged_append(const saf_paged_append_args* a, void* stream) {
     if (a->q_weight.dtype != a->k_weight.dtype) return fail(SAF_EINVAL, "q_weight and k_weight must share a dtype");
     if (!(a->eps >= 0.f)) return fail(SAF_EINVAL, "eps must be a non-negative number");
     p.q_w = a->q_weight.data; p.k_w = a->k_weight.data; p.w_dtype = a->q_weight.dtype; p.eps = a->eps;
+    p.w_vec = (reinterpret_cast<uintptr_t>(p.q_w) | reinterpret_cast<uintptr_t>(p.k_w)) % 16 == 0;
   }
   if (B > 65535 || T > (int64_t(1) << 20)) return fail(SAF_EUNSUPPORTED, "paged_append: at most 65535 sequences and 2^20 tokens");
   p.v = v.data; p.v_sb = v.stride[0]; p.v_sh = v.stride[1]; p.v_st = v.stride[2];

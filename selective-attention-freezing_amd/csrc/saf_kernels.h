@@ -208,10 +208,30 @@ struct ProjGemmParams {
   int64_t cs_st, sn_st;
 };
 
+// Waves per SIMD that the paged attention kernel's registers leave (its launch
+// bound) and the largest workgroup, by element size and head dim.
+constexpr int paged_simd_waves(int es, int hd) {
+  return es == 2 ? (hd == 32 ? 5 : (hd == 64 ? 3 : (hd <= 128 ? 2 : 1))) : (hd == 32 ? 4 : (hd == 64 ? 2 : 1));
+}
+constexpr int paged_max_waves(int es, int hd) { return paged_simd_waves(es, hd) >= 2 ? 8 : 4; }
+
 // Single-token attention over a paged cache (paged_attn.hip).  Columns are the
-// query heads in unit order: unit u covers columns unit_c0[u]..unit_c0[u+1]-1
-// (at most 16, its unit_live[u] live heads first), which share key head
-// unit_k[u] and value head unit_v[u].
+// query heads in unit order: a unit covers the columns c0..c0 + cols - 1 (at
+// most 16, its live heads first), which share key head k and value head v.
+struct PagedUnit {
+  int16_t k, v;
+  uint8_t c0, cols, live, pad;
+};
+// A column: natural head, state, q slot, pattern row (dense) or buffer row
+// (decomposed), in one word.
+inline int64_t col_word(int head, int state, int q, int pat) {
+  return (int64_t)head | (int64_t)state << 8 | (int64_t)q << 16 | (int64_t)pat << 32;
+}
+__host__ __device__ inline int col_head(int64_t w) { return (int)(w & 0xff); }
+__host__ __device__ inline int col_state(int64_t w) { return (int)(w >> 8 & 0xff); }
+__host__ __device__ inline int col_q(int64_t w) { return (int)(w >> 16 & 0x7fff); }
+__host__ __device__ inline int col_pat(int64_t w) { return (int)(w >> 32); }
+
 struct PagedAttnParams {
   const void* q;
   const void* kc;
@@ -226,7 +246,10 @@ struct PagedAttnParams {
   int64_t t_sb;
   const int32_t* lengths;
   int page_shift, n_pages, capacity;  // capacity = page_table columns x page size
-  int B, n_heads, n_units, n_splits, chunk, waves, max_cols;
+  int B, n_heads, n_units, waves, max_cols;
+  int n_splits;  // key ranges per sequence
+  int chunk;     // n_splits 1: the capacity; else the least keys of a range
+  int w_floats;  // LDS floats for the frozen columns' weights (0: no frozen column)
   float scale_log2;
   float* part_o;   // [B][n_heads][n_splits][HD] (by column), n_splits > 1
   float* part_ml;  // [B][n_heads][n_splits][2]
@@ -238,14 +261,8 @@ struct PagedAttnParams {
   const void* z;
   int a_dtype, r_dtype, z_dtype, d_S;
   int64_t a_sh, a_ss, r_sh, r_ss, z_sh, z_ss;
-  int16_t unit_c0[kMaxHeads + 2];
-  int16_t unit_live[kMaxHeads];
-  int16_t unit_k[kMaxHeads];
-  int16_t unit_v[kMaxHeads];
-  int16_t col_head[kMaxHeads];
-  int16_t col_q[kMaxHeads];
-  int16_t col_pat[kMaxHeads];   // dense: pattern row; decomposed: buffer row
-  int16_t col_state[kMaxHeads];
+  PagedUnit unit[kMaxHeads];
+  int64_t col[kMaxHeads];
 };
 static_assert(sizeof(PagedAttnParams) <= 4096, "PagedAttnParams must fit the kernel argument segment");
 
@@ -270,7 +287,8 @@ struct PagedAppendParams {
   const void* sin;
   int64_t cs_st, sn_st;
   int cs_dtype, cs_rows, rd;
-  const void* q_w;  // null: no norm
+  int cs_vec, w_vec;  // rows 16-byte aligned
+  const void* q_w;    // null: no norm
   const void* k_w;
   int w_dtype;
   float eps;
