@@ -432,7 +432,8 @@ typedef struct saf_token_logprobs_args {
   saf_tensor_t tokens;     /* (R,) int32 or int64 */
   saf_tensor_t logp;       /* (R,) fp32 */
   saf_tensor_t entropy;    /* optional (R,) fp32 */
-  saf_tensor_t stats;      /* (R, 2) fp32, contiguous: the largest logit, log2 of the sum relative to it */
+  saf_tensor_t stats;      /* (R, 2) fp32, contiguous: the largest logit, log2 of the sum relative to it;
+                              optional in the forward, read by the backward */
   saf_tensor_t top_index;  /* with top > 0: (R, top) int64 */
   saf_tensor_t top_logp;   /* with top > 0: (R, top) fp32 */
   int32_t top;             /* alternatives per row, 0..32 and at most V */

@@ -258,8 +258,9 @@ int plan_logprobs(const saf_token_logprobs_args* a, LogprobParams& p, bool outpu
   if (V > 1 && x.stride[1] != 1) return fail(SAF_EALIGN, "logits need a unit column stride");
   if (t.ndim != 1 || t.size[0] != R || (t.dtype != SAF_I32 && t.dtype != SAF_I64) || (R > 0 && !present(t)))
     return fail(SAF_EINVAL, "tokens must be int32 or int64 with one entry per row");
-  if (st.ndim != 2 || st.size[0] != R || st.size[1] != 2 || st.dtype != SAF_F32 || (R > 0 && !present(st)) ||
-      (R > 0 && (st.stride[1] != 1 || (R > 1 && st.stride[0] != 2))))
+  if (R > 0 && !outputs && !present(st)) return fail(SAF_EINVAL, "the forward's stats are required");
+  if (present(st) && (st.ndim != 2 || st.size[0] != R || st.size[1] != 2 || st.dtype != SAF_F32 || st.stride[1] != 1 ||
+                      (R > 1 && st.stride[0] != 2)))
     return fail(SAF_EINVAL, "stats must be contiguous fp32 (R, 2)");
   if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(SAF_EINVAL, "scale must be positive and finite");
   if (a->top < 0 || a->top > 32 || a->top > V)
@@ -294,12 +295,16 @@ int plan_logprobs(const saf_token_logprobs_args* a, LogprobParams& p, bool outpu
   p.top_index = reinterpret_cast<int64_t*>(a->top_index.data);
   p.top_logp = reinterpret_cast<float*>(a->top_logp.data);
   p.n_cu = cu_count();
-  // segments: rows enough for two workgroups per CU stay whole; shorter
-  // segments than 8192 elements are not worth the join
-  int64_t seg = R > 0 ? (2 * (int64_t)p.n_cu + R - 1) / R : 1;
-  const int64_t most = (V + 8191) / 8192;
-  if (seg > most) seg = most;
-  if (seg > 64) seg = 64;
+  // few long rows (256 KB and more) are cut into segments of at least 16 KB, one
+  // workgroup each: one CU reads about 55 GB/s (4 rows of 151936: 10 us with the
+  // join, 16 us whole; shorter rows do not pay for the second launch)
+  const int64_t row_bytes = V * elem_size(x.dtype);
+  int64_t seg = 1;
+  if (R > 0 && R <= p.n_cu / 4 && row_bytes >= (256 << 10)) {
+    seg = 2 * (int64_t)p.n_cu / R;
+    if (seg > row_bytes >> 14) seg = row_bytes >> 14;
+    if (seg > 64) seg = 64;
+  }
   const int64_t len = ((V + seg - 1) / seg + 63) / 64 * 64;
   p.seg_len = (int)(seg == 1 ? V : len);
   p.n_seg = seg == 1 ? 1 : (int)((V + len - 1) / len);

@@ -307,7 +307,7 @@ struct LogprobParams {
   float scale;
   float* logp;
   float* entropy;   // null: none
-  float* stats;     // (R, 2)
+  float* stats;     // (R, 2), null: none
   int64_t* top_index;
   float* top_logp;
   int top;

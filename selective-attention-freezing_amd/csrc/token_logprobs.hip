@@ -24,7 +24,8 @@
 namespace saf {
 
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kCand = 1024;  // collected elements; more (adversarial rows) take the slow selection
+// collected elements; more (adversarial rows) take the slow selection
+constexpr int cand_room(int nt) { return nt == 64 ? 256 : 1024; }
 
 template <typename T> struct Chunk {
   static constexpr int N = 8;
@@ -61,29 +62,69 @@ __device__ inline uint32_t value_key(float v) {
 __device__ inline float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ inline uint64_t order_key(float v, uint32_t pos) { return (uint64_t)value_key(v) << 32 | (uint32_t)~pos; }
 
-__device__ inline uint64_t shfl_xor64(uint64_t x, int m) {
-  const uint32_t lo = __shfl_xor((uint32_t)x, m, 64), hi = __shfl_xor((uint32_t)(x >> 32), m, 64);
-  return (uint64_t)hi << 32 | lo;
+// The value of lane ^ M, by moves inside the vector unit (an LDS shuffle takes
+// several times as long, and the sorts below are chains of them).
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_u32(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);
 }
-__device__ inline uint64_t wave_max64(uint64_t x) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) {
-    const uint64_t y = shfl_xor64(x, m);
-    x = y > x ? y : x;
+template <int M> __device__ __forceinline__ uint32_t lane_xor(uint32_t x, int lane) {
+  if constexpr (M == 1) return dpp_u32<0xb1>(x);                  // quad_perm [1, 0, 3, 2]
+  if constexpr (M == 2) return dpp_u32<0x4e>(x);                  // quad_perm [2, 3, 0, 1]
+  if constexpr (M == 4) return dpp_u32<0x1b>(dpp_u32<0x141>(x));  // row_half_mirror, quad_perm [3, 2, 1, 0]
+  if constexpr (M == 8) return dpp_u32<0x128>(x);                 // row_ror:8
+  if constexpr (M == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return lane & 16 ? r[0] : r[1];
   }
+  if constexpr (M == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return lane & 32 ? r[0] : r[1];
+  }
+}
+template <int M> __device__ __forceinline__ uint64_t lane_xor64(uint64_t x, int lane) {
+  return (uint64_t)lane_xor<M>((uint32_t)(x >> 32), lane) << 32 | lane_xor<M>((uint32_t)x, lane);
+}
+// One exchange of a bitonic sort: the lane keeps the larger key where want_max.
+template <int M> __device__ __forceinline__ uint64_t exchange(uint64_t x, int lane, bool want_max) {
+  const uint64_t y = lane_xor64<M>(x, lane);
+  return (y > x) == want_max ? y : x;
+}
+// Descending (ascending where !down) order of bitonic runs of 2 M keys.
+template <int M> __device__ __forceinline__ uint64_t merge_runs(uint64_t x, int lane, bool down) {
+  x = exchange<M>(x, lane, ((lane & M) == 0) == down);
+  if constexpr (M > 1) x = merge_runs<M / 2>(x, lane, down);
   return x;
 }
-// The wave's 64 keys in descending order by lane (bitonic).
-__device__ inline uint64_t wave_sort_desc(uint64_t x, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const uint64_t y = shfl_xor64(x, j);
-      const bool want_max = ((lane & k) == 0) == ((lane & j) == 0);
-      x = (y > x) == want_max ? y : x;
-    }
+template <int M> __device__ __forceinline__ uint64_t wave_max64_step(uint64_t x, int lane) {
+  x = exchange<M>(x, lane, true);
+  if constexpr (M > 1) x = wave_max64_step<M / 2>(x, lane);
   return x;
+}
+__device__ inline uint64_t wave_max64(uint64_t x, int lane) { return wave_max64_step<32>(x, lane); }
+
+// Sum over the wave's 64 lanes, the moves of wave_max with zeros where a row
+// does not take part.
+template <int CTRL, int ROWMASK> __device__ __forceinline__ float dpp_add(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWMASK, 0xf, false));
+}
+__device__ inline float wave_sum(float x) {
+  x = dpp_add<0xb1, 0xf>(x);
+  x = dpp_add<0x4e, 0xf>(x);
+  x = dpp_add<0x141, 0xf>(x);
+  x = dpp_add<0x140, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);
+  x = dpp_add<0x143, 0xc>(x);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+// Descending order of a bitonic sequence over the lanes, and of any keys.
+__device__ inline uint64_t wave_merge_desc(uint64_t x, int lane) { return merge_runs<32>(x, lane, true); }
+__device__ inline uint64_t wave_sort_desc(uint64_t x, int lane) {
+  x = merge_runs<1>(x, lane, (lane & 2) == 0);
+  x = merge_runs<2>(x, lane, (lane & 4) == 0);
+  x = merge_runs<4>(x, lane, (lane & 8) == 0);
+  x = merge_runs<8>(x, lane, (lane & 16) == 0);
+  x = merge_runs<16>(x, lane, (lane & 32) == 0);
+  return merge_runs<32>(x, lane, true);
 }
 
 // Exponents x' - M of one row or thread, M = m log2 e scale.  Where M is far
@@ -116,14 +157,6 @@ struct Sums {
     s *= f;
     m = m_new;
   }
-  template <bool ENT> __device__ inline void merge(const Sums& o, float sl2) {
-    Sums b = o;
-    const float mm = fmaxf(m, b.m);
-    raise<ENT>(mm, sl2);
-    b.raise<ENT>(mm, sl2);
-    s += b.s;
-    t += b.t;
-  }
   // one element that does not exceed m, with its exponent
   template <bool ENT> __device__ inline void add(float v) {
     const float e = fast_exp2(v);
@@ -141,12 +174,11 @@ struct Sums {
     }
   }
 };
-template <bool ENT> __device__ inline Sums shfl_xor_sums(const Sums& a, int m) {
-  Sums b;
-  b.m = __shfl_xor(a.m, m, 64);
-  b.s = __shfl_xor(a.s, m, 64);
-  if (ENT) b.t = __shfl_xor(a.t, m, 64);
-  return b;
+// The sums of a whole wave: one common maximum, then plain sums.
+template <bool ENT> __device__ inline void wave_merge(Sums& a, float sl2) {
+  a.raise<ENT>(wave_max(a.m), sl2);
+  a.s = wave_sum(a.s);
+  if (ENT) a.t = wave_sum(a.t);
 }
 
 __device__ inline int64_t token_of(const LogprobParams& p, int64_t r) {
@@ -169,8 +201,10 @@ template <typename T>
 __device__ inline void write_row(const LogprobParams& p, int64_t row, const Sums& a, float sl2) {
   const Anchor c(a.m, sl2);
   const float lg = a.s > 0.f ? log2f(a.s) : __builtin_nanf("");
-  p.stats[2 * row] = c.m;
-  p.stats[2 * row + 1] = lg;
+  if (p.stats) {
+    p.stats[2 * row] = c.m;
+    p.stats[2 * row + 1] = lg;
+  }
   const int64_t tok = token_of(p, row);
   float lp = 0.f;
   if (tok != p.ignore) {
@@ -216,21 +250,30 @@ __global__ __launch_bounds__(NT) void logprob_kernel(const LogprobParams p) {
     a.add<ENT>(Anchor(a.m, sl2).exponent(f));
   };
   if (tid < head) single(tid);
-  int k = tid;
-  for (; k + (U - 1) * NT < nv; k += U * NT) {
-    uint4 r[U];
+  // groups of U pieces per thread, the next group's loads in flight while one is
+  // summed; pieces past the end are -inf (no weight, never a new maximum)
+  auto load = [&](uint4 (&r)[U], int k) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) r[u] = xv[k + u * NT];
+    for (int u = 0; u < U; ++u) r[u] = xv[min(k + u * NT, nv - 1)];
+  };
+  auto sum = [&](const uint4 (&r)[U], int k) {
     float f[U][N], cm[U], gm = -INFINITY;
+    const bool whole = k - tid + U * NT <= nv;  // the whole block's group
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      cm[u] = -INFINITY;
+      if (k - tid + u * NT >= nv) break;  // nothing left for any thread
       C::unpack(r[u], f[u]);
+      if (!whole && k + u * NT >= nv) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[u][e] = -INFINITY;
+      }
       cm[u] = f[u][0];
 #pragma unroll
       for (int e = 1; e < N; ++e) cm[u] = fmaxf(cm[u], f[u][e]);
       gm = fmaxf(gm, cm[u]);
     }
-    if (TOP && best == 0xffffffffu) best = head + k * N;
+    if (TOP && best == 0xffffffffu && k < nv) best = head + k * N;
     if (gm > a.m) {
       a.raise<ENT>(gm, sl2);
       if (TOP) {
@@ -240,28 +283,29 @@ __global__ __launch_bounds__(NT) void logprob_kernel(const LogprobParams p) {
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) a.add_all<ENT>(f[u], sl2);
-  }
-  for (; k < nv; k += NT) {
-    float f[N];
-    C::unpack(xv[k], f);
-    float cm = f[0];
-#pragma unroll
-    for (int e = 1; e < N; ++e) cm = fmaxf(cm, f[e]);
-    if (TOP && best == 0xffffffffu) best = head + k * N;
-    if (cm > a.m) {
-      a.raise<ENT>(cm, sl2);
-      if (TOP) best = head + k * N;
+    for (int u = 0; u < U; ++u)
+      if (k - tid + u * NT < nv) a.add_all<ENT>(f[u], sl2);
+  };
+  if (nv > 0) {
+    uint4 ra[U], rb[U];
+    load(ra, tid);
+    for (int k = tid;;) {
+      load(rb, k + U * NT);
+      sum(ra, k);
+      k += U * NT;
+      if (k - tid >= nv) break;
+      load(ra, k + U * NT);
+      sum(rb, k);
+      k += U * NT;
+      if (k - tid >= nv) break;
     }
-    a.add_all<ENT>(f, sl2);
   }
   if (tail0 + tid < n) single(tail0 + tid);
   const uint64_t mykey = TOP && best != 0xffffffffu ? order_key(a.m, best) : 0;
 
-  // the block's sums, in every thread of wave 0
+  // the block's sums (with TOP in every thread)
   __shared__ float sm_a[W][3];
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) a.merge<ENT>(shfl_xor_sums<ENT>(a, m), sl2);
+  wave_merge<ENT>(a, sl2);
   if constexpr (W > 1) {
     if (lane == 0) {
       sm_a[wave][0] = a.m;
@@ -269,8 +313,10 @@ __global__ __launch_bounds__(NT) void logprob_kernel(const LogprobParams p) {
       sm_a[wave][2] = a.t;
     }
     __syncthreads();
-    a = Sums{sm_a[0][0], sm_a[0][1], sm_a[0][2]};
-    for (int w = 1; w < W; ++w) a.merge<ENT>(Sums{sm_a[w][0], sm_a[w][1], sm_a[w][2]}, sl2);
+    if (!TOP && wave != 0) return;
+    a = Sums{};
+    if (lane < W) a = Sums{sm_a[lane][0], sm_a[lane][1], sm_a[lane][2]};
+    wave_merge<ENT>(a, sl2);
   }
   const int64_t part = row * p.n_seg + seg;
   if (tid == 0) {
@@ -284,35 +330,35 @@ __global__ __launch_bounds__(NT) void logprob_kernel(const LogprobParams p) {
   }
   if constexpr (!TOP) return;
 
-  __shared__ uint64_t sm_key[W][32];
+  constexpr int kCand = cand_room(NT);
   __shared__ uint64_t sm_cand[kCand];
   __shared__ int sm_win[32];
-  __shared__ uint64_t sm_tau;
   __shared__ int sm_nwin, sm_ncand;
   const int K = p.top;
-  {
-    const uint64_t sorted = wave_sort_desc(mykey, lane);
-    if (lane < K) sm_key[wave][lane] = sorted;
-    if (tid == 0) sm_nwin = sm_ncand = 0;
+  if (tid == 0) sm_nwin = sm_ncand = 0;
+  // tau, the K-th largest thread key (0: fewer than K threads hold elements)
+  uint64_t keys = wave_sort_desc(mykey, lane);
+  if constexpr (W > 1) {
+    __shared__ uint64_t sm_key[W][32];
+    __shared__ uint64_t sm_tau;
+    if (lane < 32) sm_key[wave][lane] = keys;
     __syncthreads();
     if (wave == 0) {
-      // merge of the waves' lists: lane w holds the head of list w
-      uint64_t tau = 0;
-      int at = 0;
-      uint64_t head_key = lane < W ? sm_key[lane < W ? lane : 0][0] : 0;
-      for (int i = 0; i < K; ++i) {
-        tau = wave_max64(head_key);
-        if (tau == 0) break;
-        if (head_key == tau) {
-          ++at;
-          head_key = at < K ? sm_key[lane][at] : 0;
-        }
+      // the waves' lists one after the other behind the largest 32 so far, in
+      // reverse: a bitonic sequence
+      for (int w = 1; w < W; ++w) {
+        if (lane >= 32) keys = sm_key[w][63 - lane];
+        keys = wave_merge_desc(keys, lane);
       }
-      if (lane == 0) sm_tau = tau;  // 0: fewer than K threads hold elements
+      if (lane == K - 1) sm_tau = keys;
     }
     __syncthreads();
+    keys = sm_tau;
+  } else {
+    __syncthreads();
+    keys = (uint64_t)__shfl((uint32_t)(keys >> 32), K - 1, 64) << 32 | __shfl((uint32_t)keys, K - 1, 64);
   }
-  const uint64_t tau = sm_tau;
+  const uint64_t tau = keys;
   const bool win = mykey != 0 && mykey >= tau;
   // with tau = 0 (short segments) every element is collected below
   if (win && tau != 0) sm_win[atomicAdd(&sm_nwin, 1)] = tid;
@@ -363,7 +409,7 @@ __global__ __launch_bounds__(NT) void logprob_kernel(const LogprobParams p) {
         const uint64_t key = order_key(elem_f32(x + j), v0 + j);
         if (key < last && key > bk) bk = key;
       }
-      bk = wave_max64(bk);
+      bk = wave_max64(bk, lane);
       __syncthreads();
       if (lane == 0) sm_cand[wave] = bk;
       __syncthreads();
@@ -387,13 +433,12 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(const LogprobParams p)
     a.s = p.part[4 * part + 1];
     a.t = p.part[4 * part + 2];
   }
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) a.merge<ENT>(shfl_xor_sums<ENT>(a, m), sl2);
+  wave_merge<ENT>(a, sl2);
   if (lane == 0) write_row<T>(p, row, a, sl2);
   int at = 0;
   uint64_t head = p.top > 0 && lane < p.n_seg ? p.part_top[part * p.top] : 0;
   for (int i = 0; i < p.top; ++i) {
-    const uint64_t best = wave_max64(head);
+    const uint64_t best = wave_max64(head, lane);
     if (head == best && best != 0) {
       write_top(p, row, i, best, a, sl2);
       ++at;
@@ -484,8 +529,17 @@ static hipError_t launch_logprob_nt(const LogprobParams& p, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Threads per row (or segment): one wave where a row is at most eight pieces per
+// lane (4096 rows of 4000, top 10: 12 us against 21 with 256 threads, whose
+// barriers cost more than the row), 512 where a row has a CU to itself (200 rows
+// of 151936: 18 us against 22), else 256 (8192 rows of 50304, top 10: 165 us
+// against 182 with 512; with one wave the second look at the top threads' pieces
+// is a long chain, 243).
 template <typename T> static hipError_t launch_logprob_t(const LogprobParams& p, hipStream_t s) {
-  return p.seg_len <= 64 * Chunk<T>::N * 4 ? launch_logprob_nt<T, 64>(p, s) : launch_logprob_nt<T, 256>(p, s);
+  const int pieces = p.seg_len / Chunk<T>::N;
+  if (pieces <= 512) return launch_logprob_nt<T, 64>(p, s);
+  if (pieces >= 4096 && p.R * p.n_seg <= p.n_cu) return launch_logprob_nt<T, 512>(p, s);
+  return launch_logprob_nt<T, 256>(p, s);
 }
 
 hipError_t launch_token_logprobs(const LogprobParams& p, int dtype, hipStream_t s) {

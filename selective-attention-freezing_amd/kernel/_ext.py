@@ -226,17 +226,35 @@ def fill(block, **tensors):
             _DESC.pack_into(block, offset[name], *_desc_values(t))
 
 
+def fill_rows(block, name, t):
+    """fill() of a (B, U, T, HD) tensor that is only read, as a copy where its
+    rows are not 16-byte aligned; returns what the block points to."""
+    v = _desc_values(t)
+    mask = 3 if v[1] == SAF_F32 else 7
+    if (v[0] & 15 or v[10] != 1 or (v[3] > 1 and v[7] & mask) or (v[4] > 1 and v[8] & mask)
+            or (v[5] > 1 and v[9] & mask)):
+        t = t.clone(memory_format=torch.contiguous_format)
+        v = _desc_values(t)
+    _DESC.pack_into(block, _OFFSETS[type(block)][name], *v)
+    return t
+
+
 _OFFSETS = {c: {n: getattr(c, n).offset for n, kind in c._fields_ if kind is SafTensor}
             for c in (SafPagedAppendArgs, SafPagedAttnArgs, SafTokenLogprobsArgs)}
 
 
-def same_device(what, device, **tensors):
-    """Raise unless every given tensor lives on `device`, a HIP device."""
+def check_inputs(what, device, tensors, differentiable=False):
+    """Raise unless every given tensor lives on `device`, a HIP device, and,
+    for an operator without a backward, needs no gradient."""
     if device.type != "cuda":
         raise RuntimeError(f"{what} runs on HIP devices only (got a CPU tensor)")
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
+    grad = not differentiable and torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None:
+            if t.device != device:
+                raise ValueError(f"{what}: a tensor is on {t.device}, expected {device}")
+            if grad and t.requires_grad:
+                raise NotImplementedError(f"{what} has no backward: call it under torch.no_grad()")
 
 
 class _NoGuard:

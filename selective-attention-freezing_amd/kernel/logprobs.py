@@ -23,10 +23,11 @@ class TokenLogprobs(NamedTuple):
     top_logp: Optional[torch.Tensor]    # (..., top) fp32
 
 
-def _forward(logits, tokens, top, entropy, scale, ignore_index):
+def _forward(logits, tokens, top, entropy, scale, ignore_index, keep_stats):
     R, dev = logits.size(0), logits.device
     f32 = dict(device=dev, dtype=torch.float32)
-    logp, stats = torch.empty(R, **f32), torch.empty(R, 2, **f32)
+    logp = torch.empty(R, **f32)
+    stats = torch.empty(R, 2, **f32) if keep_stats else None
     ent = torch.empty(R, **f32) if entropy else None
     idx = torch.empty(R, top, device=dev, dtype=torch.int64) if top else None
     tlp = torch.empty(R, top, **f32) if top else None
@@ -49,7 +50,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, top, entropy, scale, ignore_index):
-        logp, ent, idx, tlp, stats = _forward(logits, tokens, top, entropy, scale, ignore_index)
+        logp, ent, idx, tlp, stats = _forward(logits, tokens, top, entropy, scale, ignore_index, True)
         ctx.save_for_backward(logits, tokens, stats, ent)
         ctx.scale, ctx.ignore_index = scale, ignore_index
         ctx.set_materialize_grads(False)
@@ -98,16 +99,20 @@ def token_logprobs(logits, tokens, top=0, entropy=False, scale=1.0, ignore_index
     if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens must have the logits' leading shape (got {tuple(tokens.shape)} for "
                          f"{tuple(logits.shape)})")
-    _ext.same_device("token_logprobs", logits.device, tokens=tokens)
+    _ext.check_inputs("token_logprobs", logits.device, (tokens,), differentiable=True)
     top, scale = int(top), float(scale)
-    lead, V = tokens.shape, logits.size(-1)
-    x = logits.reshape(-1, V)
-    if V > 1 and x.stride(1) != 1:
+    x, t = logits, tokens
+    if x.dim() != 2:
+        x, t = x.reshape(-1, x.size(-1)), t.reshape(-1)
+    if x.stride(1) != 1 and x.size(1) > 1:
         x = x.contiguous()
-    t = tokens.reshape(-1)
     if torch.is_grad_enabled() and logits.requires_grad:
         logp, ent, idx, tlp = _TokenLogprobsFn.apply(x, t, top, bool(entropy), scale, int(ignore_index))
     else:
-        logp, ent, idx, tlp, _ = _forward(x, t, top, bool(entropy), scale, int(ignore_index))
-    return TokenLogprobs(logp.view(lead), None if ent is None else ent.view(lead),
-                         None if idx is None else idx.view(*lead, top), None if tlp is None else tlp.view(*lead, top))
+        logp, ent, idx, tlp, _ = _forward(x, t, top, entropy, scale, int(ignore_index), False)
+    if logits.dim() != 2:
+        lead = tokens.shape
+        logp = logp.view(lead)
+        ent = None if ent is None else ent.view(lead)
+        idx, tlp = (None, None) if idx is None else (idx.view(*lead, top), tlp.view(*lead, top))
+    return TokenLogprobs(logp, ent, idx, tlp)

@@ -23,11 +23,6 @@ from . import _ext
 from .fused_attn import _table, decomposed_logz
 
 
-def _no_grad_only(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError(f"{what} has no backward: call it under torch.no_grad()")
-
-
 def paged_append_(k, v, k_cache, v_cache, page_table, positions, counts=None, q=None, cos=None, sin=None,
                   q_weight=None, k_weight=None, eps=1e-6):
     """Write T new tokens per sequence into the caches, in place, rotating
@@ -49,52 +44,42 @@ def paged_append_(k, v, k_cache, v_cache, page_table, positions, counts=None, q=
     fp32 arithmetic, one rounding.  A token whose position lies outside the
     page table or the cos / sin caches, or whose page id is not a page of the
     caches, is not written, and its rows of q are NaN."""
-    _no_grad_only("paged_append_", q, k, v, k_cache, v_cache)
+    dev = v.device
     if (k is None) != (k_cache is None):
         raise ValueError("k and k_cache go together")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
-    dev = v.device
-    if cos is not None:
-        cos = cos.reshape(-1, cos.size(-1))
-        sin = sin.reshape(-1, sin.size(-1))
-    _ext.same_device("paged_append_", dev, k=k, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
-                     positions=positions, counts=counts, q=q, cos=cos, sin=sin, q_weight=q_weight, k_weight=k_weight)
-    if k is not None and k.size(1) == 0:
-        k = k_cache = None
-    q_in, k_in, v_in = (_rows16(t) for t in (q, k, v))
+    _ext.check_inputs("paged_append_", dev, (q, k, v, k_cache, v_cache, page_table, positions, counts, cos, sin))
+    _ext.check_inputs("paged_append_", dev, (q_weight, k_weight), differentiable=True)  # module parameters
     out = None
     if q is not None:
         # token-major like the projection it came from, so that a token's rows
         # follow each other
         B, U, T, HD = q.shape
-        out = torch.empty((B, T, U, HD), device=dev, dtype=q.dtype).transpose(1, 2)
+        out = torch.empty_strided((B, U, T, HD), (T * U * HD, HD, U * HD, 1), device=dev, dtype=q.dtype)
+        if U == 0:
+            q = None
     if v.numel() == 0:
         return out
+    if k is not None and k.size(1) == 0:
+        k = None
+    if cos is not None and cos.dim() != 2:
+        cos, sin = cos.reshape(-1, cos.size(-1)), sin.reshape(-1, sin.size(-1))
     args = _ext.SafPagedAppendArgs()
-    _ext.fill(args, q=q_in, k=k_in, v=v_in, q_out=out, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
-              positions=positions, counts=counts, cos=cos, sin=sin,
-              q_weight=None if q_weight is None else q_weight.detach(),
-              k_weight=None if k_weight is None else k_weight.detach())
-    if q is not None and q.numel() == 0:
-        args.q.data = None
-    args.eps = float(eps)
+    _ext.fill(args, k_cache=k_cache if k is not None else None, v_cache=v_cache, page_table=page_table,
+              positions=positions, counts=counts, cos=cos, sin=sin, q_weight=q_weight, k_weight=k_weight)
+    held = [_ext.fill_rows(args, "v", v)]
+    if k is not None:
+        held.append(_ext.fill_rows(args, "k", k))
+    if q is not None:
+        held.append(_ext.fill_rows(args, "q", q))
+        _ext.fill(args, q_out=out)
+    args.eps = eps
     with _ext.on_device(dev):
         rc = _ext.lib().saf_paged_append(args, _ext.current_stream_ptr(dev))
     if rc:
         _ext.check(rc)
     return out
-
-
-def _rows16(t):
-    """t, or a copy whose (B, U, T, HD) rows are 16-byte aligned (rows may
-    overlap or repeat: they are only read)."""
-    if t is None:
-        return None
-    es = t.element_size()
-    ok = t.data_ptr() % 16 == 0 and (t.size(-1) == 1 or t.stride(-1) == 1) and all(
-        n <= 1 or (s * es) % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def paged_mixed_attn(q, k_cache, v_cache, page_table, lengths, patt, frozen, hidx=None, pidx=None, sm_scale=None,
@@ -113,35 +98,36 @@ def paged_mixed_attn(q, k_cache, v_cache, page_table, lengths, patt, frozen, hid
     Returns (B, H, 1, HD).  A length past the page table, a page id outside
     the caches, and for a frozen head a length past its pattern give NaN rows.
     validate also checks shapes with the reference operator's messages."""
-    H = frozen.numel() if isinstance(frozen, torch.Tensor) else len(frozen)
-    _no_grad_only("paged_mixed_attn", q, k_cache, v_cache, alpha, rho, z, patt)
     dev = v_cache.device
-    _ext.same_device("paged_mixed_attn", dev, q=q, k_cache=k_cache, page_table=page_table, lengths=lengths, patt=patt,
-                     alpha=alpha, rho=rho, z=z, lse=lse)
+    _ext.check_inputs("paged_mixed_attn", dev, (q, k_cache, v_cache, page_table, lengths, patt, alpha, rho, z, lse))
     if sm_scale is None:
-        sm_scale = 1.0 / (v_cache.size(-1) ** 0.5)
+        sm_scale = v_cache.size(-1) ** -0.5
     if alpha is not None and z is None:
         z = decomposed_logz(alpha.float(), rho.float())
     frozen_h, frozen_c = _table(frozen)
     if validate:
         _validate(q, k_cache, v_cache, page_table, lengths, patt, frozen_h, alpha, rho, z, kvidx)
-    tables = [_table(t)[1] for t in (hidx, pidx, kvidx)]
-    for name, t in zip(("hidx", "pidx", "kvidx"), tables):
-        if t is not None and len(t) < H:
-            raise ValueError(f"{name} must have one entry per output head")
-    B, HD = page_table.size(0), v_cache.size(-1)
-    out = torch.empty((B, H, 1, HD), device=dev, dtype=v_cache.dtype)
+    H = len(frozen_c)
+    args = _ext.SafPagedAttnArgs()
+    args.frozen = frozen_c
+    for name, t in (("hidx", hidx), ("pidx", pidx), ("kvidx", kvidx)):
+        if t is not None:
+            c = _table(t)[1]
+            if len(c) < H:
+                raise ValueError(f"{name} must have one entry per output head")
+            setattr(args, name, c)
+    B = page_table.size(0)
+    out = torch.empty((B, H, 1, v_cache.size(-1)), device=dev, dtype=v_cache.dtype)
     if B == 0:
         return out
-    q = _rows16(q)
-    args = _ext.SafPagedAttnArgs()
-    live = q is not None and q.numel() > 0
-    _ext.fill(args, q=q if live else None, k_cache=k_cache if live else None, v_cache=v_cache, out=out, lse=lse, patt=patt,
-              alpha=alpha, rho=rho, z=z, page_table=page_table, lengths=lengths)
+    if q is not None and q.numel() > 0:
+        q = _ext.fill_rows(args, "q", q)
+    else:
+        k_cache = None
+    _ext.fill(args, k_cache=k_cache, v_cache=v_cache, out=out, lse=lse, patt=patt, alpha=alpha, rho=rho, z=z,
+              page_table=page_table, lengths=lengths)
     args.n_heads = H
-    args.frozen = frozen_c
-    args.hidx, args.pidx, args.kvidx = tables
-    args.sm_scale = float(sm_scale)
+    args.sm_scale = sm_scale
     L = _ext.lib()
     with _ext.on_device(dev):
         nbytes = L.saf_paged_attn_workspace_bytes(args)

@@ -178,7 +178,7 @@ LOGP_BAD = [
     (dict(tokens=T((4,), I64)), "one entry per row", "inval"),
     (dict(tokens=T((3,), F32)), "int32 or int64", "inval"),
     (dict(logp=None), "logp is required", "inval"),
-    (dict(stats=None), "stats must be", "inval"),
+    (dict(stats=T((3, 3), F32)), "stats must be", "inval"),
     (dict(entropy=T((3,), BF16)), "entropy must be", "inval"),
     (dict(scale=0.0), "positive and finite", "inval"),
     (dict(scale=float("inf")), "positive and finite", "inval"),
@@ -208,6 +208,8 @@ def test_token_logprobs_bwd_refusals():
                      ((g, None, T((3, 100), stride=[1, 3])), "unit column stride")):
         assert L.saf_token_logprobs_bwd(_logp(), *bad, None) < 0
         assert msg in L.saf_last_error().decode(), msg
+    assert L.saf_token_logprobs_bwd(_logp(stats=None), g, None, d, None) < 0
+    assert "stats are required" in L.saf_last_error().decode()
     a = _logp(logits=T((1, 200000)), tokens=T((1,), I64), logp=T((1,), F32), stats=T((1, 2), F32))
     assert L.saf_token_logprobs_workspace_bytes(a) > 0
     assert L.saf_token_logprobs(a, None) == _ext.SAF_EWORKSPACE
@@ -247,5 +249,3 @@ def test_cpu_tensors_and_python_checks():
         kernel.paged_append_(x, x, None, kc, table, one)
     with pytest.raises(ValueError, match="go together"):
         kernel.paged_append_(x, x, kc, kc, table, one, cos=torch.zeros(5, 64))
-    with pytest.raises(NotImplementedError, match="no backward"):
-        kernel.paged_mixed_attn(x.requires_grad_(), kc, kc, table, one, None, frozen)

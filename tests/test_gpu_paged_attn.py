@@ -221,3 +221,33 @@ def test_shared_page():
     c = paged_case([40, 40], H=2, seed=17)
     c["table"][1, :2] = c["table"][0, :2]
     _check(c)
+
+
+def test_gradients_are_refused():
+    c = paged_case([20], H=2, seed=18)
+    m = {n: (t.cuda() if isinstance(t, torch.Tensor) else t) for n, t in c.items()}
+    q = m["q"].requires_grad_()
+    with pytest.raises(NotImplementedError, match="no backward"):
+        kernel.paged_mixed_attn(q, m["kc"], m["vc"], m["table"], m["lengths"], None, m["frozen"], m["hidx"])
+    with torch.no_grad():
+        out = kernel.paged_mixed_attn(q, m["kc"], m["vc"], m["table"], m["lengths"], None, m["frozen"], m["hidx"])
+    assert not out.requires_grad
+    v = m["vc"].new_zeros(1, 2, 1, 64).requires_grad_()
+    with pytest.raises(NotImplementedError, match="no backward"):
+        kernel.paged_append_(v, v, m["kc"], m["vc"], m["table"], m["lengths"])
+
+
+def test_tensors_of_another_device_are_refused():
+    c = paged_case([20], H=2, seed=19)
+    m = {n: (t.cuda() if isinstance(t, torch.Tensor) else t) for n, t in c.items()}
+    for name in ("q", "kc", "table", "lengths"):
+        d = dict(m)
+        d[name] = c[name]
+        with pytest.raises(ValueError, match="is on cpu"):
+            kernel.paged_mixed_attn(d["q"], d["kc"], d["vc"], d["table"], d["lengths"], None, d["frozen"], d["hidx"])
+    with pytest.raises(ValueError, match="is on cpu"):
+        kernel.token_logprobs(torch.zeros(2, 5, device="cuda"), torch.zeros(2, dtype=torch.long))
+    # the routing tables may live on the host
+    a = kernel.paged_mixed_attn(m["q"], m["kc"], m["vc"], m["table"], m["lengths"], None, m["frozen"], m["hidx"])
+    b = kernel.paged_mixed_attn(m["q"], m["kc"], m["vc"], m["table"], m["lengths"], None, c["frozen"], c["hidx"])
+    assert torch.equal(a, b)
