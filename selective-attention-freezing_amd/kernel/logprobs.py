@@ -80,6 +80,24 @@ class _TokenLogprobsFn(torch.autograd.Function):
         return dx, None, None, None, None, None
 
 
+def _leaf_edge(logits):
+    """The gradient edge of logits that are a leaf (None otherwise), kept alive
+    by the caller while the autograd graph is built; raises in a graph capture
+    where an eager graph of this operator still holds the leaf.
+
+    The leaf's node belongs to the stream of the call that made it.  A captured
+    backward would make that stream wait for the capturing one, and with it
+    join the capture without ever leaving it: torch ends the process there."""
+    if logits.grad_fn is not None:
+        return None
+    edge = torch.autograd.graph.get_gradient_edge(logits)
+    stream = _ext.current_stream_ptr(logits.device)
+    if edge.node.metadata.setdefault("saf_stream", stream) != stream and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("token_logprobs: an eager autograd graph of these logits, made on another stream, is still "
+                           "alive; release it before capturing their gradient")
+    return edge
+
+
 def token_logprobs(logits, tokens, top=0, entropy=False, scale=1.0, ignore_index=-100):
     """Log probabilities of ``tokens`` (...) under softmax(scale * logits)
     for logits (..., V) in float32, bfloat16 or float16.
@@ -107,6 +125,7 @@ def token_logprobs(logits, tokens, top=0, entropy=False, scale=1.0, ignore_index
     if x.stride(1) != 1 and x.size(1) > 1:
         x = x.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
+        edge = _leaf_edge(logits)  # noqa: F841  (alive until the graph holds it)
         logp, ent, idx, tlp = _TokenLogprobsFn.apply(x, t, top, bool(entropy), scale, int(ignore_index))
     else:
         logp, ent, idx, tlp, _ = _forward(x, t, top, entropy, scale, int(ignore_index), False)

@@ -454,13 +454,13 @@ class CausalSelfAttention(nn.Module):
             self._wc_key = key
         return self._wc_qkv, self._wc_qkvb
 
-    def forward(self, x, rope=None):
-        if self._split_route():
+    def forward(self, x, rope=None, sink=None):
+        if sink is None and self._split_route():
             y, wc = self.split_heads(x, rope)
             if wc is None:
                 return _kernel_mod.linear_permuted_cols(y, self.c_proj.weight, self.c_proj.bias, self._cperm_cols)
             return F.linear(y, wc, self.c_proj.bias)
-        return self.c_proj(self.attend(x, rope))
+        return self.c_proj(self.attend(x, rope, sink))
 
     # K (input features) up to which the QKV projection runs as the fused
     # GEMM + RoPE kernel (measured against the library GEMM plus the RoPE pass)
@@ -470,15 +470,18 @@ class CausalSelfAttention(nn.Module):
         return (wb is None and nqk > 0 and w.size(1) <= self.FUSED_ROPE_MAX_K
                 and _kernel_mod.linear_rope_usable(x, w, nqk, self.head_dim, rope[0]))
 
-    def head_outputs(self, x, rope=None):
+    def head_outputs(self, x, rope=None, sink=None):
         """(y, W): head outputs before c_proj and the c_proj weight whose
         input columns match their order (inference)."""
-        if self._split_route():
+        if sink is None and self._split_route():
             return self.split_heads(x, rope)
-        return self.attend(x, rope), self.c_proj.weight
+        return self.attend(x, rope, sink), self.c_proj.weight
 
-    def attend(self, x, rope=None):
-        """The block's attention before the output projection: (B, T, C) head outputs."""
+    def attend(self, x, rope=None, sink=None):
+        """The block's attention before the output projection: (B, T, C) head
+        outputs.  sink(k, v), if given, is handed the live heads' rotated keys
+        (None when no head is live) and every head's values, (B, heads, T, hd)
+        views: what a paged cache keeps of the sequence."""
         global _FUSED_DISPATCH_COUNT
         if self._fz_dirty:
             self._refresh_freeze_cache()
@@ -523,6 +526,8 @@ class CausalSelfAttention(nn.Module):
                         _kernel_mod.rope_qk_(qu, ku, *rope)
                     else:  # the in-place kernel is bf16 / fp16; fp32 keeps torch's rotation
                         qu, ku = apply_rotary_pos_emb(qu, ku, *rope)
+        if sink is not None:
+            sink(ku if nuf else None, v)
         _FUSED_DISPATCH_COUNT += 1
         dec = self._dec_any
         if dec and self._patterns is not None:
@@ -538,6 +543,36 @@ class CausalSelfAttention(nn.Module):
         if dec and self._patterns is not None:
             y = self._patterns.attach_gradient(self, y, v, pk["z"])
         return y.transpose(1, 2).reshape(B, T, nh * hd)
+
+    def attend_cached(self, x, store, positions, lengths, active, rope=None):
+        """attend() of one new token per sequence (inference): x (B, 1, C),
+        store = this layer's (k_cache, v_cache, page_table).  The token of
+        sequence b stands at positions[b] and its K / V are written there where
+        active[b] is 1; lengths counts the cached tokens it attends to."""
+        if self._fz_dirty:
+            self._refresh_freeze_cache()
+        kc, vc, table = store
+        B = x.size(0)
+        nh, hd = self.n_head, self.head_dim
+        nuf = nh - self._n_frozen
+        w, wb = self._infer_weight_cache()
+        y = F.linear(x, w, wb)[..., :(2 * nuf + nh) * hd].view(B, 1, 2 * nuf + nh, hd).transpose(1, 2)
+        q, k, v = y[:, :nuf], y[:, nuf:2 * nuf], y[:, 2 * nuf:]
+        if nuf == 0:
+            q = k = None
+        cos, sin = rope if self.position_encoding == "rope" else (None, None)
+        rotated = _kernel_mod.paged_append_(k, v, kc, vc, table, positions, active, q=q, cos=cos, sin=sin)
+        pk = {}
+        if self._dec_any:
+            if self._patterns is not None:
+                pk = self._patterns.kernel_inputs(self, self.block_size)
+                pk.pop("closed_form")
+            else:
+                pk = dict(alpha=self.dyn_alpha, rho=self.dyn_rho, z=self.dyn_z)
+        out = _kernel_mod.paged_mixed_attn(rotated, kc, vc, table, lengths, self.dyn_pattern, self._fz_mask_i32,
+                                           self._hidx_i32, self._pidx_i32 if self.dyn_pattern is not None else None,
+                                           validate=False, **pk)
+        return out.view(B, 1, nh * hd)
 
 
 class MLP(nn.Module):
@@ -580,8 +615,8 @@ class Block(nn.Module):
         self.ln_2 = LayerNorm(config.n_embd, bias=config.bias)
         self.mlp = MLP(config)
 
-    def forward(self, x, rope=None):
-        x = x + self.attn(self.ln_1(x), rope=rope)
+    def forward(self, x, rope=None, sink=None):
+        x = x + self.attn(self.ln_1(x), rope=rope, sink=sink)
         return x + self.mlp(self.ln_2(x))
 
 
@@ -633,8 +668,11 @@ class GPT(nn.Module):
             dtype = torch.get_autocast_gpu_dtype()
         return x, self.rotary(t, dtype)
 
-    def forward_hidden(self, idx):
+    def forward_hidden(self, idx, sinks=None):
+        """Hidden states of every position; sinks[i], if given, receives layer
+        i's keys and values (CausalSelfAttention.attend)."""
         x, rope = self.prepare_inputs(idx)
+        sinks = sinks or [None] * len(self.transformer.h)
         blocks = self.transformer.h
         if (x.is_cuda and not torch.is_grad_enabled()
                 and x.dtype in (torch.bfloat16, torch.float16)):
@@ -651,11 +689,11 @@ class GPT(nn.Module):
             for i, block in enumerate(blocks):
                 attn, mlp = block.attn, block.mlp
                 if attn.c_proj.bias is None:
-                    y, wc = attn.head_outputs(h, rope=rope)
+                    y, wc = attn.head_outputs(h, rope=rope, sink=sinks[i])
                     x2.addmm_(y.reshape(x2.size(0), -1), wc.t())
                     h = _kernel_mod.add_layernorm_(x, None, block.ln_2.weight, block.ln_2.bias)
                 else:
-                    h = _kernel_mod.add_layernorm_(x, attn(h, rope=rope), block.ln_2.weight, block.ln_2.bias)
+                    h = _kernel_mod.add_layernorm_(x, attn(h, rope=rope, sink=sinks[i]), block.ln_2.weight, block.ln_2.bias)
                 ln = blocks[i + 1].ln_1 if i + 1 < len(blocks) else self.transformer.ln_f
                 if mlp.c_proj.bias is None:
                     u = mlp.fc_gelu(h)
@@ -664,8 +702,8 @@ class GPT(nn.Module):
                 else:
                     h = _kernel_mod.add_layernorm_(x, mlp(h), ln.weight, ln.bias)
             return h
-        for block in blocks:
-            x = block(x, rope=rope)
+        for block, sink in zip(blocks, sinks):
+            x = block(x, rope=rope, sink=sink)
         return self.transformer.ln_f(x)
 
     def forward_all_positions(self, idx):
@@ -675,3 +713,9 @@ class GPT(nn.Module):
         """Prefill: last-position logits (B, 1, vocab)."""
         x = self.forward_hidden(idx)
         return self.lm_head(x[:, -1:, :])
+
+    def token_logprobs(self, idx, tokens, **kw):
+        """Log probabilities of tokens (B, T) as the next tokens of idx (B, T),
+        with kernel.token_logprobs' options (top, entropy, scale,
+        ignore_index); differentiable, so -logp.mean() is the training loss."""
+        return _kernel_mod.token_logprobs(self.forward_all_positions(idx), tokens, **kw)
