@@ -389,8 +389,9 @@ typedef struct saf_paged_append_args {
  * in fp32 and rounded once.  v is copied.  Rows of q_out with t >= counts[b]
  * are zero.  A token whose position lies outside the table or the caches of
  * cos / sin, or whose page id is not a page, is not written and its q_out rows
- * are NaN.  Two tokens on one slot: either may win.  bf16, fp16 and fp32, one
- * dtype for q, k, v and the caches. */
+ * are NaN.  Two tokens on one slot leave it unspecified; q_out and the caches
+ * must not overlap q, k or v.  bf16, fp16 and fp32, one dtype for q, k, v and
+ * the caches. */
 int saf_paged_append(const saf_paged_append_args* args, void* stream);
 
 typedef struct saf_paged_attn_args {
@@ -421,7 +422,8 @@ typedef struct saf_paged_attn_args {
  * gets zero rows (lse -inf); a length past the table, or a page id outside the
  * cache, gives NaN rows, as does a frozen head whose pattern is shorter than
  * the sequence.  Slots past a sequence's length are not read into the result.
- * bf16, fp16 and fp32; HD as in the prefill. */
+ * bf16, fp16 and fp32; HD as in the prefill.  16-bit storage rounds the weights
+ * to two 16-bit terms (fp16: pattern weights up to 255). */
 int saf_paged_attn_fwd(const saf_paged_attn_args* args, void* stream);
 
 /* Workspace of saf_paged_attn_fwd (0: none needed), -1 on invalid arguments. */

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendPara
   uint4 raw[HPT], pair[HPT];
 #pragma unroll
   for (int j = 0; j < HPT; ++j) {
-    raw[j] = make_uint4(0, 0, 0, 0);
+    raw[j] = pair[j] = make_uint4(0, 0, 0, 0);
     if (active && j < nh) raw[j] = *reinterpret_cast<const uint4*>(src + j * s_sh + d0);
   }
   if (is_v) {
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendPara
   const int half = p.rd / 2;
   const bool rot = active && p.cos != nullptr && d0 < p.rd;
   const int dp = d0 < half ? d0 + half : d0 - half;  // the pair's piece
-  float cs[N], sn[N], w[N], wp[N];
+  float cs[N], sn[N], w[N] = {}, wp[N] = {};
   if (rot) {
 #pragma unroll
     for (int j = 0; j < HPT; ++j)

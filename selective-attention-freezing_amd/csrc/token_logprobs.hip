@@ -473,7 +473,7 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(const LogprobBwdParams
     H = p.entropy[row];
   }
   // a row that takes no part has a zero gradient whatever it holds
-  const bool zero = skip && !ENT;
+  const bool zero = skip && (!ENT || ge == 0.f);
   auto grad = [&](float f, int i) {
     if (zero) return 0.f;
     const float v = c.exponent(f) - lg, q = fast_exp2(v);

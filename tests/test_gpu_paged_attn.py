@@ -74,6 +74,41 @@ def test_empty_sequences():
     assert (l[:, ~live] == 7.0).all()       # frozen heads' entries are left alone
 
 
+@pytest.mark.parametrize("dtype,bits", [(BF16, 16), (FP16, 16), (FP32, 17)])
+@pytest.mark.parametrize("lens", [[70, 200], [5000, 1]])
+def test_lse(lens, dtype, bits):
+    """Base-2 log-sum-exp of the live heads (values below 16: a few fp32 steps),
+    whole and joined."""
+    c = paged_case(lens, H=4, HKV=2, dtype=dtype, page=64, states=[0, 2, 0, 0], seed=21)
+    lse = torch.zeros(2, 4, 1, device="cuda")
+    run_paged(kernel, c, lse=lse)
+    _, _, want = paged_reference(c)
+    live = c["frozen"] == 0
+    assert bool(((lse.cpu().double()[:, :, 0] - want).abs()[:, live] <= 2.0 ** -bits).all())
+
+
+@pytest.mark.parametrize("lens", [[3000, 40], [40, 41]])
+def test_many_frozen_columns(lens):
+    """A group whose frozen weights exceed the LDS block: the keys in turns."""
+    _check(paged_case(lens, H=16, HKV=1, page=64, states=[0] + [2] * 15, seed=22))
+    _check(paged_case(lens, H=16, HKV=1, page=64, states=[2] * 16, dtype=FP16, seed=23))
+
+
+def test_wide_table_of_short_sequences():
+    """A table far wider than the sequences: the ranges follow the lengths."""
+    c = paged_case([300, 700], H=2, seed=24)
+    wide = torch.full((2, 2000), -1, dtype=torch.int32)
+    wide[:, :c["table"].size(1)] = c["table"]
+    c["table"] = wide
+    _check(c)
+
+
+def test_large_uncut_batch():
+    """More units than resident workgroups, long enough for eight waves."""
+    lens = [(331 * i) % 2100 + 1 for i in range(160)]
+    _check(paged_case(lens, H=8, HKV=8, hd=32, page=64, states=[0, 2, 0, 0, 0, 1, 0, 0], seed=25))
+
+
 @pytest.mark.parametrize("patt_dtype", [FP32, BF16, FP16])
 def test_pattern_types(patt_dtype):
     _check(paged_case([130, 64, 3], states=[1, 0, 1, 1], patt_dtype=patt_dtype, seed=5))

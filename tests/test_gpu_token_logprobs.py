@@ -102,6 +102,18 @@ def test_every_element_a_candidate():
     _check(x, torch.zeros(600, dtype=torch.long), top=20)
 
 
+@pytest.mark.parametrize("R,V,nt", [(600, 4000, 64), (100, 60000, 512), (3, 160000, 256), (600, 30000, 256)])
+def test_candidates_of_every_block_size(R, V, nt):
+    """The same in the one-wave, 512-thread and segmented forms, and with all
+    large values in one thread's pieces."""
+    piece = torch.arange(V) // 8
+    many = torch.where(piece % nt < 20, 5.0 + (torch.arange(V) % 97) / 64.0, torch.zeros(V))
+    one = torch.where(piece % nt == 3, 5.0 - (torch.arange(V) % 1009) / 512.0, torch.zeros(V))
+    x = torch.stack([many, one, many.flip(0)]).to(BF16)
+    x = x.repeat((R + 2) // 3, 1)[:R].contiguous()
+    _check(x, torch.zeros(R, dtype=torch.long), top=20, entropy=True)
+
+
 @pytest.mark.parametrize("V", [50, 5000, 40000])
 def test_masked_rows(V):
     """-inf entries, the type's lowest value, fewer finite entries than top."""
@@ -260,6 +272,50 @@ def test_padding_rows_have_zero_gradient_whatever_they_hold():
     assert float(r.logp[1].detach()) == 0.0
     r.logp.sum().backward()
     assert (xg.grad[1] == 0).all() and torch.isfinite(xg.grad).all()
+
+
+def test_padding_rows_of_an_entropy_term():
+    x, t = _inputs(3, 700, seed=12)
+    x[1] = float("nan")
+    t[1] = -100
+    xg = x.cuda().requires_grad_()
+    r = kernel.token_logprobs(xg, t.cuda(), entropy=True)
+    keep = torch.tensor([0, 2]).cuda()
+    (r.logp[keep].sum() + r.entropy[keep].sum()).backward()
+    assert (xg.grad[1] == 0).all() and torch.isfinite(xg.grad).all()
+
+
+def test_entropy_alone():
+    x, t = _inputs(4, 900, FP32, seed=13)
+    ge = torch.linspace(-1, 1, 4)
+    xg = x.cuda().requires_grad_()
+    r = kernel.token_logprobs(xg, t.cuda(), entropy=True)
+    (dx,) = torch.autograd.grad(r.entropy, xg, ge.cuda())
+    want = _grad_reference(x, t, torch.zeros(4), ge, 1.0)
+    p = torch.softmax(x.double(), -1)
+    assert bool(((dx.double().cpu() - want).abs() <= 2.0 ** -22 * want.abs() + 2.0 ** -16 * 40 * p + 1e-37).all())
+
+
+def test_second_derivatives_are_refused():
+    x, t = _inputs(2, 50, FP32, seed=14)
+    xg = x.cuda().requires_grad_()
+    (dx,) = torch.autograd.grad(kernel.token_logprobs(xg, t.cuda()).logp.sum(), xg, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), xg)
+
+
+def test_expanded_rows_and_another_stream():
+    x, t = _inputs(1, 3000, seed=15)
+    one = kernel.token_logprobs(x.cuda(), t.cuda(), top=3)
+    many = kernel.token_logprobs(x.cuda().expand(5, -1), t.cuda().expand(5), top=3)
+    assert all(torch.equal(a.expand(5, *a.shape[1:]), b) for a, b in zip(one[:1] + one[2:], many[:1] + many[2:]))
+    side = torch.cuda.Stream()
+    xd, td = x.cuda(), t.cuda()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = kernel.token_logprobs(xd, td, top=3)
+    side.synchronize()
+    assert torch.equal(other.logp, one.logp) and torch.equal(other.top_index, one.top_index)
 
 
 def test_masked_entries_have_zero_gradient():
