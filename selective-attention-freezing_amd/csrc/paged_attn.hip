@@ -45,6 +45,21 @@ __device__ inline float column_sum(float x) {
   return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// Inclusive sum over the lanes up to this one (GFX9 DPP moves; every lane
+// active): shifts inside 16-lane rows, then lane 15 of rows 0 and 2 and lane 31
+// into the rows behind them.
+template <int CTRL, int ROWMASK> __device__ __forceinline__ int dpp_add_i32(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWMASK, 0xf, false);
+}
+__device__ inline int wave_scan(int x) {
+  x = dpp_add_i32<0x111, 0xf>(x);  // row_shr:1
+  x = dpp_add_i32<0x112, 0xf>(x);  // row_shr:2
+  x = dpp_add_i32<0x114, 0xf>(x);  // row_shr:4
+  x = dpp_add_i32<0x118, 0xf>(x);  // row_shr:8
+  x = dpp_add_i32<0x142, 0xa>(x);  // row_bcast:15, rows 1 and 3
+  return dpp_add_i32<0x143, 0xc>(x);  // row_bcast:31, rows 2 and 3
+}
+
 __device__ inline f32x4_t mfma16(__bf16, uint4 a, uint4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                  0, 0);
@@ -401,20 +416,64 @@ __device__ inline void walk(const PagedAttnParams& p, PagedWave<T, HD>& st, cons
   }
 }
 
-// Keys per range where sequences are cut into n_splits ranges: the longest
-// sequence's share, so that a page table wider than the sequences costs
-// nothing (whole wave, uniform result).
-__device__ inline int range_keys(const PagedAttnParams& p, int lane) {
-  int most = 0;
-  for (int b = lane; b < p.B; b += 64) most = max(most, p.lengths[b]);
-  // in runs of 64 keys, which float32 holds exactly (capacity is at most 2^30)
-  most = min(64 * (int)wave_max((float)((most + 63) >> 6)), p.capacity);
-  const int keys = (most + p.n_splits - 1) / p.n_splits;
-  return max((keys + 127) & ~127, p.chunk);
-}
+// Cut sequences.  The launch has n_ranges workgroups per unit, and the
+// sequences' keys are dealt to them in ranges of `runs` runs of 128 keys (at
+// least p.chunk keys): as even a share of all cached tokens as whole ranges
+// allow, whatever the sequences' lengths and the page table's width are.  Every
+// wave works this out from the lengths for itself (n_ranges >= 2 B).
+struct Ranges {
+  int runs;   // runs of 128 keys per range
+  int n0;     // this lane's sequence among the first 64, in runs
+  __device__ static inline int len(const PagedAttnParams& p, int b) {  // in runs, at most 2^23
+    return b < p.B ? (min(max(p.lengths[b], 0), p.capacity) + 127) >> 7 : 0;
+  }
+  // ceil(n / runs): the reciprocal's estimate is off by at most one
+  __device__ inline int count(int n) const {
+    const int x = n + runs - 1;
+    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)runs));
+    q -= q * runs > x;
+    q += (q + 1) * runs <= x;
+    return q;
+  }
 
-// Grid: one workgroup per (sequence, unit, key range).
-template <typename T, int HD>
+  __device__ inline Ranges(const PagedAttnParams& p, int lane) {
+    n0 = len(p, lane);
+    float total = (float)n0;
+    for (int b = lane + 64; b < p.B; b += 64) total += (float)len(p, b);
+    // about half a range per sequence is lost to whole ranges
+    const float share = dpp_wave_sum(total) * __builtin_amdgcn_rcpf((float)p.n_ranges - 0.5f * (float)p.B);
+    runs = max((int)share + 1, p.chunk >> 7);
+    for (;;) {  // ends at the latest where every sequence is one range
+      int n = count(n0);
+      for (int b = lane + 64; b < p.B; b += 64) n += count(len(p, b));
+      if ((int)dpp_wave_sum((float)n) <= p.n_ranges) break;
+      runs += (runs >> 3) + 1;
+    }
+    runs = __builtin_amdgcn_readfirstlane(runs);
+  }
+  // Sequence and place in it of range j (b = -1: there is none), or, with
+  // want >= 0, the first range of sequence `want` in `first`.
+  __device__ inline void find(const PagedAttnParams& p, int lane, int j, int want, int& b, int& place, int& first) const {
+    int base = 0;
+    b = -1;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const int r = count(b0 == 0 ? n0 : len(p, b0 + lane));
+      const int incl = wave_scan(r), excl = base + incl - r;
+      if (want >= b0 && want < b0 + 64) first = __builtin_amdgcn_readlane(excl, want - b0);
+      const uint64_t hit = __ballot(j >= excl && j < excl + r);
+      if (hit != 0) {
+        const int at = __builtin_ctzll(hit);
+        b = b0 + at;
+        place = j - __builtin_amdgcn_readlane(excl, at);
+      }
+      base += __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+};
+
+// Grid: one workgroup per (unit, range), units fastest; uncut: per (unit,
+// sequence).
+template <typename T, int HD, bool CUT>
 __global__ __launch_bounds__(64 * paged_max_waves(sizeof(T), HD), paged_simd_waves(sizeof(T), HD)) void paged_attn_kernel(
     const PagedAttnParams p) {
   using Tile = PagedTile<T, HD>;
@@ -422,18 +481,22 @@ __global__ __launch_bounds__(64 * paged_max_waves(sizeof(T), HD), paged_simd_wav
   const int lane = threadIdx.x & 63, W = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  int wg = blockIdx.x;
-  const int split = wg % p.n_splits;
-  wg /= p.n_splits;
-  const int u = wg % p.n_units, b = wg / p.n_units;
+  const int u = blockIdx.x % p.n_units, item = blockIdx.x / p.n_units;
+  int b = item, chunk = p.chunk, place = 0, unused;
+  if constexpr (CUT) {
+    const Ranges ranges(p, lane);
+    ranges.find(p, lane, item, -1, b, place, unused);
+    chunk = 128 * ranges.runs;
+    b = __builtin_amdgcn_readfirstlane(b);
+    place = __builtin_amdgcn_readfirstlane(place);
+    if (b < 0) return;
+  }
   const PagedUnit un = p.unit[u];
   const int c0 = un.c0, nc = un.cols, nl = un.live;
 
   const int n_in = p.lengths[b];
   const int n = n_in < 0 ? 0 : (n_in > p.capacity ? p.capacity : n_in);
-  const int chunk = p.n_splits > 1 ? range_keys(p, lane) : p.chunk;
-  const int j0 = split * chunk, j1 = min(n, j0 + chunk);
-  if (split > 0 && j0 >= n) return;  // the join knows the live ranges from the lengths
+  const int j0 = place * chunk, j1 = min(n, j0 + chunk);
 
   extern __shared__ __align__(16) float lds[];
   float* sm_ml = lds;           // [W][16][2]
@@ -513,8 +576,8 @@ __global__ __launch_bounds__(64 * paged_max_waves(sizeof(T), HD), paged_simd_wav
       ll += f * sm_ml[(w * 16 + col) * 2 + 1];
       acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
     }
-    if (p.n_splits > 1) {
-      const int64_t slot = ((int64_t)b * p.n_heads + c0 + col) * p.n_splits + split;
+    if constexpr (CUT) {
+      const int64_t slot = (int64_t)item * p.n_heads + c0 + col;
       *reinterpret_cast<float4*>(p.part_o + slot * HD + d) = acc;
       if (d == 0) {
         p.part_ml[2 * slot] = mm;
@@ -545,24 +608,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   const bool bad = n_in > p.capacity;
   const int n = n_in < 0 ? 0 : (bad ? p.capacity : n_in);
   const int lane = threadIdx.x & 63;
-  const int chunk = range_keys(p, lane);
-  const int ns = n == 0 ? 0 : (n - 1) / chunk + 1;
-  const int64_t slot = ((int64_t)b * p.n_heads + col) * p.n_splits;
+  const Ranges ranges(p, lane);
+  int first = 0, unused_b, unused_place;
+  ranges.find(p, lane, -1, b, unused_b, unused_place, first);
+  const int ns = ranges.count((n + 127) >> 7);
+  const int64_t slot = (int64_t)first * p.n_heads + col;  // of range 0; the next ones n_heads further
   const float* ml = p.part_ml + 2 * slot;
+  const int step = 2 * p.n_heads;
   float mm = -INFINITY;
-  for (int s = lane; s < ns; s += 64) mm = fmaxf(mm, ml[2 * s]);
+  for (int s = lane; s < ns; s += 64) mm = fmaxf(mm, ml[s * step]);
   mm = wave_max(mm);
   const float mu = mm == -INFINITY ? 0.f : mm;
   float ll = 0.f;
-  for (int s = lane; s < ns; s += 64) ll += fast_exp2(ml[2 * s] - mu) * ml[2 * s + 1];
-#pragma unroll
-  for (int k = 32; k > 0; k >>= 1) ll += __shfl_xor(ll, k, 64);
+  for (int s = lane; s < ns; s += 64) ll += fast_exp2(ml[s * step] - mu) * ml[s * step + 1];
+  ll = dpp_wave_sum(ll);
   const int grp = threadIdx.x / L, d4 = threadIdx.x % L;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (grp < G) {
     for (int s = grp; s < ns; s += G) {
-      const float f = fast_exp2(ml[2 * s] - mu);
-      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot + s) * HD + 4 * d4);
+      const float f = fast_exp2(ml[s * step] - mu);
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot + (int64_t)s * p.n_heads) * HD + 4 * d4);
       acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
     }
     sm[grp][d4] = acc;
@@ -588,10 +653,14 @@ template <typename T, int HD>
 static hipError_t launch_paged_t(const PagedAttnParams& p, hipStream_t s) {
   const size_t o_floats = (size_t)p.waves * p.max_cols * (HD + kOPad);
   const size_t lds = sizeof(float) * (p.waves * 32 + (o_floats > (size_t)p.w_floats ? o_floats : (size_t)p.w_floats));
-  hipLaunchKernelGGL((paged_attn_kernel<T, HD>), dim3((unsigned)((int64_t)p.B * p.n_units * p.n_splits)),
-                     dim3(64 * p.waves), lds, s, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.n_splits == 1) return e;
+  const dim3 block(64 * p.waves);
+  if (p.n_ranges == 1) {
+    hipLaunchKernelGGL((paged_attn_kernel<T, HD, false>), dim3((unsigned)((int64_t)p.B * p.n_units)), block, lds, s, p);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL((paged_attn_kernel<T, HD, true>), dim3((unsigned)(p.n_ranges * p.n_units)), block, lds, s, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3((unsigned)(p.B * p.n_heads)), dim3(256), 0, s, p);
   return hipGetLastError();
 }

@@ -72,19 +72,21 @@ int check_vec(const saf_tensor_t& t, const char* name, int64_t n) {
 
 // ---- paged attention ----------------------------------------------------------
 
-// Key ranges.  A sequence is cut only where its units leave resident
-// workgroups idle, into as many ranges as fill them (whole rounds cost more
-// than a ragged tail: 64 sequences of up to 4096 keys, 768 units for 768
-// workgroups, 86 us whole, 94 us in two ranges, 106 us in eight), of at least
-// kMinKeys keys, and not below kSplitFrom positions, where the second launch
-// costs what the shorter walk saves (one sequence of 1024 keys: 9.2 us either
-// way and 4.6 us more host time; of 2000 keys in a group of seven: 21 us whole,
-// 11 us cut).  Uncut sequences from kWideFrom positions on run eight waves
-// where the registers allow (64 x 4096 keys: 79 us against 86; 128 x 8192 keys
-// at hd 128: 422 against 442); short ones four (64 x 128 keys: 7.4 us against
-// 12.6, idle waves cost their launch).
+// Key ranges.  Sequences are cut only where whole ones would leave half of the
+// resident workgroups idle, into as many ranges together as fill them once
+// (whole rounds cost more than a ragged tail: 64 sequences of up to 4096 keys,
+// 768 units for 768 workgroups, took 86 us whole, 94 us in two ranges each,
+// 106 us in eight), of at least kMinKeys keys, and not below kSplitFrom
+// positions, where the second launch costs what the shorter walk saves (one
+// sequence of 1024 keys: 9.2 us either way and 4.6 us more host time; of 2000
+// keys in a group of seven: 21 us whole, 12 us cut).  Ranges dealt over all
+// sequences instead of an equal number to each: 16 ragged sequences in two KV
+// groups 25 us against 29, 8 at hd 256 69 against 73.  Uncut sequences from
+// kWideFrom positions on run eight waves where the registers allow (64 x 4096
+// keys: 80 us against 86; 128 x 8192 keys at hd 128: 422 against 442); short
+// ones four (64 x 128 keys: 7.4 us against 12.6, idle waves cost their launch).
 constexpr int kMinKeys = 256, kSplitFrom = 1536, kWideFrom = 2048;
-constexpr int kWeightFloats = 8192;  // 32 KB: four workgroups of a CU still fit its LDS
+constexpr int kWeightFloats = 6144;  // 24 KB: five workgroups of a CU fit its LDS with their partial sums
 
 int plan_paged(const saf_paged_attn_args* a, PagedAttnParams& p, int& dtype, int& hd) {
   if (a == nullptr) return fail(SAF_EINVAL, "args is NULL");
@@ -217,33 +219,27 @@ int plan_paged(const saf_paged_attn_args* a, PagedAttnParams& p, int& dtype, int
 
   if (B > kMaxGrid / SAF_MAX_HEADS / 64) return fail(SAF_EUNSUPPORTED, "batch %lld is too large", (long long)B);
   p.B = (int)B;
-  // key ranges: as many as the resident workgroups leave for each unit
-  const int64_t tasks = B * nu;
+  // ranges: as many as the resident workgroups leave for each unit
   const int64_t slots = (int64_t)cu_count() * paged_simd_waves(elem_size(dtype), hd);
-  int64_t want = tasks > 0 ? slots / tasks : 1;
-  const int64_t most = ((int64_t)p.capacity + kMinKeys - 1) / kMinKeys;
-  if (want > most) want = most;
-  if (p.capacity < kSplitFrom) want = 1;
-  p.n_splits = want > 1 ? (int)want : 1;
-  p.chunk = p.n_splits > 1 ? kMinKeys : (p.capacity + 31) / 32 * 32;
+  int64_t ranges = slots / nu;
+  const int64_t most = ((int64_t)p.capacity + kMinKeys - 1) / kMinKeys * B;
+  if (ranges > most) ranges = most;
+  p.n_ranges = ranges >= 2 * B && B > 0 && p.capacity >= kSplitFrom ? (int)ranges : 1;
+  p.chunk = p.n_ranges > 1 ? kMinKeys : (p.capacity + 31) / 32 * 32;
   if (p.chunk < 32) p.chunk = 32;
-  p.waves = p.n_splits == 1 && p.capacity >= kWideFrom ? paged_max_waves(elem_size(dtype), hd) : 4;
-  // key range of a workgroup at its largest
-  int64_t range = p.n_splits > 1 ? ((p.capacity + p.n_splits - 1) / p.n_splits + 127) / 128 * 128 : p.chunk;
-  if (range < p.chunk) range = p.chunk;
-  // LDS of the frozen columns' weights: a whole key range where that is within
+  p.waves = p.n_ranges == 1 && p.capacity >= kWideFrom ? paged_max_waves(elem_size(dtype), hd) : 4;
+  // LDS of the frozen columns' weights: the whole capacity where that is within
   // kWeightFloats, at least one step per column
   if (max_frozen > 0) {
     int64_t keys = kWeightFloats / max_frozen / 32 * 32;
-    if (keys > range) keys = range;
+    if (keys > (p.capacity + 31) / 32 * 32) keys = (p.capacity + 31) / 32 * 32;
+    if (keys < 32) keys = 32;
     p.w_floats = (int)keys * max_frozen;
   }
   return SAF_OK;
 }
 
-int64_t paged_slots(const PagedAttnParams& p) {
-  return p.n_splits > 1 ? (int64_t)p.B * p.n_heads * p.n_splits : 0;
-}
+int64_t paged_slots(const PagedAttnParams& p) { return p.n_ranges > 1 ? (int64_t)p.n_heads * p.n_ranges : 0; }
 
 // ---- log probabilities -----------------------------------------------------------
 

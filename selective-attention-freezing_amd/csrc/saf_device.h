@@ -171,6 +171,22 @@ __device__ inline float wave_max(float x) {
 }
 __device__ inline float wave_min(float x) { return -wave_max(-x); }
 
+// Sum over the 64 lanes (every lane active), wave-uniform, by the moves of
+// wave_max with zeros where a row takes no part.
+template <int CTRL, int ROWMASK>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWMASK, 0xf, false));
+}
+__device__ inline float dpp_wave_sum(float x) {
+  x = dpp_add<0xb1, 0xf>(x);
+  x = dpp_add<0x4e, 0xf>(x);
+  x = dpp_add<0x141, 0xf>(x);
+  x = dpp_add<0x140, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);
+  x = dpp_add<0x143, 0xc>(x);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
 // Entry i (wave-uniform) of an int16 table in the kernel arguments, read as
 // its aligned 32-bit word: the compiler then reads it with a scalar load
 // (waited with the other argument reads) instead of a 16-bit vector load

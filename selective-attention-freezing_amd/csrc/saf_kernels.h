@@ -247,12 +247,12 @@ struct PagedAttnParams {
   const int32_t* lengths;
   int page_shift, n_pages, capacity;  // capacity = page_table columns x page size
   int B, n_heads, n_units, waves, max_cols;
-  int n_splits;  // key ranges per sequence
-  int chunk;     // n_splits 1: the capacity; else the least keys of a range
+  int n_ranges;  // ranges of keys that the sequences are cut into, 1: uncut
+  int chunk;     // uncut: the capacity; else the least keys of a range
   int w_floats;  // LDS floats for the frozen columns' weights (0: no frozen column)
   float scale_log2;
-  float* part_o;   // [B][n_heads][n_splits][HD] (by column), n_splits > 1
-  float* part_ml;  // [B][n_heads][n_splits][2]
+  float* part_o;   // [n_ranges][n_heads][HD] (by column), cut sequences
+  float* part_ml;  // [n_ranges][n_heads][2]
   const void* patt;
   int patt_dtype, p_S;
   int64_t p_sh, p_si, p_sj;

@@ -102,20 +102,6 @@ template <int M> __device__ __forceinline__ uint64_t wave_max64_step(uint64_t x,
 }
 __device__ inline uint64_t wave_max64(uint64_t x, int lane) { return wave_max64_step<32>(x, lane); }
 
-// Sum over the wave's 64 lanes, the moves of wave_max with zeros where a row
-// does not take part.
-template <int CTRL, int ROWMASK> __device__ __forceinline__ float dpp_add(float x) {
-  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWMASK, 0xf, false));
-}
-__device__ inline float wave_sum(float x) {
-  x = dpp_add<0xb1, 0xf>(x);
-  x = dpp_add<0x4e, 0xf>(x);
-  x = dpp_add<0x141, 0xf>(x);
-  x = dpp_add<0x140, 0xf>(x);
-  x = dpp_add<0x142, 0xa>(x);
-  x = dpp_add<0x143, 0xc>(x);
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
-}
 // Descending order of a bitonic sequence over the lanes, and of any keys.
 __device__ inline uint64_t wave_merge_desc(uint64_t x, int lane) { return merge_runs<32>(x, lane, true); }
 __device__ inline uint64_t wave_sort_desc(uint64_t x, int lane) {
@@ -177,8 +163,8 @@ struct Sums {
 // The sums of a whole wave: one common maximum, then plain sums.
 template <bool ENT> __device__ inline void wave_merge(Sums& a, float sl2) {
   a.raise<ENT>(wave_max(a.m), sl2);
-  a.s = wave_sum(a.s);
-  if (ENT) a.t = wave_sum(a.t);
+  a.s = dpp_wave_sum(a.s);
+  if (ENT) a.t = dpp_wave_sum(a.t);
 }
 
 __device__ inline int64_t token_of(const LogprobParams& p, int64_t r) {
