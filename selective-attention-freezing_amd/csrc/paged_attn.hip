@@ -257,10 +257,16 @@ __device__ inline void frozen_weights(const PagedAttnParams& p, float* w, int pi
         a[k] = load_bits(p.alpha, row * p.a_sh + key * p.a_ss, p.a_dtype);
         d[k] = load_bits(p.rho, row * p.r_sh + (n - 1 - key) * p.r_ss, p.r_dtype);
       }
+      const float zf = bits_to_f32(z, p.z_dtype);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        x[k] = fast_exp2((bits_to_f32(a[k], p.a_dtype) + bits_to_f32(d[k], p.r_dtype) - bits_to_f32(z, p.z_dtype)) *
-                         kLog2e) * scale;
+      for (int k = 0; k < 4; ++k) {
+        // where the weight matters z is close to the sum and their difference
+        // exact: the sum's own rounding (TwoSum) is all that large logits lose
+        const float af = bits_to_f32(a[k], p.a_dtype), df = bits_to_f32(d[k], p.r_dtype);
+        const float sum = af + df, back = sum - af;
+        const float lost = sum == -INFINITY ? 0.f : (af - (sum - back)) + (df - back);
+        x[k] = fast_exp2(((sum - zf) + lost) * kLog2e) * scale;
+      }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {

@@ -133,6 +133,20 @@ def test_decomposed_without_z():
     assert bool(((out.double().cpu()[:, :, 0] - ref).abs() <= paged_tolerance(c, ref, mag)).all())
 
 
+def test_large_pattern_logits():
+    """Logits of size 150: the sum's rounding alone (2^-24 150 = 9e-6 of the
+    weight) would show in float32; what is left is exp2's argument (2^-24 of
+    its size where the weight matters, below 40) and a few roundings."""
+    c = paged_case([300, 77], H=3, states=[2, 0, 2], dtype=FP32, seed=26)
+    c["alpha"] *= 80
+    c["rho"] *= 80
+    c["z"] = torch.stack([torch.logsumexp(c["alpha"][:, :n].double() + c["rho"][:, :n].flip(1).double(), 1)
+                          for n in range(1, 301)], 1).float()
+    out = run_paged(kernel, c).double().cpu()[:, :, 0]
+    ref, mag, _ = paged_reference(c)
+    assert bool(((out - ref).abs() <= 2.0 ** -17 * mag + 2.0 ** -24 * ref.abs())[:, [0, 2]].all())
+
+
 def test_window_pattern():
     """rho = -inf past a window: exact zeros for the far keys."""
     c = paged_case([300, 40], states=[2, 0, 2, 0], seed=8)
