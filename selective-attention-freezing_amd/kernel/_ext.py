@@ -217,44 +217,41 @@ def set_desc(args, offset, t):
     _DESC.pack_into(args, offset, *_desc_values(t))
 
 
-def fill(block, **tensors):
-    """Write the descriptors of the given tensors (None: left absent) into
-    their fields of an argument block."""
-    offset = _OFFSETS[type(block)]
-    for name, t in tensors.items():
-        if t is not None:
-            _DESC.pack_into(block, offset[name], *_desc_values(t))
+_desc_fill = None
 
 
-def fill_rows(block, name, t):
-    """fill() of a (B, U, T, HD) tensor that is only read, as a copy where its
-    rows are not 16-byte aligned; returns what the block points to."""
-    v = _desc_values(t)
-    mask = 3 if v[1] == SAF_F32 else 7
-    if (v[0] & 15 or v[10] != 1 or (v[3] > 1 and v[7] & mask) or (v[4] > 1 and v[8] & mask)
-            or (v[5] > 1 and v[9] & mask)):
-        t = t.clone(memory_format=torch.contiguous_format)
-        v = _desc_values(t)
-    _DESC.pack_into(block, _OFFSETS[type(block)][name], *v)
-    return t
+def desc_fill():
+    """kernel._desc.fill (csrc/py_desc.cpp), loaded once per process."""
+    global _desc_fill
+    if _desc_fill is None:
+        try:
+            from . import _desc
+        except ImportError as e:
+            raise RuntimeError("kernel/_desc.so is not built or does not load: run __graft_entry__.build() (or "
+                               "build_ext.build()) first") from e
+        _desc_fill = _desc.fill
+    return _desc_fill
 
 
-_OFFSETS = {c: {n: getattr(c, n).offset for n, kind in c._fields_ if kind is SafTensor}
-            for c in (SafPagedAppendArgs, SafPagedAttnArgs, SafTokenLogprobsArgs)}
+def offsets(block, *names):
+    """Byte offsets of descriptors in an argument block class, for fill()."""
+    return tuple(getattr(block, n).offset for n in names)
 
 
-def check_inputs(what, device, tensors, differentiable=False):
-    """Raise unless every given tensor lives on `device`, a HIP device, and,
-    for an operator without a backward, needs no gradient."""
-    if device.type != "cuda":
+def device_index(what, t):
+    """Index of the HIP device that t lives on."""
+    if not t.is_cuda:
         raise RuntimeError(f"{what} runs on HIP devices only (got a CPU tensor)")
-    grad = not differentiable and torch.is_grad_enabled()
-    for t in tensors:
-        if t is not None:
-            if t.device != device:
-                raise ValueError(f"{what}: a tensor is on {t.device}, expected {device}")
-            if grad and t.requires_grad:
-                raise NotImplementedError(f"{what} has no backward: call it under torch.no_grad()")
+    return t.get_device()
+
+
+def aligned_copies(what, block, at, mask, index, tensors):
+    """Second step of a fill() whose result was not 0: contiguous copies of the
+    tensors in the mask, described in their places; the caller keeps them
+    until the call is enqueued."""
+    held = [t.clone(memory_format=torch.contiguous_format) if mask >> i & 1 else None for i, t in enumerate(tensors)]
+    desc_fill()(what, block, at, 0, index, False, *held)
+    return held
 
 
 class _NoGuard:
@@ -268,12 +265,10 @@ class _NoGuard:
 _NO_GUARD = _NoGuard()
 
 
-def on_device(device):
-    """Context that makes `device` the current one (launches and cached device
-    properties follow it); nothing to do where it is."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _NO_GUARD
-    return torch.cuda.device(device)
+def on_device(index):
+    """Context that makes HIP device `index` the current one (launches and
+    cached device properties follow it); nothing to do where it is."""
+    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 # saf_mixed_attn_args: offsets of the tensor descriptors, and the fields from

@@ -9,11 +9,16 @@ serves the evaluation that the reference does with log_softmax and gather
 (/root/reference/nanogpt/eval_nanogpt_logprobs.py) and sampling loops that
 report alternatives.
 """
+import ctypes
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _ext
+
+_stream = torch._C._cuda_getCurrentRawStream
+_AT = _ext.offsets(_ext.SafTokenLogprobsArgs, "logits", "tokens", "logp", "entropy", "stats", "top_index", "top_logp")
+_GRAD_AT = tuple(i * ctypes.sizeof(_ext.SafTensor) for i in range(3))
 
 
 class TokenLogprobs(NamedTuple):
@@ -32,15 +37,17 @@ def _forward(logits, tokens, top, entropy, scale, ignore_index, keep_stats):
     idx = torch.empty(R, top, device=dev, dtype=torch.int64) if top else None
     tlp = torch.empty(R, top, **f32) if top else None
     args = _ext.SafTokenLogprobsArgs()
-    _ext.fill(args, logits=logits, tokens=tokens, logp=logp, entropy=ent, stats=stats, top_index=idx, top_logp=tlp)
+    index = logits.get_device()
+    _ext.desc_fill()("token_logprobs", ctypes.addressof(args), _AT, 0, index, False, logits, tokens, logp, ent, stats, idx,
+                     tlp)
     args.top, args.ignore_index, args.scale = top, ignore_index, scale
     L = _ext.lib()
-    with _ext.on_device(dev):
+    with _ext.on_device(index):
         nbytes = L.saf_token_logprobs_workspace_bytes(args)
         if nbytes > 0:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-        rc = L.saf_token_logprobs(args, _ext.current_stream_ptr(dev))
+        rc = L.saf_token_logprobs(args, _stream(index))
     if rc:
         _ext.check(rc)
     return logp, ent, idx, tlp, stats
@@ -69,12 +76,13 @@ class _TokenLogprobsFn(torch.autograd.Function):
         R, V = logits.shape
         dx = torch.empty(R, V, device=logits.device, dtype=logits.dtype)
         args = _ext.SafTokenLogprobsArgs()
-        _ext.fill(args, logits=logits, tokens=tokens, stats=stats, entropy=ent)
+        index, fill = logits.get_device(), _ext.desc_fill()
+        fill("token_logprobs", ctypes.addressof(args), _AT, 0, index, False, logits, tokens, None, ent, stats, None, None)
         args.ignore_index, args.scale = ctx.ignore_index, ctx.scale
-        with _ext.on_device(logits.device):
-            rc = _ext.lib().saf_token_logprobs_bwd(
-                args, _ext.tensor_desc(glogp), _ext.tensor_desc(gent), _ext.tensor_desc(dx),
-                _ext.current_stream_ptr(logits.device))
+        descs = (_ext.SafTensor * 3)()
+        fill("token_logprobs", ctypes.addressof(descs), _GRAD_AT, 0, index, False, glogp, gent, dx)
+        with _ext.on_device(index):
+            rc = _ext.lib().saf_token_logprobs_bwd(args, descs[0], descs[1], descs[2], _stream(index))
         if rc:
             _ext.check(rc)
         return dx, None, None, None, None, None
@@ -117,7 +125,7 @@ def token_logprobs(logits, tokens, top=0, entropy=False, scale=1.0, ignore_index
     if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens must have the logits' leading shape (got {tuple(tokens.shape)} for "
                          f"{tuple(logits.shape)})")
-    _ext.check_inputs("token_logprobs", logits.device, (tokens,), differentiable=True)
+    _ext.device_index("token_logprobs", logits)
     top, scale = int(top), float(scale)
     x, t = logits, tokens
     if x.dim() != 2:

@@ -17,10 +17,19 @@ that no call reads back; what they get wrong shows as NaN, never as a stray
 access (libsafattn.so ``saf_paged_append``, ``saf_paged_attn_fwd``).  Forward
 only.
 """
+import ctypes
+
 import torch
 
 from . import _ext
 from .fused_attn import _table, decomposed_logz
+
+_stream = torch._C._cuda_getCurrentRawStream
+_APPEND = ("v", "k", "q", "q_out", "k_cache", "v_cache", "page_table", "positions", "counts", "cos", "sin")
+_APPEND_AT = _ext.offsets(_ext.SafPagedAppendArgs, *_APPEND)
+_WEIGHTS_AT = _ext.offsets(_ext.SafPagedAppendArgs, "q_weight", "k_weight")
+_ATTN_AT = _ext.offsets(_ext.SafPagedAttnArgs, "q", "k_cache", "v_cache", "out", "lse", "patt", "alpha", "rho", "z",
+                        "page_table", "lengths")
 
 
 def paged_append_(k, v, k_cache, v_cache, page_table, positions, counts=None, q=None, cos=None, sin=None,
@@ -44,39 +53,37 @@ def paged_append_(k, v, k_cache, v_cache, page_table, positions, counts=None, q=
     fp32 arithmetic, one rounding.  A token whose position lies outside the
     page table or the cos / sin caches, or whose page id is not a page of the
     caches, is not written, and its rows of q are NaN."""
-    dev = v.device
     if (k is None) != (k_cache is None):
         raise ValueError("k and k_cache go together")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
-    _ext.check_inputs("paged_append_", dev, (q, k, v, k_cache, v_cache, page_table, positions, counts, cos, sin))
-    _ext.check_inputs("paged_append_", dev, (q_weight, k_weight), differentiable=True)  # module parameters
+    dev = _ext.device_index("paged_append_", v)
     out = None
     if q is not None:
         # token-major like the projection it came from, so that a token's rows
         # follow each other
         B, U, T, HD = q.shape
-        out = torch.empty_strided((B, U, T, HD), (T * U * HD, HD, U * HD, 1), device=dev, dtype=q.dtype)
+        out = torch.empty_strided((B, U, T, HD), (T * U * HD, HD, U * HD, 1), device=v.device, dtype=q.dtype)
         if U == 0:
             q = None
     if v.numel() == 0:
         return out
     if k is not None and k.size(1) == 0:
-        k = None
+        k = k_cache = None
     if cos is not None and cos.dim() != 2:
         cos, sin = cos.reshape(-1, cos.size(-1)), sin.reshape(-1, sin.size(-1))
     args = _ext.SafPagedAppendArgs()
-    _ext.fill(args, k_cache=k_cache if k is not None else None, v_cache=v_cache, page_table=page_table,
-              positions=positions, counts=counts, cos=cos, sin=sin, q_weight=q_weight, k_weight=k_weight)
-    held = [_ext.fill_rows(args, "v", v)]
-    if k is not None:
-        held.append(_ext.fill_rows(args, "k", k))
-    if q is not None:
-        held.append(_ext.fill_rows(args, "q", q))
-        _ext.fill(args, q_out=out)
+    block, fill = ctypes.addressof(args), _ext.desc_fill()
+    tensors = (v, k, q, None if q is None else out, k_cache, v_cache, page_table, positions, counts, cos, sin)
+    held = None
+    mask = fill("paged_append_", block, _APPEND_AT, 7, dev, True, *tensors)
+    if mask:
+        held = _ext.aligned_copies("paged_append_", block, _APPEND_AT, mask, dev, tensors)  # noqa: F841
+    if q_weight is not None or k_weight is not None:  # module parameters, which may need gradients elsewhere
+        fill("paged_append_", block, _WEIGHTS_AT, 0, dev, False, q_weight, k_weight)
     args.eps = eps
     with _ext.on_device(dev):
-        rc = _ext.lib().saf_paged_append(args, _ext.current_stream_ptr(dev))
+        rc = _ext.lib().saf_paged_append(args, _stream(dev))
     if rc:
         _ext.check(rc)
     return out
@@ -98,8 +105,7 @@ def paged_mixed_attn(q, k_cache, v_cache, page_table, lengths, patt, frozen, hid
     Returns (B, H, 1, HD).  A length past the page table, a page id outside
     the caches, and for a frozen head a length past its pattern give NaN rows.
     validate also checks shapes with the reference operator's messages."""
-    dev = v_cache.device
-    _ext.check_inputs("paged_mixed_attn", dev, (q, k_cache, v_cache, page_table, lengths, patt, alpha, rho, z, lse))
+    dev = _ext.device_index("paged_mixed_attn", v_cache)
     if sm_scale is None:
         sm_scale = v_cache.size(-1) ** -0.5
     if alpha is not None and z is None:
@@ -117,24 +123,26 @@ def paged_mixed_attn(q, k_cache, v_cache, page_table, lengths, patt, frozen, hid
                 raise ValueError(f"{name} must have one entry per output head")
             setattr(args, name, c)
     B = page_table.size(0)
-    out = torch.empty((B, H, 1, v_cache.size(-1)), device=dev, dtype=v_cache.dtype)
+    out = torch.empty((B, H, 1, v_cache.size(-1)), device=v_cache.device, dtype=v_cache.dtype)
     if B == 0:
         return out
-    if q is not None and q.numel() > 0:
-        q = _ext.fill_rows(args, "q", q)
-    else:
-        k_cache = None
-    _ext.fill(args, k_cache=k_cache, v_cache=v_cache, out=out, lse=lse, patt=patt, alpha=alpha, rho=rho, z=z,
-              page_table=page_table, lengths=lengths)
+    if q is None or q.numel() == 0:
+        q = k_cache = None
+    block = ctypes.addressof(args)
+    tensors = (q, k_cache, v_cache, out, lse, patt, alpha, rho, z, page_table, lengths)
+    held = None
+    mask = _ext.desc_fill()("paged_mixed_attn", block, _ATTN_AT, 1, dev, True, *tensors)
+    if mask:
+        held = _ext.aligned_copies("paged_mixed_attn", block, _ATTN_AT, mask, dev, tensors)  # noqa: F841
     args.n_heads = H
     args.sm_scale = sm_scale
     L = _ext.lib()
     with _ext.on_device(dev):
         nbytes = L.saf_paged_attn_workspace_bytes(args)
         if nbytes > 0:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=v_cache.device)
             args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-        rc = L.saf_paged_attn_fwd(args, _ext.current_stream_ptr(dev))
+        rc = L.saf_paged_attn_fwd(args, _stream(dev))
     if rc:
         _ext.check(rc)
     return out
