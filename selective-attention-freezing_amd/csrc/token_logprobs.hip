@@ -517,14 +517,16 @@ static hipError_t launch_logprob_nt(const LogprobParams& p, hipStream_t s) {
 
 // Threads per row (or segment): one wave where a row is at most eight pieces per
 // lane (4096 rows of 4000, top 10: 12 us against 21 with 256 threads, whose
-// barriers cost more than the row), 512 where a row has a CU to itself (200 rows
-// of 151936: 18 us against 22), else 256 (8192 rows of 50304, top 10: 165 us
-// against 182 with 512; with one wave the second look at the top threads' pieces
-// is a long chain, 243).
+// barriers cost more than the row); 512 for long rows without alternatives (8192
+// rows of 50304: 130 us against 137 with 256, 6.3 TB/s) and where a row has a CU
+// to itself (200 rows of 151936, top 5: 18 us against 22); else 256 (8192 rows of
+// 50304, top 10: 158 us against 209 with 512, whose sorts and barriers leave the
+// CU idle; with one wave the second look at the top threads' pieces is a long
+// chain, 243).
 template <typename T> static hipError_t launch_logprob_t(const LogprobParams& p, hipStream_t s) {
   const int pieces = p.seg_len / Chunk<T>::N;
   if (pieces <= 512) return launch_logprob_nt<T, 64>(p, s);
-  if (pieces >= 4096 && p.R * p.n_seg <= p.n_cu) return launch_logprob_nt<T, 512>(p, s);
+  if (pieces >= 4096 && (p.top == 0 || p.R * p.n_seg <= p.n_cu)) return launch_logprob_nt<T, 512>(p, s);
   return launch_logprob_nt<T, 256>(p, s);
 }
 
