@@ -76,16 +76,18 @@ int check_vec(const saf_tensor_t& t, const char* name, int64_t n) {
 // resident workgroups idle, into as many ranges together as fill them once
 // (whole rounds cost more than a ragged tail: 64 sequences of up to 4096 keys,
 // 768 units for 768 workgroups, took 86 us whole, 94 us in two ranges each,
-// 106 us in eight), of at least kMinKeys keys, and not below kSplitFrom
-// positions, where the second launch costs what the shorter walk saves (one
-// sequence of 1024 keys: 9.2 us either way and 4.6 us more host time; of 2000
-// keys in a group of seven: 21 us whole, 12 us cut).  Ranges dealt over all
+// 106 us in eight), of at least kMinKeys keys, and only where a unit's keys and
+// values reach kSplitBytes (one CU reads about 55 GB/s): below, the second
+// launch and its 4.6 us of host time cost what the shorter walk saves (256 KB,
+// 12 heads of 1024 keys: 9.1 us whole, 10.7 us cut; 500 KB: 15.0 and 10.6; 512
+// KB in two groups of seven: 18.9 and 12.6; 750 KB: 17.3 and 11.5).  Ranges dealt over all
 // sequences instead of an equal number to each: 16 ragged sequences in two KV
 // groups 25 us against 29, 8 at hd 256 69 against 73.  Uncut sequences from
 // kWideFrom positions on run eight waves where the registers allow (64 x 4096
 // keys: 80 us against 86; 128 x 8192 keys at hd 128: 422 against 442); short
 // ones four (64 x 128 keys: 7.4 us against 12.6, idle waves cost their launch).
-constexpr int kMinKeys = 256, kSplitFrom = 1536, kWideFrom = 2048;
+constexpr int kMinKeys = 256, kWideFrom = 2048;
+constexpr int64_t kSplitBytes = 512 << 10;
 constexpr int kWeightFloats = 6144;  // 24 KB: five workgroups of a CU fit its LDS with their partial sums
 
 int plan_paged(const saf_paged_attn_args* a, PagedAttnParams& p, int& dtype, int& hd) {
@@ -224,7 +226,8 @@ int plan_paged(const saf_paged_attn_args* a, PagedAttnParams& p, int& dtype, int
   int64_t ranges = slots / nu;
   const int64_t most = ((int64_t)p.capacity + kMinKeys - 1) / kMinKeys * B;
   if (ranges > most) ranges = most;
-  p.n_ranges = ranges >= 2 * B && B > 0 && p.capacity >= kSplitFrom ? (int)ranges : 1;
+  const int64_t unit_bytes = (int64_t)p.capacity * hd * elem_size(dtype) * 2;
+  p.n_ranges = ranges >= 2 * B && B > 0 && unit_bytes >= kSplitBytes ? (int)ranges : 1;
   p.chunk = p.n_ranges > 1 ? kMinKeys : (p.capacity + 31) / 32 * 32;
   if (p.chunk < 32) p.chunk = 32;
   p.waves = p.n_ranges == 1 && p.capacity >= kWideFrom ? paged_max_waves(elem_size(dtype), hd) : 4;
