@@ -14,7 +14,7 @@ REPO = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "kernel", "libsafattn.so")
-DESC = os.path.join(HERE, "kernel", "_desc.so")
+BIND = os.path.join(HERE, "kernel", "_bind.so")
 SOURCES = ("saf_capi.hip", "flash_fwd.hip", "frozen_pv.hip", "frozen_scan.hip", "rope.hip", "layernorm.hip",
            "attn_bwd.hip", "decomp_logz.hip", "attn_f32.hip", "proj_gemm.hip", "saf_capi_decode.hip",
            "paged_attn.hip", "paged_append.hip", "token_logprobs.hip")
@@ -56,23 +56,24 @@ def _run(cmd):
     return "\n".join(lines)
 
 
-def _desc_cmd(out):
-    """Compile command of the CPython module kernel._desc (csrc/py_desc.cpp),
+def _bind_cmd(out):
+    """Compile command of the CPython module kernel._bind (csrc/py_bind.cpp),
     against the headers and libraries of the installed torch."""
     import sysconfig
     import torch
     from torch.utils.cpp_extension import include_paths
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     incs = [i for p in (*include_paths(), sysconfig.get_paths()["include"], os.path.join(REPO, "include"))
-            for i in ("-I", p)]
+            for i in ("-I", p)] + ["-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *incs,
-            os.path.join(CSRC, "py_desc.cpp"), "-o", out, "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10"]
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1",
+            "-DUSE_ROCM=1", *incs,
+            os.path.join(CSRC, "py_bind.cpp"), "-o", out, "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10", "-lamdhip64"]
 
 
 def build(verbose=False, jobs=None):
     """Compile every HIP source for gfx950 and link kernel/libsafattn.so, and
-    the CPython module kernel/_desc.so."""
+    the CPython module kernel/_bind.so."""
     os.makedirs(BUILD, exist_ok=True)
     hipcc = _hipcc()
     objs = []
@@ -81,7 +82,7 @@ def build(verbose=False, jobs=None):
         obj = os.path.join(BUILD, src.replace(".hip", ".o"))
         objs.append(obj)
         cmds.append([hipcc, *HIPCC_FLAGS, *SOURCE_FLAGS.get(src, ()), "-c", os.path.join(CSRC, src), "-o", obj])
-    cmds.append(_desc_cmd(DESC + ".tmp"))
+    cmds.append(_bind_cmd(BIND + ".tmp"))
     jobs = jobs or min(len(cmds), max(1, os.cpu_count() or 1))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         for out in ex.map(_run, cmds):
@@ -90,7 +91,7 @@ def build(verbose=False, jobs=None):
     tmp = OUT + ".tmp"
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs])
     os.replace(tmp, OUT)
-    os.replace(DESC + ".tmp", DESC)
+    os.replace(BIND + ".tmp", BIND)
     if verbose:
         print(f"built {OUT}")
     return OUT

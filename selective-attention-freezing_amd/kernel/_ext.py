@@ -217,20 +217,25 @@ def set_desc(args, offset, t):
     _DESC.pack_into(args, offset, *_desc_values(t))
 
 
-_desc_fill = None
+_bind = None
 
 
-def desc_fill():
-    """kernel._desc.fill (csrc/py_desc.cpp), loaded once per process."""
-    global _desc_fill
-    if _desc_fill is None:
+def bind():
+    """The module kernel._bind (csrc/py_bind.cpp), loaded once per process and
+    given the library's entry points."""
+    global _bind
+    if _bind is None:
         try:
-            from . import _desc
+            from . import _bind as module
         except ImportError as e:
-            raise RuntimeError("kernel/_desc.so is not built or does not load: run __graft_entry__.build() (or "
+            raise RuntimeError("kernel/_bind.so is not built or does not load: run __graft_entry__.build() (or "
                                "build_ext.build()) first") from e
-        _desc_fill = _desc.fill
-    return _desc_fill
+        L = lib()
+        module.library(*[ctypes.cast(getattr(L, n), ctypes.c_void_p).value
+                         for n in ("saf_token_logprobs", "saf_token_logprobs_workspace_bytes", "saf_token_logprobs_bwd",
+                                   "saf_last_error")])
+        _bind = module
+    return _bind
 
 
 def offsets(block, *names):
@@ -250,7 +255,7 @@ def aligned_copies(what, block, at, mask, index, tensors):
     tensors in the mask, described in their places; the caller keeps them
     until the call is enqueued."""
     held = [t.clone(memory_format=torch.contiguous_format) if mask >> i & 1 else None for i, t in enumerate(tensors)]
-    desc_fill()(what, block, at, 0, index, False, *held)
+    bind().fill(what, block, at, 0, index, False, *held)
     return held
 
 

@@ -73,7 +73,7 @@ def paged_append_(k, v, k_cache, v_cache, page_table, positions, counts=None, q=
     if cos is not None and cos.dim() != 2:
         cos, sin = cos.reshape(-1, cos.size(-1)), sin.reshape(-1, sin.size(-1))
     args = _ext.SafPagedAppendArgs()
-    block, fill = ctypes.addressof(args), _ext.desc_fill()
+    block, fill = ctypes.addressof(args), _ext.bind().fill
     tensors = (v, k, q, None if q is None else out, k_cache, v_cache, page_table, positions, counts, cos, sin)
     held = None
     mask = fill("paged_append_", block, _APPEND_AT, 7, dev, True, *tensors)
@@ -131,7 +131,7 @@ def paged_mixed_attn(q, k_cache, v_cache, page_table, lengths, patt, frozen, hid
     block = ctypes.addressof(args)
     tensors = (q, k_cache, v_cache, out, lse, patt, alpha, rho, z, page_table, lengths)
     held = None
-    mask = _ext.desc_fill()("paged_mixed_attn", block, _ATTN_AT, 1, dev, True, *tensors)
+    mask = _ext.bind().fill("paged_mixed_attn", block, _ATTN_AT, 1, dev, True, *tensors)
     if mask:
         held = _ext.aligned_copies("paged_mixed_attn", block, _ATTN_AT, mask, dev, tensors)  # noqa: F841
     args.n_heads = H

@@ -260,26 +260,33 @@ def test_logprob_graph_forward_and_backward():
         assert all(torch.equal(a, b) for a, b in zip(out, want)), i
 
 
-def test_capture_is_refused_while_an_eager_graph_of_the_leaf_lives():
+@pytest.mark.parametrize("view", [False, True])
+def test_capture_is_refused_while_an_eager_graph_of_the_leaf_lives(view):
     """The refusal comes before anything is captured (the capture itself would
     end the process in torch's engine)."""
-    x = torch.randn(4, 1000, device="cuda").requires_grad_()
-    t = torch.zeros(4, dtype=torch.long, device="cuda")
+    x = torch.randn(2, 2, 1000, device="cuda") if view else torch.randn(4, 1000, device="cuda")
+    x.requires_grad_()
+    t = torch.zeros(x.shape[:-1], dtype=torch.long, device="cuda")
     alive = kernel.token_logprobs(x, t)
     side = torch.cuda.Stream()
-    edge = torch.autograd.graph.get_gradient_edge(x)
-    assert edge.node.metadata["saf_stream"] == torch.cuda.current_stream().cuda_stream
+    side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):                # another stream, no capture: allowed
         kernel.token_logprobs(x, t)
     torch.cuda.synchronize()
-    from unittest import mock
-    with torch.cuda.stream(side), mock.patch("torch.cuda.is_current_stream_capturing", return_value=True):
-        with pytest.raises(RuntimeError, match="still alive"):
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph):
             kernel.token_logprobs(x, t)
-        with torch.no_grad():
-            kernel.token_logprobs(x, t)
-        del alive, edge
-        kernel.token_logprobs(x, t)              # released: allowed
+    torch.cuda.synchronize()
+    assert torch.isfinite(alive.logp).all()
+    del alive
+    with torch.no_grad():                        # no gradient: nothing to refuse
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            r = kernel.token_logprobs(x, t)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(r.logp, kernel.token_logprobs(x.detach(), t).logp)
 
 
 def test_training_loss_and_gradients():
