@@ -10,6 +10,9 @@ Same import surface as the reference's ``kernel`` package
 
 The attention operators run hand-written gfx950 HIP kernels from
 libsafattn.so (see include/saf_attn.h); there is no Triton and no CPU path.
+Behind the prefill: ``paged_append_`` and ``paged_mixed_attn`` (single-token
+attention over a paged cache), ``token_logprobs`` (log probabilities, entropy,
+alternatives, with gradients).
 """
 from .frozen_attn import frozen_pv, frozen_pv_usable, HAVE_TRITON
 from .indexed_linear import linear_rows, linear_rows2, linear_permuted_cols

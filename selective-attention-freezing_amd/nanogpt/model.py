@@ -29,7 +29,8 @@ Differences that follow from the MI355X design:
     scan kernel.
 There is no CPU path: on a CPU tensor ``fused_mixed_attn`` raises.  The
 randomisation ablations, stateful blocks, checkpoint loading and training
-utilities of the reference model are outside this path.
+utilities of the reference model are outside this path.  Decoding (a paged
+cache, one token per step) is in ``nanogpt.decode``.
 """
 import math
 import os
