@@ -9,8 +9,9 @@
 // 4 in float32), the lanes of a row are an aligned power-of-two group, and the
 // rows of one token (its q, k and v heads) follow each other, so a wave reads
 // and writes whole rows.  The bound is HBM for prompts (8 ragged prompts of up
-// to 4096 tokens, 9 + 9 + 12 heads of 64: 38 us, 4.7 TB/s read and written) and
-// the launch for single tokens (64 tokens, 14 + 2 + 2 heads: 4 us).
+// to 4096 tokens, 9 + 9 + 12 heads of 64: 39 us, 4.6 TB/s read and written) and
+// the launch for single tokens (64 tokens, 14 + 2 + 2 heads: 3.9 us replayed as
+// a graph, 7.7 us a call).
 #include "saf_kernels.h"
 
 namespace saf {

@@ -28,9 +28,10 @@
 // first (their small ones would be subnormal: weights above 255 overflow).
 //
 // Measured: 128 ragged sequences of up to 8192 keys, 8 KV heads of 128, 2.3 GB:
-// 422 us, 5.5 TB/s; one sequence of 65537 keys, 16 heads of 128, fp16: 84 us and
-// 5 us for the join; 64 ragged sequences of up to 4096 keys, 12 heads of 64: 80
-// us, 4.7 TB/s; one sequence of 1024 keys: 9 us.
+// 423 us, 5.5 TB/s; one sequence of 65537 keys, fp16 at hd 128: 90 us with the
+// join, 5.2 TB/s; 64 ragged sequences of up to 4096 keys, 12 heads of 64: 80 us,
+// 4.7 TB/s; one sequence of 1024 keys: 9.1 us.  (Graph replays on one input;
+// the Infinity Cache serves the last one and a part of the two before it.)
 #include "saf_kernels.h"
 
 namespace saf {

@@ -20,10 +20,11 @@
 // Few long rows are cut into segments, one workgroup each; a second kernel
 // joins the segments' sums and merges their sorted top lists.
 //
-// Measured: 8192 x 50304 bf16 130 us (6.3 TB/s), with entropy and 10
-// alternatives 158 us, its gradient 277 us (5.9 TB/s read and written); 511 x
-// 50257 fp32, entropy and 20 alternatives, 26 us; 4 x 151936, 5 alternatives,
-// 10 us.
+// Measured: 8192 x 50304 bf16 133 us replayed on one input, partly from the
+// Infinity Cache, and 170 us (4.9 TB/s) behind its gradient, which takes 271 us
+// (6.1 TB/s read and written); with entropy and 10 alternatives 157 us a call
+// (5.3 TB/s).  511 x 50257 fp32, entropy and 20 alternatives, 31 us, 26 us from
+// the cache; 4 x 151936, 5 alternatives, 10.3 us with the join.
 #include "saf_kernels.h"
 
 namespace saf {

@@ -6,7 +6,7 @@ alternatives (libsafattn.so ``saf_token_logprobs``); its backward writes the
 logits' gradient in one pass (``saf_token_logprobs_bwd``), so
 ``-token_logprobs(logits, tokens).logp.mean()`` is the cross-entropy loss.  It
 serves the evaluation that the reference does with log_softmax and gather
-(/root/reference/nanogpt/eval_nanogpt_logprobs.py) and sampling loops that
+(nanogpt/eval_nanogpt_logprobs.py) and sampling loops that
 report alternatives.
 """
 from typing import NamedTuple, Optional
