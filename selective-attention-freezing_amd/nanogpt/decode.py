@@ -36,12 +36,13 @@ class PagedCache:
         p = model.lm_head.weight
         dev, dt, hd = p.device, p.dtype, cfg.n_embd // cfg.n_head
         self.max_length, self.page_size = max_length, page_size
-        self.layers, self._live = [], []
+        self.layers, self._live, self._seen = [], [], []
         for attn in model.attn_modules():
             live = self._live_heads(attn)
             kc = torch.empty(n_pages, len(live), page_size, hd, device=dev, dtype=dt) if live else None
             self.layers.append((kc, torch.empty(n_pages, cfg.n_head, page_size, hd, device=dev, dtype=dt)))
             self._live.append(live)
+            self._seen.append(attn._uf_idx)
         self.page_table = torch.full((batch, per_seq), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.active = torch.ones(batch, dtype=torch.int32, device=dev)
@@ -58,9 +59,13 @@ class PagedCache:
         return attn._uf_idx.tolist()
 
     def check(self, model):
-        for attn, live in zip(model.attn_modules(), self._live):
-            if attn._fz_dirty and self._live_heads(attn) != live:
-                raise RuntimeError("the model's live heads changed since the cache was made")
+        # a refresh of a layer's freeze tables, here or in another forward, makes
+        # a new _uf_idx: only then are its heads read back
+        for i, attn in enumerate(model.attn_modules()):
+            if attn._fz_dirty or attn._uf_idx is not self._seen[i]:
+                if self._live_heads(attn) != self._live[i]:
+                    raise RuntimeError("the model's live heads changed since the cache was made")
+                self._seen[i] = attn._uf_idx
 
     def reserve(self, new):
         """Pages for `new` more tokens of every active sequence (a number, or
