@@ -116,9 +116,13 @@ def prefill(model, idx, cache, counts=None):
         raise ValueError("prefill starts from empty sequences (PagedCache.release)")
     if not 1 <= min(counts) or max(counts) > T:
         raise ValueError("counts must lie between 1 and the prompts' width")
-    cache._on = [True] * B
+    on, cache._on = cache._on, [True] * B
+    try:
+        cache.reserve(counts)
+    except ValueError:
+        cache._on = on
+        raise
     cache.active.fill_(1)
-    cache.reserve(counts)
     n = torch.tensor(counts, dtype=torch.int32, device=idx.device)
     start = torch.zeros_like(n)
 

@@ -33,3 +33,14 @@ def test_changed_live_heads_are_seen_after_another_forward():
     for _ in range(2):
         with pytest.raises(RuntimeError, match="live heads changed"):
             cache.check(m)
+
+
+def test_refused_prefill_changes_nothing():
+    m = _model()
+    cache = decode.PagedCache(m, 2, page_size=16, n_pages=3)
+    cache.release(1)
+    with pytest.raises(ValueError, match="used up"):
+        decode.prefill(m, torch.zeros(2, 40, dtype=torch.long), cache)
+    assert cache._on == [True, False] and cache.active.tolist() == [1, 0]
+    assert cache._held == [0, 0] and len(cache._free) == 3
+    assert (cache.page_table == -1).all()
