@@ -142,7 +142,8 @@ def decode_tokens(model, tokens, cache):
     tr = model.transformer
     pos = cache.lengths
     lengths = pos + cache.active
-    x = tr.wte(tokens.view(-1, 1))
+    # an inactive sequence's token may be anything: token 0 stands for it
+    x = tr.wte(torch.where(cache.active > 0, tokens.reshape(-1), 0)[:, None])
     if model.rotary is None:
         x = x + tr.wpe(pos.long().clamp(max=model.config.block_size - 1))[:, None]
     fused = x.dtype in (torch.bfloat16, torch.float16) and x.size(-1) <= 2048

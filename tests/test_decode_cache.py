@@ -44,3 +44,17 @@ def test_refused_prefill_changes_nothing():
     assert cache._on == [True, False] and cache.active.tolist() == [1, 0]
     assert cache._held == [0, 0] and len(cache._free) == 3
     assert (cache.page_table == -1).all()
+
+
+@pytest.mark.parametrize("token", [-1, -100, 128])
+def test_inactive_sequences_ignore_their_token(token, monkeypatch):
+    """Also one that is no token at all, before it reaches the embedding."""
+    m = _model()
+    cache = decode.PagedCache(m, 2, page_size=16)
+    cache.release(1)
+    seen = []
+    wte = m.transformer.wte.forward
+    monkeypatch.setattr(m.transformer.wte, "forward", lambda t: seen.append(t.clone()) or wte(t))
+    with pytest.raises(RuntimeError, match="HIP devices only"):   # past the embedding
+        decode.decode_step(m, torch.tensor([5, token]), cache)
+    assert seen[0].reshape(-1)[0] == 5 and 0 <= int(seen[0].reshape(-1)[1]) < 128
