@@ -14,7 +14,8 @@ cache unusable (checked at each call).  Inference only.
 
 ``decode_tokens`` is the device half of ``decode_step``: it reads no host state,
 so it can be captured into a HIP graph; ``cache.reserve(1)`` before each replay
-provides the pages.
+provides the pages, and ``cache.check(model)`` after a change of trainable
+patterns their normalisers.
 """
 import torch
 
@@ -66,6 +67,8 @@ class PagedCache:
                 if self._live_heads(attn) != self._live[i]:
                     raise RuntimeError("the model's live heads changed since the cache was made")
                 self._seen[i] = attn._uf_idx
+            if attn._dec_any and attn._patterns is not None:
+                attn._patterns.step_z(attn)
 
     def reserve(self, new):
         """Pages for `new` more tokens of every active sequence (a number, or

@@ -566,8 +566,7 @@ class CausalSelfAttention(nn.Module):
         pk = {}
         if self._dec_any:
             if self._patterns is not None:
-                pk = self._patterns.kernel_inputs(self, self.block_size)
-                pk.pop("closed_form")
+                pk = self._patterns.step_inputs(self)
             else:
                 pk = dict(alpha=self.dyn_alpha, rho=self.dyn_rho, z=self.dyn_z)
         out = _kernel_mod.paged_mixed_attn(rotated, kc, vc, table, lengths, self.dyn_pattern, self._fz_mask_i32,

@@ -17,7 +17,8 @@ and trains them through the frozen path.  This module keeps its entry points
   model's pattern generation is unchanged and the two parameters' version
   counters are the ones it was computed from; the optimizer's step hook
   (``attach_optimizer``) advances the generation, since a fused step need not
-  bump version counters;
+  bump version counters.  Decoding has normalisers of its own (``step_z``),
+  which prefills do not replace;
 * ``state_dict()`` of a trainable layer reports the normalisers of the current
   parameters under ``dyn_z`` (a state-dict post-hook rewrites that entry; the
   module's own buffer is left alone);
@@ -55,6 +56,10 @@ def _host_states(attn):
     return _host_table(attn._fz_mask_i32)
 
 
+def _capturing(t):
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class TrainablePatterns:
     """The trainable alpha / rho of one model and the normalisers derived
     from them."""
@@ -66,6 +71,7 @@ class TrainablePatterns:
         self.layers = []           # attention modules with trainable patterns
         self.generation = 0        # advanced by the optimizer step hook
         self._z = {}               # attn -> (T, stamp, z)
+        self._step_z = {}          # attn -> (stamp, z over the whole block)
         for attn in _attn_modules(model):
             dec = getattr(attn, "dyn_decomp", None)
             if dec is None or getattr(attn, "dyn_alpha", None) is None:
@@ -89,7 +95,8 @@ class TrainablePatterns:
             attn._fz_dirty = True
 
     def invalidate(self):
-        """Forget every cached z (the parameters changed)."""
+        """Forget every cached z (the parameters changed); step_z keeps its
+        storage, out of date by the generation."""
         self.generation += 1
         self._z.clear()
 
@@ -99,6 +106,10 @@ class TrainablePatterns:
     def z_for(self, attn, T):
         """Row normalisers of attn's current parameters for sequence length T."""
         alpha, rho = attn.dyn_alpha, attn.dyn_rho
+        if _capturing(alpha):
+            # each replay follows the parameters, and an eager call never meets
+            # normalisers that are only recorded
+            return normalisers(alpha, rho, T)
         hit = self._z.get(attn)
         stamp = self._stamp(alpha, rho)
         if hit is not None and hit[0] == T and hit[1] == stamp and hit[2].device == alpha.device:
@@ -107,10 +118,36 @@ class TrainablePatterns:
         self._z[attn] = (T, stamp, z)
         return z
 
+    def step_z(self, attn):
+        """Row normalisers of attn's current parameters over the whole block,
+        for single-token attention.  A captured step reads them at each replay,
+        so their storage stays where it is: changed parameters refresh it in
+        place, and no prefill replaces it.  A capture that finds them out of
+        date records their computation and keeps nothing of it."""
+        alpha, rho = attn.dyn_alpha, attn.dyn_rho
+        hit = self._step_z.get(attn)
+        stamp = self._stamp(alpha, rho)
+        if hit is not None and hit[1].device != alpha.device:
+            hit = None
+        if hit is not None and hit[0] == stamp:
+            return hit[1]
+        with torch.inference_mode(False):   # refreshed later, in whatever mode
+            z = normalisers(alpha, rho, alpha.shape[1])
+            if _capturing(alpha):
+                return z
+            if hit is not None:
+                z = hit[1].copy_(z)
+        self._step_z[attn] = (stamp, z)
+        return z
+
     def kernel_inputs(self, attn, T):
         """fused_mixed_attn keyword arguments of a trainable layer."""
         return dict(alpha=attn.dyn_alpha.detach(), rho=attn.dyn_rho.detach(), z=self.z_for(attn, T),
                     closed_form=None)
+
+    def step_inputs(self, attn):
+        """paged_mixed_attn keyword arguments of a trainable layer."""
+        return dict(alpha=attn.dyn_alpha.detach(), rho=attn.dyn_rho.detach(), z=self.step_z(attn))
 
     def attach_gradient(self, attn, out, v, z):
         """out, with the pattern-parameter gradients of attn's decomposed
