@@ -14,8 +14,9 @@ cache unusable (checked at each call).  Inference only.
 
 ``decode_tokens`` is the device half of ``decode_step``: it reads no host state,
 so it can be captured into a HIP graph; ``cache.reserve(1)`` before each replay
-provides the pages, and ``cache.check(model)`` after a change of trainable
-patterns their normalisers.
+provides the pages, and after a change of weights or trainable patterns
+``cache.check(model)`` what the step derives from them.  A step captured before
+other heads were frozen has to be captured again.
 """
 import torch
 
@@ -67,6 +68,7 @@ class PagedCache:
                 if self._live_heads(attn) != self._live[i]:
                     raise RuntimeError("the model's live heads changed since the cache was made")
                 self._seen[i] = attn._uf_idx
+            attn._infer_weight_cache()
             if attn._dec_any and attn._patterns is not None:
                 attn._patterns.step_z(attn)
 

@@ -181,7 +181,7 @@ class CausalSelfAttention(nn.Module):
         self.register_buffer("dyn_pattern", None)
         self.register_buffer("dyn_pattern_slot", torch.full((H,), -1, dtype=torch.int32))
         self._fz_dirty = True
-        self._wc_key = None
+        self._wc_key = self._wc_qkv = self._wc_qkvb = None
         self._ws_key = None
         # trainable-pattern owner (supplement.enable), consulted per forward
         self._patterns = None
@@ -422,6 +422,14 @@ class CausalSelfAttention(nn.Module):
         y = torch.cat([yu.transpose(1, 2), yf.transpose(1, 2)], dim=2)
         return y.reshape(B, T, C), wc
 
+    @staticmethod
+    def _packed(held, parts):
+        """The parts one after the other, in held's storage where that fits."""
+        new = torch.cat(parts)
+        if held is None or (held.shape, held.dtype, held.device) != (new.shape, new.dtype, new.device):
+            return new
+        return held.copy_(new)
+
     def _infer_weight_cache(self):
         """[Wq[live]; Wk[live]; Wv] gathered once per weight version / freeze
         change, so inference runs ONE projection GEMM for Q/K of the live heads
@@ -432,7 +440,10 @@ class CausalSelfAttention(nn.Module):
         odd multiple of 128 output columns ran 1.5x as long as for the next
         multiple of 256 (M = 16384, K = 768 on MI355X: 1920 columns 72.6 us
         against 46.5 us for 2048, 1664 columns 70.2 us against 43.6 us for
-        1792), the way nanoGPT pads its vocabulary to 50304."""
+        1792), the way nanoGPT pads its vocabulary to 50304.
+
+        A captured step reads these rows at each replay, so they are refreshed
+        in place while their shape stays."""
         qw, kw, vw = self.q_proj.weight, self.k_proj.weight, self.v_proj.weight
         key = tuple((w._version, w.data_ptr()) for w in (qw, kw, vw))
         if self._wc_key != key:
@@ -442,16 +453,21 @@ class CausalSelfAttention(nn.Module):
             pad = -rows % 256
             if pad:
                 ws.append(vw.new_zeros(pad, vw.size(1)))
-            self._wc_qkv = torch.cat(ws).detach()
-            if self.q_proj.bias is None:
-                self._wc_qkvb = None
-            else:
+            bs = None
+            if self.q_proj.bias is not None:
                 bs = [self.v_proj.bias] if uf is None else [
                     self.q_proj.bias.index_select(0, uf), self.k_proj.bias.index_select(0, uf),
                     self.v_proj.bias]
                 if pad:
                     bs.append(self.v_proj.bias.new_zeros(pad))
-                self._wc_qkvb = torch.cat(bs).detach()
+            if qw.is_cuda and torch.cuda.is_current_stream_capturing():
+                # gathered by each replay; an eager call must not meet rows
+                # that are only recorded
+                return torch.cat(ws), None if bs is None else torch.cat(bs)
+            # normal (non-inference) tensors: refreshed in whatever mode
+            with torch.inference_mode(False), torch.no_grad():
+                self._wc_qkv = self._packed(self._wc_qkv, ws)
+                self._wc_qkvb = None if bs is None else self._packed(self._wc_qkvb, bs)
             self._wc_key = key
         return self._wc_qkv, self._wc_qkvb
 

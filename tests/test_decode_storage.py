@@ -1,5 +1,5 @@
 """What a captured decoding step reads stays where it is (CPU): the step's row
-normalisers of trainable patterns."""
+normalisers of trainable patterns, and the packed projection weights."""
 import pytest
 import torch
 
@@ -79,3 +79,41 @@ def test_a_capture_keeps_nothing(patterns, what, monkeypatch):
         assert call() is not z              # a replay follows the parameters
     else:
         assert call() is z                  # refreshed in place, outside the capture
+
+
+def test_packed_weights_are_refreshed_in_place():
+    """eval() again, or changed weights: the same storage with the current
+    rows, whichever mode made it; other live heads: their rows."""
+    m = _model().eval()
+    attn = m.transformer.h[1].attn
+    attn._refresh_freeze_cache()
+    with torch.inference_mode():
+        w, b = attn._infer_weight_cache()
+    assert b is None and torch.equal(w[:128], attn.q_proj.weight)
+    m.train()
+    m.eval()
+    with torch.no_grad():
+        attn.q_proj.weight[5] += 1.0
+        assert attn._infer_weight_cache()[0] is w and torch.equal(w[:128], attn.q_proj.weight)
+    attn.dyn_frozen[0] = True
+    attn._refresh_freeze_cache()
+    with torch.inference_mode():
+        fewer, _ = attn._infer_weight_cache()
+    assert torch.equal(fewer[:96], attn.q_proj.weight[32:]) and torch.equal(fewer[192:320], attn.v_proj.weight)
+    m.to(torch.bfloat16)
+    with torch.no_grad():
+        assert torch.equal(attn._infer_weight_cache()[0][:96], attn.q_proj.weight[32:])
+
+
+def test_packed_biases_are_refreshed_in_place():
+    from nanogpt.model import GPT, GPTConfig
+    torch.manual_seed(0)
+    m = GPT(GPTConfig(block_size=64, vocab_size=256, n_layer=1, n_head=4, n_embd=128, bias=True,
+                      rand_attn_prior_repr="dense")).eval()
+    attn = m.transformer.h[0].attn
+    attn._refresh_freeze_cache()
+    with torch.no_grad():
+        b = attn._infer_weight_cache()[1]
+        attn.v_proj.bias += 2.0
+        attn.v_proj.weight += 1.0           # the weights' versions are the key
+        assert attn._infer_weight_cache()[1] is b and torch.equal(b[256:384], attn.v_proj.bias)

@@ -68,3 +68,32 @@ def test_trainable_patterns(warm):
         cache.check(m)
         _replays(m, x, 64, 3, graph, logits, tok, cache, twin)
         assert len(held) > 0
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_packed_weights(bias):
+    """eval() again and a prefill, which packs the projection weights anew,
+    leave the captured step's rows in place; so does a change of the weights,
+    which the step follows."""
+    if bias:
+        from test_gpu_decode import _plain_model
+        m = _plain_model(bias=True, frozen=(1,))
+        x = torch.randint(0, 512, (1, 128), generator=torch.Generator().manual_seed(3)).cuda()
+    else:
+        m, x = _small_model(T=128, layers=2, device="cuda", dtype=BF16)
+    with torch.no_grad():
+        twin, cache = decode.PagedCache(m, 1, page_size=16), decode.PagedCache(m, 1, page_size=16)
+        decode.prefill(m, x[:, :60], twin)
+        decode.prefill(m, x[:, :60], cache)
+        tok = x[0, 60:61].clone()
+        graph, logits = _capture(m, tok, cache)
+        _replays(m, x, 60, 2, graph, logits, tok, cache, twin)
+        m.train()
+        m.eval()
+        decode.prefill(m, x[:, :37], decode.PagedCache(m, 1, page_size=16))
+        held = _junk()
+        _replays(m, x, 62, 2, graph, logits, tok, cache, twin)
+        m.transformer.h[1].attn.v_proj.weight.mul_(1.5)
+        cache.check(m)
+        _replays(m, x, 64, 2, graph, logits, tok, cache, twin)
+        assert len(held) > 0
