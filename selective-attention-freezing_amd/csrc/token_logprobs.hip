@@ -143,7 +143,8 @@ struct Sums {
   template <bool ENT> __device__ inline void raise(float m_new, float sl2) {
     const Anchor a(m, sl2), b(m_new, sl2);
     const bool none = m == -INFINITY;
-    const float d = none ? 0.f : fmaxf(a.wide || b.wide ? (a.m - b.m) * sl2 : a.ref - b.ref, -1000.f);
+    // not a.ref - b.ref, which the compiler may form as fma(a.m, sl2, -b.ref)
+    const float d = none ? 0.f : fmaxf(fmaf(a.m - b.m, sl2, b.delta() - a.delta()), -1000.f);
     const float f = none ? 0.f : fast_exp2(d);  // times 0 keeps a NaN
     if (ENT) t = f * fmaf(s, d, t);
     s *= f;
