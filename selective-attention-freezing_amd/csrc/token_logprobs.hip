@@ -119,11 +119,11 @@ __device__ inline uint64_t wave_sort_desc(uint64_t x, int lane) {
   return merge_runs<32>(x, lane, true);
 }
 
-// Exponents x' - M of one row or thread, M = m log2 e scale.  Where M is far
-// from overflow they are one FMA against the rounded M: every term of a sum
-// then carries the same offset m sl2 - round(m sl2), which delta() gives back.
-// Elsewhere (a thread or row whose largest logit is near the type's lowest or
-// largest value, as masks leave it) the difference is formed first.
+// Exponents x' - M of one row or thread, M = m log2 e scale.  Below 2^24 they are
+// one FMA against the rounded M: every term of a sum then carries the same offset
+// m sl2 - round(m sl2), at most a half there, which delta() gives back.  Beyond
+// (a thread or row that holds nothing but a mask's value, say -1e10) the offset
+// would overflow 2^offset, and the difference is formed first.
 struct Anchor {
   float m, ref, sl2;
   bool wide;
@@ -131,7 +131,7 @@ struct Anchor {
   __device__ inline Anchor(float m_, float sl2_) : sl2(sl2_) {
     m = m_ == -INFINITY ? 0.f : m_;
     ref = m * sl2;
-    wide = !(fabsf(ref) < 1e38f);
+    wide = !(fabsf(ref) < 16777216.f);
   }
   __device__ inline float exponent(float x) const { return wide ? (x - m) * sl2 : fmaf(x, sl2, -ref); }
   __device__ inline float delta() const { return wide ? 0.f : fmaf(m, sl2, -ref); }

@@ -1,5 +1,6 @@
 """Token log probabilities of logits far from zero against float64: finite mask
-values, and rows that hold nothing else."""
+values of any size, rows that hold nothing else, and maxima around the size
+from which exponents are formed as differences."""
 import math
 
 import pytest
@@ -47,7 +48,7 @@ def _check(x, t, top=4, scale=1.0):
     assert bool(((dx.double().cpu() - want).abs() <= tol).all())
 
 
-MASKS = [-1e4]
+MASKS = [-1e4, -1e9, -1e10, -3e10, -1e20, -1e30, -5e37, -3e38]
 
 
 @pytest.mark.parametrize("value", MASKS)
@@ -69,10 +70,20 @@ def test_mask_values(R, V, dtype, value):
     _check(x, t)
 
 
-@pytest.mark.parametrize("middle", [0.0, 65536.0])
+@pytest.mark.parametrize("value", [1e10, 3e10, 1e30, 3e38])
+def test_large_maximum(value):
+    """One token far above the rest, and a uniform row of such values."""
+    x = torch.randn(2, 3000, generator=torch.Generator().manual_seed(1))
+    x[0, 77] = value
+    x[1] = value
+    _check(x, torch.tensor([77, 5]))
+
+
+@pytest.mark.parametrize("middle", [0.0, 65536.0, 11629080.0, 11629080.0 * 2, 1e9])
 @pytest.mark.parametrize("order", ["up", "down", "mixed"])
 def test_maxima_of_any_size(middle, order):
-    """Rows of whole steps around `middle`, on either side of zero."""
+    """Rows of whole steps around `middle` (11629080 log2 e = 2^24): running
+    maxima that cross the size, on either side of zero."""
     V = 20000
     step = max(1.0, 2.0 ** (math.frexp(middle)[1] - 24))
     base = torch.arange(V) // (V // 40)
@@ -88,3 +99,5 @@ def test_large_scale():
     """A scale (inverse temperature) that puts ordinary logits there."""
     x = torch.arange(700).float().remainder(37)[None] * 2.0 ** -20
     _check(x, torch.tensor([36]), scale=float(2 ** 20))
+    x = (torch.randn(2, 700, generator=torch.Generator().manual_seed(3)) * 3).to(FP16)
+    _check(x, x.float().argmax(-1), scale=3000.0)
