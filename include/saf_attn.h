@@ -422,6 +422,8 @@ typedef struct saf_paged_attn_args {
  * gets zero rows (lse -inf); a length past the table, or a page id outside the
  * cache, gives NaN rows, as does a frozen head whose pattern is shorter than
  * the sequence.  Slots past a sequence's length are not read into the result.
+ * An infinite value of a held token counts as weight times value in float32
+ * does: infinite, NaN where both signs meet or the weight is 0.
  * bf16, fp16 and fp32; HD as in the prefill.  16-bit storage rounds the weights
  * to two 16-bit terms (fp16: pattern weights up to 255). */
 int saf_paged_attn_fwd(const saf_paged_attn_args* args, void* stream);

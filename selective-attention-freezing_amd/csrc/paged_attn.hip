@@ -217,6 +217,12 @@ template <typename T> __device__ inline void store4(T* p, float4 x) {
 }
 template <> __device__ inline void store4<float>(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
 
+template <typename T> __device__ inline float4 load4(const T* p) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  return make_float4(Elem<T>::lo(w.x), Elem<T>::hi(w.x), Elem<T>::lo(w.y), Elem<T>::hi(w.y));
+}
+template <> __device__ inline float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
+
 constexpr int kOPad = 4;  // floats after each column's HD partial sums
 
 // What one wave keeps of its unit while it walks the keys.
@@ -228,6 +234,14 @@ template <typename T, int HD> struct PagedWave {
   float m, l;
   bool bad;
 };
+
+// exp(alpha + rho - z).  Where the weight matters z is close to the sum and their
+// difference exact: the sum's own rounding (TwoSum) is all that large logits lose.
+__device__ inline float decomposed_weight(float a, float d, float z) {
+  const float sum = a + d, back = sum - a;
+  const float lost = sum == -INFINITY ? 0.f : (a - (sum - back)) + (d - back);
+  return fast_exp2(((sum - z) + lost) * kLog2e);
+}
 
 // Weights of the frozen columns for the keys kb0..kb1-1, into w[f][key - kb0]
 // (f = column - nl), before the walk: the waves take runs of 256 keys of one
@@ -265,14 +279,8 @@ __device__ inline void frozen_weights(const PagedAttnParams& p, float* w, int pi
       }
       const float zf = bits_to_f32(z, p.z_dtype);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        // where the weight matters z is close to the sum and their difference
-        // exact: the sum's own rounding (TwoSum) is all that large logits lose
-        const float af = bits_to_f32(a[k], p.a_dtype), df = bits_to_f32(d[k], p.r_dtype);
-        const float sum = af + df, back = sum - af;
-        const float lost = sum == -INFINITY ? 0.f : (af - (sum - back)) + (df - back);
-        x[k] = fast_exp2(((sum - zf) + lost) * kLog2e) * scale;
-      }
+      for (int k = 0; k < 4; ++k)
+        x[k] = decomposed_weight(bits_to_f32(a[k], p.a_dtype), bits_to_f32(d[k], p.r_dtype), zf) * scale;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -483,6 +491,66 @@ struct Ranges {
   }
 };
 
+// Four d of one column's sum over the keys j0..j1-1, where the products of the
+// walk gave NaN: an infinite value times the two terms of its weight (0 inf,
+// inf - inf), or times the weight 0 of a row that a step repeats past the end.
+// Once more then, each value that is not finite times its whole weight (what is
+// finite does not change the sum).  A sum without such a value stays NaN.
+template <typename T, int HD>
+__device__ __forceinline__ float4 sum_of_unfinite(const PagedAttnParams& p, float4 acc, int u, int b, int col, int j0, int j1,
+                                                  float mu, int d) {
+  const int n = p.lengths[b];
+  if (n > p.capacity) return acc;
+  const PagedUnit un = p.unit[u];
+  const int64_t word = p.col[un.c0 + col];
+  const int state = col_state(word), row = col_pat(word);
+  const bool fits = state == 0 || n <= (state == 1 ? p.p_S : p.d_S);
+  const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_sb + col_q(word) * p.q_sh;
+  const T* kc = reinterpret_cast<const T*>(p.kc) + un.k * p.k_sh;
+  const T* vc = reinterpret_cast<const T*>(p.vc) + un.v * p.v_sh;
+  const int32_t* table = p.table + b * p.t_sb;
+  float r[4] = {0.f, 0.f, 0.f, 0.f}, a[4] = {acc.x, acc.y, acc.z, acc.w};
+  int found = 0;  // bit e: a[e] has one
+  for (int j = j0; j < j1; ++j) {
+    const int page = table[j >> p.page_shift], slot = j & ((1 << p.page_shift) - 1);
+    if (page < 0 || page >= p.n_pages) return acc;
+    const float4 v4 = load4(vc + page * p.v_sp + (int64_t)slot * p.v_st + d);
+    const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) any |= !(fabsf(v[e]) < INFINITY);
+    float w = __builtin_nanf("");
+    if (state == 0) {  // a weight that is not finite makes the column's sum of weights NaN
+      if (!any) continue;
+      const T* k = kc + page * p.k_sp + (int64_t)slot * p.k_st;
+      float s = 0.f;
+      for (int c = 0; c < HD; c += 4) {
+        const float4 x = load4(q + c), y = load4(k + c);
+        s = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s))));
+      }
+      w = fast_exp2(s * p.scale_log2 - mu);
+    } else if (!fits) {
+    } else if (state == 1) {
+      w = load_as_f32(p.patt, row * p.p_sh + (n - 1) * p.p_si + j * p.p_sj, p.patt_dtype);
+    } else {
+      w = decomposed_weight(load_as_f32(p.alpha, row * p.a_sh + j * p.a_ss, p.a_dtype),
+                            load_as_f32(p.rho, row * p.r_sh + (n - 1 - j) * p.r_ss, p.r_dtype),
+                            load_as_f32(p.z, row * p.z_sh + (n - 1) * p.z_ss, p.z_dtype));
+    }
+    const bool all = !(fabsf(w) < INFINITY);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (all || !(fabsf(v[e]) < INFINITY)) {
+        r[e] += w * v[e];
+        found |= 1 << e;
+      }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (a[e] != a[e] && (found >> e & 1)) a[e] = r[e];
+  return make_float4(a[0], a[1], a[2], a[3]);
+}
+
 // Grid: one workgroup per (unit, range), units fastest; uncut: per (unit,
 // sequence).
 template <typename T, int HD, bool CUT>
@@ -587,6 +655,15 @@ __global__ __launch_bounds__(64 * paged_max_waves(sizeof(T), HD), paged_simd_wav
       const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * nc + col) * (HD + kOPad) + d);
       ll += f * sm_ml[(w * 16 + col) * 2 + 1];
       acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+    }
+    const float any = (acc.x + acc.y) + (acc.z + acc.w);  // NaN also of +inf and -inf: each is looked at
+    if (any != any) {
+      // the arguments read again, by an address that the compiler does not see
+      // through, so that none of this is kept in registers during the walk
+      // (the kernel has one argument, the start of its segment)
+      uint64_t segment = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+      asm volatile("" : "+v"(segment));
+      acc = sum_of_unfinite<T, HD>(*reinterpret_cast<const PagedAttnParams*>(segment), acc, u, b, col, j0, j1, mu, d);
     }
     if constexpr (CUT) {
       const int64_t slot = (int64_t)item * p.n_heads + c0 + col;
