@@ -4,8 +4,8 @@
 // fill(what, block, offsets, rows, device, refuse_grad, t0, t1, ...) writes the
 // saf_tensor_t of each tensor (None: left as it is) at block + offsets[i].
 // It raises where a tensor is not on HIP device `device`, has more than four
-// dimensions or a dtype the library does not know, or (refuse_grad) needs a
-// gradient while grad mode is on.  Bit i of `rows` asks for rows of tensor i
+// dimensions or a dtype the library does not know, carries a forward-mode
+// tangent, or (refuse_grad) needs a gradient while grad mode is on.  Bit i of `rows` asks for rows of tensor i
 // (4-D, only read) to be 16-byte aligned with a unit last stride; the result
 // has the bits of those that are not.
 //
@@ -30,6 +30,7 @@
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -58,6 +59,12 @@ bool rows_ok(const at::Tensor& x) {
   return true;
 }
 
+// A dual tensor: none of the operators has a forward-mode derivative, and
+// their results would drop the tangent without a word.
+bool has_tangent(const at::Tensor& x) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(0).defined();
+}
+
 PyObject* fill(PyObject*, PyObject* const* args, Py_ssize_t n) {
   constexpr Py_ssize_t kFixed = 6;
   if (n < kFixed || !PyTuple_Check(args[2]) || PyTuple_GET_SIZE(args[2]) != n - kFixed) {
@@ -75,6 +82,7 @@ PyObject* fill(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (o == Py_None) continue;
     if (!THPVariable_Check(o)) return PyErr_Format(PyExc_TypeError, "%s: a tensor is required, got %R", what, Py_TYPE(o));
     const at::Tensor& x = THPVariable_Unpack(o);
+    if (has_tangent(x)) return PyErr_Format(PyExc_NotImplementedError, "%s has no forward-mode derivative", what);
     if (!x.is_cuda() || x.device().index() != device)
       return PyErr_Format(PyExc_ValueError, "%s: a tensor is on %s, expected cuda:%ld", what, x.device().str().c_str(),
                           device);
@@ -271,6 +279,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor &logits = THPVariable_Unpack(args[0]), &tokens = THPVariable_Unpack(args[1]);
   Options o{PyLong_AsLongLong(args[2]), PyLong_AsLongLong(args[5]), PyObject_IsTrue(args[3]) == 1, PyFloat_AsDouble(args[4])};
   if (PyErr_Occurred()) return nullptr;
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(logits), "token_logprobs has no forward-mode derivative");
   TORCH_CHECK_VALUE(logits.is_cuda() && tokens.device() == logits.device(), "token_logprobs: a tensor is on ",
                     tokens.device(), ", expected ", logits.device());
   TORCH_CHECK_NOT_IMPLEMENTED(o.top >= 0 && o.top <= 32, "top = ", o.top, " outside 0..32 or above the vocabulary");

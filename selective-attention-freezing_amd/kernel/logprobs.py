@@ -36,7 +36,8 @@ def token_logprobs(logits, tokens, top=0, entropy=False, scale=1.0, ignore_index
       entropy  also return -sum p log p (nats)
       scale    1 / temperature, > 0
     fp32 arithmetic throughout; the gradient of logp and entropy with respect
-    to the logits is rounded once to their dtype.  As with log_softmax, a row
+    to the logits is rounded once to their dtype (reverse mode, once; logits with
+    a forward-mode tangent are refused).  As with log_softmax, a row
     holding NaN or +inf, or nothing above -inf, gives NaN (its top indices are
     then some indices of the row)."""
     if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:

@@ -14,8 +14,8 @@ page (a power of two, at least 16).  ``page_table`` (B, N) int32 lists each
 sequence's pages: its position s is slot s % PS of page
 ``page_table[b, s // PS]``.  Page ids, positions and lengths are device data
 that no call reads back; what they get wrong shows as NaN, never as a stray
-access (libsafattn.so ``saf_paged_append``, ``saf_paged_attn_fwd``).  Forward
-only.
+access (libsafattn.so ``saf_paged_append``, ``saf_paged_attn_fwd``).  Without
+derivatives: tensors that need a gradient or carry a tangent are refused.
 """
 import ctypes
 
