@@ -110,8 +110,9 @@ class PagedCache:
 
 @torch.no_grad()
 def prefill(model, idx, cache, counts=None):
-    """Run prompts idx (B, T), right-padded where counts (B,) are smaller than
-    T, from empty sequences; returns each prompt's next-token logits (B, vocab)."""
+    """Run prompts idx (B, T), right-padded (with any numbers) where counts
+    (B,) are smaller than T, from empty sequences; returns each prompt's
+    next-token logits (B, vocab)."""
     B, T = idx.shape
     cache.check(model)
     counts = [T] * B if counts is None else [int(c) for c in counts]
@@ -135,6 +136,8 @@ def prefill(model, idx, cache, counts=None):
         kc, vc = layer
         return lambda k, v: _kernel_mod.paged_append_(k, v, kc if k is not None else None, vc, cache.page_table, start, n)
 
+    if min(counts) < T:   # token 0 stands for the padding, which need not be one
+        idx = torch.where(torch.arange(T, device=idx.device) < n[:, None], idx, 0)
     h = model.forward_hidden(idx, [sink(layer) for layer in cache.layers])
     cache.lengths.copy_(n)
     last = h[torch.arange(B, device=idx.device), (n - 1).long()]
