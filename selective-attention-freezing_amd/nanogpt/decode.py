@@ -97,6 +97,16 @@ class PagedCache:
             ids = torch.tensor(self._pages[b], dtype=torch.int32)
             self.page_table[b, :len(ids)].copy_(ids)
 
+    def _back_to(self, held, on):
+        """Undo reservations: the sequences hold `held` tokens again."""
+        self._held, self._on = held, on
+        for b, pages in enumerate(self._pages):
+            keep = -(-held[b] // self.page_size)
+            if len(pages) > keep:
+                self._free += reversed(pages[keep:])
+                del pages[keep:]
+                self.page_table[b, keep:].fill_(-1)
+
     def release(self, b):
         """Give back sequence b's pages; it becomes empty and inactive."""
         self._free += self._pages[b]
@@ -112,7 +122,7 @@ class PagedCache:
 def prefill(model, idx, cache, counts=None):
     """Run prompts idx (B, T), right-padded (with any numbers) where counts
     (B,) are smaller than T, from empty sequences; returns each prompt's
-    next-token logits (B, vocab)."""
+    next-token logits (B, vocab).  A call that raises leaves them empty."""
     B, T = idx.shape
     cache.check(model)
     counts = [T] * B if counts is None else [int(c) for c in counts]
@@ -122,26 +132,30 @@ def prefill(model, idx, cache, counts=None):
         raise ValueError("prefill starts from empty sequences (PagedCache.release)")
     if not 1 <= min(counts) or max(counts) > T:
         raise ValueError("counts must lie between 1 and the prompts' width")
-    on, cache._on = cache._on, [True] * B
+    if T > model.config.block_size:
+        raise ValueError(f"prompts of {T} tokens exceed the model's block size {model.config.block_size}")
+    on = cache._on
     try:
+        cache._on = [True] * B
         cache.reserve(counts)
-    except ValueError:
-        cache._on = on
+        n = torch.tensor(counts, dtype=torch.int32, device=idx.device)
+        start = torch.zeros_like(n)
+
+        def sink(layer):
+            kc, vc = layer
+            return lambda k, v: _kernel_mod.paged_append_(k, v, kc if k is not None else None, vc, cache.page_table, start,
+                                                          n)
+
+        if min(counts) < T:   # token 0 stands for the padding, which need not be one
+            idx = torch.where(torch.arange(T, device=idx.device) < n[:, None], idx, 0)
+        h = model.forward_hidden(idx, [sink(layer) for layer in cache.layers])
+        logits = model.lm_head(h[torch.arange(B, device=idx.device), (n - 1).long()])
+    except BaseException:
+        cache._back_to([0] * B, on)
         raise
-    cache.active.fill_(1)
-    n = torch.tensor(counts, dtype=torch.int32, device=idx.device)
-    start = torch.zeros_like(n)
-
-    def sink(layer):
-        kc, vc = layer
-        return lambda k, v: _kernel_mod.paged_append_(k, v, kc if k is not None else None, vc, cache.page_table, start, n)
-
-    if min(counts) < T:   # token 0 stands for the padding, which need not be one
-        idx = torch.where(torch.arange(T, device=idx.device) < n[:, None], idx, 0)
-    h = model.forward_hidden(idx, [sink(layer) for layer in cache.layers])
     cache.lengths.copy_(n)
-    last = h[torch.arange(B, device=idx.device), (n - 1).long()]
-    return model.lm_head(last)
+    cache.active.fill_(1)
+    return logits
 
 
 @torch.no_grad()
@@ -171,18 +185,25 @@ def decode_tokens(model, tokens, cache):
         y = attn.attend_cached(h, (*cache.layers[i], cache.page_table), pos, lengths, cache.active, cache.rope)
         h = norm(attn.c_proj(y), block.ln_2)
         h = norm(mlp(h), tr.h[i + 1].ln_1 if i + 1 < len(tr.h) else tr.ln_f)
+    logits = model.lm_head(h[:, 0])
     cache.lengths.copy_(lengths)
-    return model.lm_head(h[:, 0])
+    return logits
 
 
 def decode_step(model, tokens, cache):
     """Append tokens (B,) to the sequences (inactive ones ignore theirs) and
-    return the next tokens' logits (B, vocab)."""
+    return the next tokens' logits (B, vocab).  A call that raises leaves the
+    sequences as they were."""
     cache.check(model)
     if tokens.numel() != len(cache._held):
         raise ValueError("one token per sequence of the cache is required")
-    cache.reserve(1)
-    return decode_tokens(model, tokens, cache)
+    held = cache._held
+    try:
+        cache.reserve(1)
+        return decode_tokens(model, tokens, cache)
+    except BaseException:
+        cache._back_to(held, cache._on)
+        raise
 
 
 @torch.no_grad()
