@@ -60,17 +60,24 @@ class PagedCache:
             attn._refresh_freeze_cache()
         return attn._uf_idx.tolist()
 
-    def check(self, model):
+    def check_heads(self, model):
+        """Raise if the model's live heads are not the cache's."""
         # a refresh of a layer's freeze tables, here or in another forward, makes
         # a new _uf_idx: only then are its heads read back
         for i, attn in enumerate(model.attn_modules()):
             if attn._fz_dirty or attn._uf_idx is not self._seen[i]:
+                if self.lengths.is_cuda and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("heads were frozen or unfrozen: call PagedCache.check(model) before the capture")
                 if self._live_heads(attn) != self._live[i]:
                     raise RuntimeError("the model's live heads changed since the cache was made")
                 self._seen[i] = attn._uf_idx
-            attn._infer_weight_cache()
-            if attn._dec_any and attn._patterns is not None:
-                attn._patterns.step_z(attn)
+
+    def check(self, model):
+        """check_heads(), and what a step keeps of the model's weights, freeze
+        states and trainable patterns brought up to date."""
+        self.check_heads(model)
+        for attn in model.attn_modules():
+            attn.prepare_step()
 
     def reserve(self, new):
         """Pages for `new` more tokens of every active sequence (a number, or
@@ -161,6 +168,7 @@ def prefill(model, idx, cache, counts=None):
 @torch.no_grad()
 def decode_tokens(model, tokens, cache):
     """The device half of decode_step (pages are reserved by the caller)."""
+    cache.check_heads(model)
     tr = model.transformer
     pos = cache.lengths
     lengths = pos + cache.active
@@ -194,7 +202,6 @@ def decode_step(model, tokens, cache):
     """Append tokens (B,) to the sequences (inactive ones ignore theirs) and
     return the next tokens' logits (B, vocab).  A call that raises leaves the
     sequences as they were."""
-    cache.check(model)
     if tokens.numel() != len(cache._held):
         raise ValueError("one token per sequence of the cache is required")
     held = cache._held

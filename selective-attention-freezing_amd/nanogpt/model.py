@@ -43,6 +43,7 @@ import torch.nn.functional as F
 from kernel import (fused_mixed_attn, decomposed_logz, classify_closed_form,  # noqa: F401
                     BAND_ROWS)
 import kernel as _kernel_mod
+from kernel.fused_attn import _host_table
 
 # One mixed-head operator call for live and frozen heads (the default).
 # FROZEN_ATTN_FUSED=0 selects the split route instead (nanogpt/model.py:29-32,
@@ -560,6 +561,18 @@ class CausalSelfAttention(nn.Module):
         if dec and self._patterns is not None:
             y = self._patterns.attach_gradient(self, y, v, pk["z"])
         return y.transpose(1, 2).reshape(B, T, nh * hd)
+
+    def prepare_step(self):
+        """Bring up to date what attend_cached keeps between calls (packed
+        weights, host copies of the routing tables, a trainable layer's row
+        normalisers), none of which a capture can do for later calls."""
+        if self._fz_dirty:
+            self._refresh_freeze_cache()
+        self._infer_weight_cache()
+        for t in (self._fz_mask_i32, self._hidx_i32, self._pidx_i32):
+            _host_table(t)
+        if self._dec_any and self._patterns is not None:
+            self._patterns.step_z(self)
 
     def attend_cached(self, x, store, positions, lengths, active, rope=None):
         """attend() of one new token per sequence (inference): x (B, 1, C),
