@@ -644,8 +644,8 @@ class Block(nn.Module):
         self.ln_2 = LayerNorm(config.n_embd, bias=config.bias)
         self.mlp = MLP(config)
 
-    def forward(self, x, rope=None, sink=None):
-        x = x + self.attn(self.ln_1(x), rope=rope, sink=sink)
+    def forward(self, x, rope=None, **sink):
+        x = x + self.attn(self.ln_1(x), rope=rope, **sink)
         return x + self.mlp(self.ln_2(x))
 
 
@@ -701,8 +701,10 @@ class GPT(nn.Module):
         """Hidden states of every position; sinks[i], if given, receives layer
         i's keys and values (CausalSelfAttention.attend)."""
         x, rope = self.prepare_inputs(idx)
-        sinks = sinks or [None] * len(self.transformer.h)
         blocks = self.transformer.h
+        # without sinks a block or attention module is called as ever, also one
+        # of the caller's own that knows of none
+        sinks = [{} for _ in blocks] if sinks is None else [dict(sink=s) for s in sinks]
         if (x.is_cuda and not torch.is_grad_enabled()
                 and x.dtype in (torch.bfloat16, torch.float16)):
             # prefill: each residual add of Block.forward runs fused with the
@@ -718,11 +720,11 @@ class GPT(nn.Module):
             for i, block in enumerate(blocks):
                 attn, mlp = block.attn, block.mlp
                 if attn.c_proj.bias is None:
-                    y, wc = attn.head_outputs(h, rope=rope, sink=sinks[i])
+                    y, wc = attn.head_outputs(h, rope=rope, **sinks[i])
                     x2.addmm_(y.reshape(x2.size(0), -1), wc.t())
                     h = _kernel_mod.add_layernorm_(x, None, block.ln_2.weight, block.ln_2.bias)
                 else:
-                    h = _kernel_mod.add_layernorm_(x, attn(h, rope=rope, sink=sinks[i]), block.ln_2.weight, block.ln_2.bias)
+                    h = _kernel_mod.add_layernorm_(x, attn(h, rope=rope, **sinks[i]), block.ln_2.weight, block.ln_2.bias)
                 ln = blocks[i + 1].ln_1 if i + 1 < len(blocks) else self.transformer.ln_f
                 if mlp.c_proj.bias is None:
                     u = mlp.fc_gelu(h)
@@ -732,7 +734,7 @@ class GPT(nn.Module):
                     h = _kernel_mod.add_layernorm_(x, mlp(h), ln.weight, ln.bias)
             return h
         for block, sink in zip(blocks, sinks):
-            x = block(x, rope=rope, sink=sink)
+            x = block(x, rope=rope, **sink)
         return self.transformer.ln_f(x)
 
     def forward_all_positions(self, idx):
