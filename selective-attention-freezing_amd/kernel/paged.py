@@ -32,6 +32,13 @@ _ATTN_AT = _ext.offsets(_ext.SafPagedAttnArgs, "q", "k_cache", "v_cache", "out",
                         "page_table", "lengths")
 
 
+def _rows_of(t):
+    """A cos / sin cache without its leading singleton dims."""
+    if t.dim() > 2 and t.numel() != t.size(-2) * t.size(-1):
+        raise ValueError(f"cos and sin must be (T', RD) caches, with leading singleton dims at most (got {tuple(t.shape)})")
+    return t.reshape(t.shape[-2:])
+
+
 def paged_append_(k, v, k_cache, v_cache, page_table, positions, counts=None, q=None, cos=None, sin=None,
                   q_weight=None, k_weight=None, eps=1e-6):
     """Write T new tokens per sequence into the caches, in place, rotating
@@ -70,8 +77,8 @@ def paged_append_(k, v, k_cache, v_cache, page_table, positions, counts=None, q=
         return out
     if k is not None and k.size(1) == 0:
         k = k_cache = None
-    if cos is not None and cos.dim() != 2:
-        cos, sin = cos.reshape(-1, cos.size(-1)), sin.reshape(-1, sin.size(-1))
+    if cos is not None and (cos.dim() != 2 or sin.dim() != 2):
+        cos, sin = _rows_of(cos), _rows_of(sin)
     args = _ext.SafPagedAppendArgs()
     block, fill = ctypes.addressof(args), _ext.bind().fill
     tensors = (v, k, q, None if q is None else out, k_cache, v_cache, page_table, positions, counts, cos, sin)
