@@ -73,8 +73,8 @@ def paged_append_(k, v, k_cache, v_cache, page_table, positions, counts=None, q=
         out = torch.empty_strided((B, U, T, HD), (T * U * HD, HD, U * HD, 1), device=v.device, dtype=q.dtype)
         if U == 0:
             q = None
-    if v.numel() == 0:
-        return out
+    if v.numel() == 0 and v.dim() == 4 and v.size(1) and v.size(3):
+        return out   # no sequence or no token
     if k is not None and k.size(1) == 0:
         k = k_cache = None
     if cos is not None and (cos.dim() != 2 or sin.dim() != 2):

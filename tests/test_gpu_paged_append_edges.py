@@ -32,3 +32,14 @@ def test_leading_dims_of_the_rotary_caches():
             call(a, b)
     with pytest.raises(ValueError):
         call(cos[0], sin[0])
+
+
+def test_values_without_heads():
+    """Refused: q rows would come back unwritten."""
+    d = _dev(_case(T=3, seed=2))
+    with pytest.raises(ValueError, match="v and v_cache are required"):
+        kernel.paged_append_(None, d["v"][:, :0], None, d["vc"][:, :0], d["table"], d["positions"], q=d["q"])
+    for shape in ((0, 2, 3, 64), (2, 2, 0, 64)):
+        v = torch.empty(shape, dtype=torch.bfloat16, device="cuda")
+        q = kernel.paged_append_(v, v, d["kc"], d["vc"], d["table"][:shape[0]], d["positions"][:shape[0]], q=v)
+        assert q.shape == shape
