@@ -245,11 +245,23 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
 // A leaf's autograd node belongs to the stream of the call that made it.  A
 // captured backward would make that stream wait for the capturing one, and with
 // it join the capture without ever leaving it: torch ends the process there.
-// So logits that are such a leaf (or a view of one) are refused.
+// So logits that are such a leaf, or come from one by operations of a single
+// input (views, slices, casts), are refused.
 void refuse_foreign_capture(const at::Tensor& logits) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   std::vector<std::shared_ptr<torch::autograd::Node>> leaves;
-  if (const auto fn = logits.grad_fn()) {
+  if (auto fn = logits.grad_fn()) {
+    for (;;) {
+      std::shared_ptr<torch::autograd::Node> only;
+      int n = 0;
+      for (const auto& e : fn->next_edges())
+        if (e.function) {
+          only = e.function;
+          ++n;
+        }
+      if (n != 1 || only->num_outputs() == 0) break;  // the leaf's own node has no next edges
+      fn = std::move(only);
+    }
     for (const auto& e : fn->next_edges())
       if (e.function && e.function->name() == "torch::autograd::AccumulateGrad") leaves.push_back(e.function);
   } else if (auto node = torch::autograd::impl::try_get_grad_accumulator(logits)) {
