@@ -169,6 +169,8 @@ def prefill(model, idx, cache, counts=None):
 def decode_tokens(model, tokens, cache):
     """The device half of decode_step (pages are reserved by the caller)."""
     cache.check_heads(model)
+    if tokens.numel() != len(cache._held):
+        raise ValueError("one token per sequence of the cache is required")
     tr = model.transformer
     pos = cache.lengths
     lengths = pos + cache.active
@@ -202,8 +204,6 @@ def decode_step(model, tokens, cache):
     """Append tokens (B,) to the sequences (inactive ones ignore theirs) and
     return the next tokens' logits (B, vocab).  A call that raises leaves the
     sequences as they were."""
-    if tokens.numel() != len(cache._held):
-        raise ValueError("one token per sequence of the cache is required")
     held = cache._held
     try:
         cache.reserve(1)

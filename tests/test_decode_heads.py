@@ -1,5 +1,6 @@
-"""Changed live heads are noticed by every call on a cache, the capturable half
-of a step among them (CPU), and refused inside a capture."""
+"""Changed live heads and a wrong number of tokens are noticed by every call on a
+cache, the capturable half of a step among them (CPU), and changed heads are
+refused inside a capture."""
 import pytest
 import torch
 
@@ -37,6 +38,17 @@ def test_every_call_checks(call, refreshed):
         with pytest.raises(RuntimeError, match="live heads changed"):
             calls[call]()
         assert cache._held == [0]
+
+
+@pytest.mark.parametrize("call", [decode.decode_tokens, decode.decode_step])
+@pytest.mark.parametrize("n", [0, 1, 2, 6])
+def test_one_token_per_sequence(call, n):
+    """A single token is not spread over the batch."""
+    m = _frozen_model()
+    cache = decode.PagedCache(m, 3, page_size=16)
+    with pytest.raises(ValueError, match="one token per sequence"):
+        call(m, torch.zeros(n, dtype=torch.long), cache)
+    assert cache._held == [0, 0, 0]
 
 
 @pytest.mark.gpu
