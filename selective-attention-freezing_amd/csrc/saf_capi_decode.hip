@@ -78,9 +78,12 @@ int check_vec(const saf_tensor_t& t, const char* name, int64_t n) {
 // 768 units for 768 workgroups, took 86 us whole, 94 us in two ranges each,
 // 106 us in eight), of at least kMinKeys keys, and only where a unit's keys and
 // values reach kSplitBytes (one CU reads about 55 GB/s): below, the second
-// launch and its 4.6 us of host time cost what the shorter walk saves (256 KB,
-// 12 heads of 1024 keys: 9.1 us whole, 10.7 us cut; 500 KB: 15.0 and 10.6; 512
-// KB in two groups of seven: 18.9 and 12.6; 750 KB: 17.3 and 11.5).  Ranges dealt over all
+// launch costs what the shorter walk saves.  As calls the two meet between 448 and
+// 512 KB whatever the type and head dim (12 heads of 64, bf16, whole and cut: 9.8
+// and 13.2 us at 256 KB, 13.8 and 13.4 at 448, 15.8 and 11.8 at 512; 32 heads on 8
+// KV heads of 128: 9.9 and 13.0, 12.9 and 12.7, 14.1 and 13.0; float32: 10.3 and
+// 14.9, 14.1 and 13.7, 15.3 and 15.0), replayed as a graph, without the host's
+// part, between 320 and 448 KB.  Ranges dealt over all
 // sequences instead of an equal number to each: 16 ragged sequences in two KV
 // groups 25 us against 29, 8 at hd 256 69 against 73.  Uncut sequences from
 // kWideFrom positions on run eight waves where the registers allow (64 x 4096

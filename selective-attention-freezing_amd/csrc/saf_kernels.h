@@ -209,7 +209,9 @@ struct ProjGemmParams {
 };
 
 // Waves per SIMD that the paged attention kernel's registers leave (its launch
-// bound) and the largest workgroup, by element size and head dim.
+// bound) and the largest workgroup, by element size and head dim.  Taken from
+// the uncut forms; the cut ones spill at hd 32 (12 VGPRs, float32 7) and, in 16
+// bits, at hd 128 (one).
 constexpr int paged_simd_waves(int es, int hd) {
   return es == 2 ? (hd == 32 ? 5 : (hd == 64 ? 3 : (hd <= 128 ? 2 : 1))) : (hd == 32 ? 4 : (hd == 64 ? 2 : 1));
 }
