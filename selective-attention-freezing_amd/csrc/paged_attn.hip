@@ -544,6 +544,10 @@ __device__ __forceinline__ float4 sum_of_unfinite(const PagedAttnParams& p, floa
         r[e] += w * v[e];
         found |= 1 << e;
       }
+    bool open = false;  // a NaN stays one
+#pragma unroll
+    for (int e = 0; e < 4; ++e) open |= a[e] != a[e] && r[e] == r[e];
+    if (!open) break;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -657,7 +661,7 @@ __global__ __launch_bounds__(64 * paged_max_waves(sizeof(T), HD), paged_simd_wav
       acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
     }
     const float any = (acc.x + acc.y) + (acc.z + acc.w);  // NaN also of +inf and -inf: each is looked at
-    if (any != any) {
+    if (any != any && ll == ll) {  // a NaN sum of weights makes the column NaN as it is
       // the arguments read again, by an address that the compiler does not see
       // through, so that none of this is kept in registers during the walk
       // (the kernel has one argument, the start of its segment)
