@@ -350,12 +350,19 @@ class CausalSelfAttention(nn.Module):
             self._refresh_freeze_cache()
         return not _FUSED and self._n_frozen > 0
 
+    def _versions(self, *weights):
+        """What the gathered copies of these weights, and of the Q / K / V
+        biases, go by."""
+        if self.q_proj.bias is not None:
+            weights += (self.q_proj.bias, self.k_proj.bias, self.v_proj.bias)
+        return tuple((w._version, w.data_ptr()) for w in weights)
+
     def _split_weight_cache(self):
         """Split route, inference: Wv[cperm], [Wq[live]; Wk[live]] and
         Wc[:, cperm] gathered once per weight version / freeze change
         (nanogpt/model.py:920-944)."""
         ws = (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight, self.c_proj.weight)
-        key = tuple((w._version, w.data_ptr()) for w in ws)
+        key = self._versions(*ws)
         if self._ws_key != key:
             qw, kw, vw, cw = ws
             perm, uf = self._cperm_cols, self._uf_cols
@@ -446,7 +453,7 @@ class CausalSelfAttention(nn.Module):
         A captured step reads these rows at each replay, so they are refreshed
         in place while their shape stays."""
         qw, kw, vw = self.q_proj.weight, self.k_proj.weight, self.v_proj.weight
-        key = tuple((w._version, w.data_ptr()) for w in (qw, kw, vw))
+        key = self._versions(qw, kw, vw)
         if self._wc_key != key:
             uf = self._uf_cols
             ws = [vw] if uf is None else [qw.index_select(0, uf), kw.index_select(0, uf), vw]

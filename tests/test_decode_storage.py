@@ -115,5 +115,25 @@ def test_packed_biases_are_refreshed_in_place():
     with torch.no_grad():
         b = attn._infer_weight_cache()[1]
         attn.v_proj.bias += 2.0
-        attn.v_proj.weight += 1.0           # the weights' versions are the key
+        attn.v_proj.weight += 1.0
         assert attn._infer_weight_cache()[1] is b and torch.equal(b[256:384], attn.v_proj.bias)
+
+
+@pytest.mark.parametrize("name", ["q_proj", "k_proj", "v_proj"])
+def test_a_changed_bias_alone_is_noticed(name):
+    from nanogpt.model import GPT, GPTConfig
+    torch.manual_seed(0)
+    m = GPT(GPTConfig(block_size=64, vocab_size=256, n_layer=1, n_head=4, n_embd=128, bias=True,
+                      rand_attn_prior_repr="dense")).eval()
+    attn = m.transformer.h[0].attn
+    attn._refresh_freeze_cache()
+    with torch.no_grad():
+        b = attn._infer_weight_cache()[1]
+        getattr(attn, name).bias.add_(2.0)
+        at = 128 * ["q_proj", "k_proj", "v_proj"].index(name)
+        assert torch.equal(attn._infer_weight_cache()[1][at:at + 128], getattr(attn, name).bias)
+        assert attn._infer_weight_cache()[1] is b
+        vb, qkb = attn._split_weight_cache()[1], attn._split_weight_cache()[3]
+        getattr(attn, name).bias.mul_(-1.0)
+        got = torch.cat([attn._split_weight_cache()[3], attn._split_weight_cache()[1]])
+        assert torch.equal(got[at:at + 128], getattr(attn, name).bias) and got.numel() == vb.numel() + qkb.numel()
