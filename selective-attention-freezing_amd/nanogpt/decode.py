@@ -48,7 +48,8 @@ class PagedCache:
         self.page_table = torch.full((batch, per_seq), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.active = torch.ones(batch, dtype=torch.int32, device=dev)
-        self.rope = model.rotary(cfg.block_size, dt) if model.rotary is not None else None
+        # (positions, hd) rows, as paged_append_ takes them
+        self.rope = tuple(t[0, 0] for t in model.rotary(cfg.block_size, dt)) if model.rotary is not None else None
         self._free = list(range(n_pages - 1, -1, -1))
         self._pages = [[] for _ in range(batch)]
         self._held = [0] * batch    # tokens that pages are reserved for
