@@ -71,7 +71,7 @@ enum {
   SAF_EWORKSPACE = -5     /* workspace missing or too small */
 };
 
-enum { SAF_F32 = 0, SAF_F16 = 1, SAF_BF16 = 2, SAF_I32 = 3, SAF_I64 = 4 };
+enum { SAF_F32 = 0, SAF_F16 = 1, SAF_BF16 = 2, SAF_I32 = 3, SAF_I64 = 4, SAF_I8 = 5, SAF_U8 = 6 };
 
 /* Head states (kernel/fused_attn.py:12-19, nanogpt/model.py:869-874). */
 enum { SAF_LIVE = 0, SAF_FROZEN_DENSE = 1, SAF_FROZEN_DECOMP = 2 };
@@ -85,7 +85,7 @@ enum { SAF_CLOSED_NONE = 0, SAF_CLOSED_MEAN = 1, SAF_CLOSED_DECAY = 2, SAF_CLOSE
 
 typedef struct saf_tensor {
   void* data;         /* device pointer (NULL = absent) */
-  int32_t dtype;      /* SAF_F32 / SAF_F16 / SAF_BF16 / SAF_I32 / SAF_I64 */
+  int32_t dtype;      /* SAF_F32 / SAF_F16 / SAF_BF16 / SAF_I32 / SAF_I64 / SAF_I8 / SAF_U8 */
   int32_t ndim;       /* number of used sizes/strides (<= 4) */
   int64_t size[4];
   int64_t stride[4];  /* in elements */
@@ -463,6 +463,69 @@ int64_t saf_token_logprobs_workspace_bytes(const saf_token_logprobs_args* args);
  * forward wrote them); dlogits (R, V) in the logits' dtype is written. */
 int saf_token_logprobs_bwd(const saf_token_logprobs_args* args, const saf_tensor_t* dlogp,
                            const saf_tensor_t* dentropy, const saf_tensor_t* dlogits, void* stream);
+
+/* ---- around the products of a training step ----------------------------------
+ *
+ * Embedding, residual LayerNorm and 8-bit activations, forward and backward, in
+ * fp32, bf16 and fp16.  2-D operands are rows (R, C) with a unit column stride
+ * and any row stride and alignment; what these entry points write is contiguous
+ * unless said otherwise.  All arithmetic is fp32, each result rounded once.  The
+ * gradients are sums in a fixed order: the same bits in every run. */
+
+/* out[n] = scale weight[tokens[n]] for tokens (N,) int32 / int64, weight (V, C),
+ * out (N, C) of any of the three types (bf16 with fp16 is refused).  Rows of
+ * ignore_index are zero, rows of other tokens outside 0..V-1 NaN. */
+int saf_embed_fwd(const saf_tensor_t* tokens, const saf_tensor_t* weight, float scale, int64_t ignore_index,
+                  const saf_tensor_t* out, void* stream);
+
+/* Gradient of saf_embed_fwd: dweight[v] = scale sum of dout[n] over the n with
+ * tokens[n] = v, added in the order of n; every row of dweight (V, C) is written,
+ * 16-byte aligned.  The workspace (256-byte aligned) is that of N tokens, V and C. */
+int saf_embed_bwd(const saf_tensor_t* tokens, const saf_tensor_t* dout, float scale, int64_t ignore_index,
+                  const saf_tensor_t* dweight, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t saf_embed_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t channels);
+
+/* r = x + delta, rounded to x's dtype, and y = (r - mean) / sqrt(var + eps) weight
+ * + bias over the C channels (at most 16384) of the rounded r.  x and r (R, C) share a
+ * dtype; delta and y share one: x's, or bf16 / fp16 beside an fp32 x.  Without
+ * delta r is x and must be absent.  weight and bias (optional) (C,) share a dtype.
+ * stats (optional) (R, 2) fp32 receives mean and 1 / sqrt(var + eps). */
+int saf_layernorm_fwd(const saf_tensor_t* x, const saf_tensor_t* delta, const saf_tensor_t* weight,
+                      const saf_tensor_t* bias, float eps, const saf_tensor_t* r, const saf_tensor_t* y,
+                      const saf_tensor_t* stats, void* stream);
+
+/* Gradients of saf_layernorm_fwd from r, its stats, dy and (optional) dr: with
+ * xh = (r - mean) rstd and g = dy weight
+ *   dx = dr + rstd (g - mean(g) - xh mean(g xh)),  ddelta = dx in dy's dtype,
+ *   dweight = sum over rows of dy xh,  dbias = sum over rows of dy.
+ * Outputs that are absent are not computed; dweight and dbias need the workspace
+ * (256-byte aligned). */
+int saf_layernorm_bwd(const saf_tensor_t* r, const saf_tensor_t* stats, const saf_tensor_t* weight,
+                      const saf_tensor_t* dy, const saf_tensor_t* dr, const saf_tensor_t* dx,
+                      const saf_tensor_t* ddelta, const saf_tensor_t* dweight, const saf_tensor_t* dbias,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+int64_t saf_layernorm_bwd_workspace_bytes(int64_t rows, int64_t channels);
+
+/* x (R, C) in 8 bits: q (R, C) int8 whole multiples of a step, exp (R, ceil(C /
+ * 32)) uint8 the steps' exponents, one per block of 32 channels of a row (its last
+ * block may be short).  With m the block's largest magnitude the step is
+ * 2^(floor(log2 m) - 6), 2^-127 at least, exp that exponent + 127; q = x / step
+ * rounded to nearest even, at most 127 in magnitude.  A block with an infinity or
+ * NaN has exp 255 and q 0. */
+int saf_act_pack(const saf_tensor_t* x, const saf_tensor_t* q, const saf_tensor_t* exp, void* stream);
+
+/* out (R, C) = q 2^(exp - 127); NaN where exp is 255.  Exact in every type that x
+ * had.  out may have any row stride. */
+int saf_act_unpack(const saf_tensor_t* q, const saf_tensor_t* exp, const saf_tensor_t* out, void* stream);
+
+/* y = x Phi(x) (the exact GELU) and x in 8 bits, in one pass. */
+int saf_gelu_pack_fwd(const saf_tensor_t* x, const saf_tensor_t* y, const saf_tensor_t* q, const saf_tensor_t* exp,
+                      void* stream);
+
+/* dx = dy (Phi(h) + h phi(h)) for the held h = q 2^(exp - 127), and y (optional)
+ * = h Phi(h). */
+int saf_gelu_pack_bwd(const saf_tensor_t* q, const saf_tensor_t* exp, const saf_tensor_t* dy, const saf_tensor_t* dx,
+                      const saf_tensor_t* y, void* stream);
 
 /* Kernel timing: the next main kernel this host thread launches through an
  * attention entry point (the flash, dense P.V, decomposed P.V or scan kernel;

@@ -17,7 +17,9 @@ OUT = os.path.join(HERE, "kernel", "libsafattn.so")
 BIND = os.path.join(HERE, "kernel", "_bind.so")
 SOURCES = ("saf_capi.hip", "flash_fwd.hip", "frozen_pv.hip", "frozen_scan.hip", "rope.hip", "layernorm.hip",
            "attn_bwd.hip", "decomp_logz.hip", "attn_f32.hip", "proj_gemm.hip", "saf_capi_decode.hip",
-           "paged_attn.hip", "paged_append.hip", "token_logprobs.hip")
+           "paged_attn.hip", "paged_append.hip", "token_logprobs.hip", "saf_capi_train.hip", "embed.hip", "layernorm_train.hip",
+           "act_pack.hip")
+BIND_SOURCES = ("py_bind.cpp", "py_bind_train.cpp")
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -56,8 +58,8 @@ def _run(cmd):
     return "\n".join(lines)
 
 
-def _bind_cmd(out):
-    """Compile command of the CPython module kernel._bind (csrc/py_bind.cpp),
+def _bind_flags():
+    """Compiler flags of the CPython module kernel._bind, and its link line,
     against the headers and libraries of the installed torch."""
     import sysconfig
     import torch
@@ -65,10 +67,10 @@ def _bind_cmd(out):
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     incs = [i for p in (*include_paths(), sysconfig.get_paths()["include"], os.path.join(REPO, "include"))
             for i in ("-I", p)] + ["-I", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]
-    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1",
-            "-DUSE_ROCM=1", *incs,
-            os.path.join(CSRC, "py_bind.cpp"), "-o", out, "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10", "-lamdhip64"]
+    return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1",
+             "-DUSE_ROCM=1", *incs],
+            ["-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10", "-lamdhip64"])
 
 
 def build(verbose=False, jobs=None):
@@ -82,7 +84,9 @@ def build(verbose=False, jobs=None):
         obj = os.path.join(BUILD, src.replace(".hip", ".o"))
         objs.append(obj)
         cmds.append([hipcc, *HIPCC_FLAGS, *SOURCE_FLAGS.get(src, ()), "-c", os.path.join(CSRC, src), "-o", obj])
-    cmds.append(_bind_cmd(BIND + ".tmp"))
+    cxx, libs = _bind_flags()
+    bind_objs = [os.path.join(BUILD, src.replace(".cpp", ".o")) for src in BIND_SOURCES]
+    cmds += [[*cxx, "-c", os.path.join(CSRC, src), "-o", obj] for src, obj in zip(BIND_SOURCES, bind_objs)]
     jobs = jobs or min(len(cmds), max(1, os.cpu_count() or 1))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         for out in ex.map(_run, cmds):
@@ -90,6 +94,7 @@ def build(verbose=False, jobs=None):
                 print(out)
     tmp = OUT + ".tmp"
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs])
+    _run([cxx[0], "-shared", "-o", BIND + ".tmp", *bind_objs, *libs])
     os.replace(tmp, OUT)
     os.replace(BIND + ".tmp", BIND)
     if verbose:

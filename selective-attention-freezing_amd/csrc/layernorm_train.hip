@@ -1,0 +1,284 @@
+// Residual addition and LayerNorm of a training step, forward and backward
+// (gfx950).
+//
+//   r = x + delta (rounded to x's type)      m = mean(r), rstd = 1 / sqrt(var(r) + eps)
+//   xh = (r - m) rstd                        y = xh w + b
+//   g = dy w
+//   dx = dr + rstd (g - mean(g) - xh mean(g xh))
+//   dw = sum over rows of dy xh, db = sum over rows of dy
+//
+// One pass over the rows each way, everything in float32 between the load and
+// the one rounding of each result; the variance is the centred sum of squares
+// (the row stays in registers, so the second sum costs no second read).  Both
+// kernels move bytes and nothing else bounds them.
+//
+// A row belongs to TPR threads (a half wave up to 1024 channels, a wave, four
+// waves, sixteen), each with NCH chunks of 8 channels, chunk k at channel
+// 8 (TPR k + thread): every load and store of the group is one run.
+//
+// Backward: a workgroup walks rows a grid apart and keeps its share of dw and db
+// of its threads' channels in registers; at the end it adds its row groups in LDS
+// and writes one (2, C) float32 partial, and a second kernel adds the partials in
+// a fixed order, so the weight gradients are the same in every run.
+#include "saf_kernels.h"
+#include "saf_rowio.h"
+
+namespace saf {
+
+namespace {
+
+template <int TPR> constexpr int kGroups = TPR >= 256 ? 1 : 256 / TPR;
+template <int TPR> constexpr int kThreads = TPR >= 256 ? TPR : 256;
+
+// Sum over the TPR threads of a row, in a fixed order.  `slot` is LDS of the
+// reduction's own (one per sum of a row) where several waves share a row.
+template <int TPR>
+__device__ inline float row_sum(float v, float* slot) {
+  if constexpr (TPR == 32) {
+    v = dpp_add<0xb1, 0xf>(v);
+    v = dpp_add<0x4e, 0xf>(v);
+    v = dpp_add<0x141, 0xf>(v);
+    v = dpp_add<0x140, 0xf>(v);
+    return v + __shfl_xor(v, 16, 64);
+  } else {
+    v = dpp_wave_sum(v);
+    if constexpr (TPR > 64) {
+      if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = 0.f;
+#pragma unroll
+      for (int i = 0; i < TPR / 64; ++i) v += slot[i];
+    }
+    return v;
+  }
+}
+
+template <typename TX, typename TB, int TPR, int NCH>
+__global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTrainParams p) {
+  __shared__ float slots[2][TPR > 64 ? TPR / 64 : 1];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * kGroups<TPR> + threadIdx.x / TPR;
+  // a whole half wave, wave or workgroup leaves together, and sums stay inside it
+  if (row >= p.rows) return;
+  const int C = p.C;
+  const TX* xr = reinterpret_cast<const TX*>(p.x) + row * p.x_rs;
+  float v[NCH][8];
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) load_row8(xr, 8 * (TPR * k + t), C, v[k]);
+  if (p.delta) {
+    const TB* dr = reinterpret_cast<const TB*>(p.delta) + row * p.d_rs;
+    TX* rr = reinterpret_cast<TX*>(p.r) + row * C;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const int c = 8 * (TPR * k + t);
+      float d[8];
+      load_row8(dr, c, C, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[k][e] = (float)static_cast<TX>(v[k][e] + d[e]);
+      store_row8(rr, c, C, v[k]);
+    }
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < NCH; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[k][e];
+  const float mean = row_sum<TPR>(s, slots[0]) / (float)C;
+  float q = 0.f;
+#pragma unroll
+  for (int k = 0; k < NCH; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = v[k][e] - mean;
+      q = 8 * (TPR * k + t) + e < C ? fmaf(d, d, q) : q;
+    }
+  const float rstd = 1.f / sqrtf(row_sum<TPR>(q, slots[1]) / (float)C + p.eps);
+  if (p.stats && t == 0) {
+    p.stats[2 * row] = mean;
+    p.stats[2 * row + 1] = rstd;
+  }
+  TB* yr = reinterpret_cast<TB*>(p.y) + row * C;
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) {
+    const int c = 8 * (TPR * k + t);
+    if (c >= C) continue;
+    float w[8], b[8] = {};
+    load_vec8(p.w, p.wb_dtype, c, C, w);
+    if (p.b) load_vec8(p.b, p.wb_dtype, c, C, b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = fmaf((v[k][e] - mean) * rstd, w[e], b[e]);
+    store_row8(yr, c, C, w);
+  }
+}
+
+template <typename TX, typename TB, int TPR, int NCH>
+__global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTrainBwdParams p) {
+  __shared__ float slots[2][TPR > 64 ? TPR / 64 : 1];
+  __shared__ float2 part[TPR >= 256 ? 1 : 8 * TPR * NCH];
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int C = p.C;
+  float w[NCH][8], aw[NCH][8], ab[NCH][8];
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) {
+    const int c = 8 * (TPR * k + t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[k][e] = aw[k][e] = ab[k][e] = 0.f;
+    if (c < C) load_vec8(p.w, p.w_dtype, c, C, w[k]);
+  }
+  for (int64_t row = (int64_t)blockIdx.x * kGroups<TPR> + group; row < p.rows;
+       row += (int64_t)gridDim.x * kGroups<TPR>) {
+    const TX* rr = reinterpret_cast<const TX*>(p.r) + row * p.r_rs;
+    const TB* gr = reinterpret_cast<const TB*>(p.dy) + row * p.dy_rs;
+    const float mean = p.stats[2 * row], rstd = p.stats[2 * row + 1];
+    float xh[NCH][8], g[NCH][8], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) load_row8(rr, 8 * (TPR * k + t), C, xh[k], mean);
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) load_row8(gr, 8 * (TPR * k + t), C, g[k]);
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        xh[k][e] = (xh[k][e] - mean) * rstd;
+        aw[k][e] = fmaf(g[k][e], xh[k][e], aw[k][e]);
+        ab[k][e] += g[k][e];
+        g[k][e] *= w[k][e];
+        s1 += g[k][e];
+        s2 = fmaf(g[k][e], xh[k][e], s2);
+      }
+    // a wave writes a slot again only behind the other sum's barrier, which
+    // every wave reaches after it has read this one
+    const float c1 = row_sum<TPR>(s1, slots[0]) / (float)C;
+    const float c2 = row_sum<TPR>(s2, slots[1]) / (float)C;
+    TX* dxr = reinterpret_cast<TX*>(p.dx) + row * C;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const int c = 8 * (TPR * k + t);
+      if (c >= C) continue;
+      float d[8] = {};
+      if (p.dr) load_row8(reinterpret_cast<const TX*>(p.dr) + row * p.dr_rs, c, C, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = fmaf(rstd, g[k][e] - c1 - xh[k][e] * c2, d[e]);
+      if (p.dx) store_row8(dxr, c, C, d);
+      if (p.ddelta) store_row8(reinterpret_cast<TB*>(p.ddelta) + row * C, c, C, d);
+    }
+  }
+  if (!p.part) return;
+  float* out = p.part + (int64_t)blockIdx.x * 2 * C;
+  if constexpr (kGroups<TPR> > 1) {
+    for (int i = 0; i < kGroups<TPR>; ++i) {
+      if (group == i)
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float2& a = part[(8 * k + e) * TPR + t];
+            a = i == 0 ? make_float2(aw[k][e], ab[k][e]) : make_float2(a.x + aw[k][e], a.y + ab[k][e]);
+          }
+      __syncthreads();
+    }
+    if (group != 0) return;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 a = part[(8 * k + e) * TPR + t];
+        aw[k][e] = a.x;
+        ab[k][e] = a.y;
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) {
+    store_row8(out, 8 * (TPR * k + t), C, aw[k]);
+    store_row8(out + C, 8 * (TPR * k + t), C, ab[k]);
+  }
+}
+
+// dw (blockIdx.y 0) and db (1): partials added by 32 lanes a channel, each its
+// own residue class in order, then the lanes in order.
+__global__ __launch_bounds__(1024) void layernorm_dw_kernel(const LnTrainBwdParams p, int n_part) {
+  __shared__ float sums[32][33];
+  void* out = blockIdx.y == 0 ? p.dw : p.db;
+  if (out == nullptr) return;
+  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, c = blockIdx.x * 32 + col, C = p.C;
+  float a = 0.f;
+  if (c < C) {
+    const float* src = p.part + blockIdx.y * C + c;
+#pragma unroll 4
+    for (int i = lane; i < n_part; i += 32) a += src[(int64_t)i * 2 * C];
+  }
+  sums[lane][col] = a;
+  __syncthreads();
+  if (lane != 0 || c >= C) return;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s += sums[i][col];
+  store_elem(out, p.w_dtype, c, s);
+}
+
+// C up to 1024: a half wave a row; 2048: a wave; 8192: four waves; 16384: sixteen.
+template <template <typename, typename, int, int> class F, typename TX, typename TB, typename... A>
+hipError_t by_width(int C, A... a) {
+  const int n = (C + 7) / 8;
+  if (n <= 32) return F<TX, TB, 32, 1>::run(a...);
+  if (n <= 64) return F<TX, TB, 32, 2>::run(a...);
+  if (n <= 96) return F<TX, TB, 32, 3>::run(a...);
+  if (n <= 128) return F<TX, TB, 32, 4>::run(a...);
+  if (n <= 192) return F<TX, TB, 64, 3>::run(a...);
+  if (n <= 256) return F<TX, TB, 64, 4>::run(a...);
+  if (n <= 512) return F<TX, TB, 256, 2>::run(a...);
+  if (n <= 768) return F<TX, TB, 256, 3>::run(a...);
+  if (n <= 1024) return F<TX, TB, 256, 4>::run(a...);
+  if (n <= 2048) return F<TX, TB, 1024, 2>::run(a...);
+  return hipErrorInvalidValue;
+}
+
+template <typename TX, typename TB, int TPR, int NCH> struct Fwd {
+  static hipError_t run(const LnTrainParams& p, hipStream_t s) {
+    constexpr int G = kGroups<TPR>;
+    hipLaunchKernelGGL((layernorm_fwd_kernel<TX, TB, TPR, NCH>), dim3((unsigned)((p.rows + G - 1) / G)), dim3(kThreads<TPR>),
+                       0, s, p);
+    return hipGetLastError();
+  }
+};
+template <typename TX, typename TB, int TPR, int NCH> struct Bwd {
+  static hipError_t run(const LnTrainBwdParams& p, hipStream_t s) {
+    if (p.n_wg > 0)
+      hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TB, TPR, NCH>), dim3((unsigned)p.n_wg), dim3(kThreads<TPR>), 0, s, p);
+    if (p.dw || p.db)
+      hipLaunchKernelGGL(layernorm_dw_kernel, dim3((unsigned)((p.C + 31) / 32), 2), dim3(1024), 0, s, p, p.n_wg);
+    return hipGetLastError();
+  }
+};
+
+template <template <typename, typename, int, int> class F, typename P>
+hipError_t by_types(const P& p, int dtype, int branch, hipStream_t s) {
+  if (dtype == kF32) {
+    if (branch == kF32) return by_width<F, float, float, const P&, hipStream_t>(p.C, p, s);
+    if (branch == kBF16) return by_width<F, float, __bf16, const P&, hipStream_t>(p.C, p, s);
+    return by_width<F, float, _Float16, const P&, hipStream_t>(p.C, p, s);
+  }
+  if (dtype == kBF16) return by_width<F, __bf16, __bf16, const P&, hipStream_t>(p.C, p, s);
+  return by_width<F, _Float16, _Float16, const P&, hipStream_t>(p.C, p, s);
+}
+
+}  // namespace
+
+// Workgroups of the backward pass: as many as are resident, each with at least
+// one round of rows.
+int layernorm_bwd_groups(int64_t rows, int C, int n_cu) {
+  const int n = (C + 7) / 8;
+  const int per = n <= 128 ? 8 : (n <= 256 ? 4 : 1);
+  const int64_t rounds = (rows + per - 1) / per;
+  const int64_t most = (int64_t)n_cu * (n <= 1024 ? 2 : 1);
+  return (int)(rounds < most ? rounds : most);
+}
+
+hipError_t launch_layernorm_train(const LnTrainParams& p, int dtype, int branch, hipStream_t s) {
+  return by_types<Fwd>(p, dtype, branch, s);
+}
+hipError_t launch_layernorm_train_bwd(const LnTrainBwdParams& p, int dtype, int branch, hipStream_t s) {
+  return by_types<Bwd>(p, dtype, branch, s);
+}
+
+}  // namespace saf

@@ -1,4 +1,4 @@
-// CPython module kernel._bind: the host path of the decoding operators where
+// CPython module kernel._bind: the host path of the decoding and training operators where
 // ctypes and Python cost more than the kernels.
 //
 // fill(what, block, offsets, rows, device, refuse_grad, t0, t1, ...) writes the
@@ -19,25 +19,15 @@
 // the interpreter: forward and backward of a small call took 90-110 us as a
 // Python autograd.Function.
 //
+// embed_tokens, add_layernorm, gelu_packed and their like are in
+// py_bind_train.cpp.
+//
 // library(addresses) hands over the entry points of libsafattn.so.
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/variable.h>
+#include "py_bind.h"
 
-#include <ATen/core/Tensor.h>
-#include <ATen/core/grad_mode.h>
-#include <ATen/ops/empty.h>
-#include <ATen/ops/zeros.h>
-#include <c10/core/AutogradState.h>
-#include <c10/hip/HIPGraphsC10Utils.h>
-#include <c10/hip/HIPGuard.h>
-#include <c10/hip/HIPStream.h>
+using namespace saf_bind;
 
-#include "saf_attn.h"
-
-namespace {
+namespace saf_bind {
 
 int dtype_code(at::ScalarType t) {
   switch (t) {
@@ -50,6 +40,78 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
+static decltype(&saf_last_error) last_error = nullptr;
+
+bool has_tangent(const at::Tensor& x) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(0).defined();
+}
+
+void check(int rc) {
+  if (rc == SAF_OK) return;
+  TORCH_CHECK_NOT_IMPLEMENTED(rc != SAF_EUNSUPPORTED, last_error());
+  TORCH_CHECK_VALUE(rc != SAF_EINVAL && rc != SAF_EALIGN && rc != SAF_EWORKSPACE, last_error());
+  TORCH_CHECK(false, last_error());
+}
+
+saf_tensor_t desc(const char* what, const at::Tensor& x) {
+  saf_tensor_t d{};
+  if (!x.defined()) return d;
+  const int code = dtype_code(x.scalar_type());
+  TORCH_CHECK_NOT_IMPLEMENTED(code >= 0, what, ": unsupported dtype ", x.scalar_type());
+  d.data = x.data_ptr();
+  d.dtype = code;
+  d.ndim = (int32_t)x.dim();
+  for (int k = 0; k < d.ndim; ++k) {
+    d.size[k] = x.size(k);
+    d.stride[k] = x.stride(k);
+  }
+  return d;
+}
+
+at::Tensor only_once(const char* what, at::Tensor dx) {
+  if (!dx.defined() || !at::GradMode::is_enabled()) return dx;
+  auto once = std::make_shared<torch::autograd::DelayedError>(std::string(what) + ": twice differentiating is not supported", 1);
+  return (*once)({dx.detach().set_requires_grad(true)})[0];
+}
+
+void refuse_foreign_capture(const char* what, const char* name, const at::Tensor& x) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  std::vector<std::shared_ptr<torch::autograd::Node>> leaves;
+  if (auto fn = x.grad_fn()) {
+    for (;;) {
+      std::shared_ptr<torch::autograd::Node> only;
+      int n = 0;
+      for (const auto& e : fn->next_edges())
+        if (e.function) {
+          only = e.function;
+          ++n;
+        }
+      if (n != 1 || only->num_outputs() == 0) break;  // the leaf's own node has no next edges
+      fn = std::move(only);
+    }
+    for (const auto& e : fn->next_edges())
+      if (e.function && e.function->name() == "torch::autograd::AccumulateGrad") leaves.push_back(e.function);
+  } else if (auto node = torch::autograd::impl::try_get_grad_accumulator(x)) {
+    leaves.push_back(std::move(node));
+  }
+  const c10::Stream now = c10::hip::getCurrentHIPStream().unwrap();
+  for (const auto& node : leaves) {
+    const auto made = node->stream();
+    TORCH_CHECK(!made || made->id() == now.id(),
+                what, ": an eager autograd graph of these ", name, ", made on another stream, is still alive; release "
+                "it before capturing their gradient");
+  }
+}
+
+PyObject* wrap(const at::Tensor& t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(t);
+}
+
+}  // namespace saf_bind
+
+namespace {
+
 bool rows_ok(const at::Tensor& x) {
   if (x.dim() != 4) return true;  // the library names the mistake
   const int64_t es = x.element_size();
@@ -57,12 +119,6 @@ bool rows_ok(const at::Tensor& x) {
   for (int i = 0; i < 3; ++i)
     if (x.size(i) > 1 && x.stride(i) * es % 16) return false;
   return true;
-}
-
-// A dual tensor: none of the operators has a forward-mode derivative, and
-// their results would drop the tangent without a word.
-bool has_tangent(const at::Tensor& x) {
-  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(0).defined();
 }
 
 PyObject* fill(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -121,30 +177,9 @@ struct {
   decltype(&saf_token_logprobs) forward;
   decltype(&saf_token_logprobs_workspace_bytes) workspace_bytes;
   decltype(&saf_token_logprobs_bwd) backward;
-  decltype(&saf_last_error) last_error;
 } lib{};
 
-void check(int rc) {
-  if (rc == SAF_OK) return;
-  TORCH_CHECK_NOT_IMPLEMENTED(rc != SAF_EUNSUPPORTED, lib.last_error());
-  TORCH_CHECK_VALUE(rc != SAF_EINVAL && rc != SAF_EALIGN && rc != SAF_EWORKSPACE, lib.last_error());
-  TORCH_CHECK(false, lib.last_error());
-}
-
-saf_tensor_t desc(const at::Tensor& x) {
-  saf_tensor_t d{};
-  if (!x.defined()) return d;
-  const int code = dtype_code(x.scalar_type());
-  TORCH_CHECK_NOT_IMPLEMENTED(code >= 0, "token_logprobs: unsupported dtype ", x.scalar_type());
-  d.data = x.data_ptr();
-  d.dtype = code;
-  d.ndim = (int32_t)x.dim();
-  for (int k = 0; k < d.ndim; ++k) {
-    d.size[k] = x.size(k);
-    d.stride[k] = x.stride(k);
-  }
-  return d;
-}
+constexpr const char* kWhat = "token_logprobs";
 
 struct Options {
   int64_t top, ignore;
@@ -157,8 +192,8 @@ struct Outputs {
 
 saf_token_logprobs_args arguments(const at::Tensor& logits, const at::Tensor& tokens, int64_t ignore, double scale) {
   saf_token_logprobs_args a{};
-  a.logits = desc(logits);
-  a.tokens = desc(tokens);
+  a.logits = desc(kWhat, logits);
+  a.tokens = desc(kWhat, tokens);
   a.ignore_index = ignore;
   a.scale = (float)scale;
   return a;
@@ -178,11 +213,11 @@ Outputs run_forward(const at::Tensor& logits, const at::Tensor& tokens, const Op
   }
   saf_token_logprobs_args a = arguments(logits, tokens, o.ignore, o.scale);
   a.top = (int32_t)o.top;
-  a.logp = desc(r.logp);
-  a.entropy = desc(r.entropy);
-  a.stats = desc(r.stats);
-  a.top_index = desc(r.index);
-  a.top_logp = desc(r.top_logp);
+  a.logp = desc(kWhat, r.logp);
+  a.entropy = desc(kWhat, r.entropy);
+  a.stats = desc(kWhat, r.stats);
+  a.top_index = desc(kWhat, r.index);
+  a.top_logp = desc(kWhat, r.top_logp);
   at::Tensor ws;
   const int64_t bytes = lib.workspace_bytes(&a);
   if (bytes > 0) {
@@ -229,57 +264,15 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
       dx = at::empty({logits.size(0), logits.size(1)}, logits.options().requires_grad(false));
       saf_token_logprobs_args a =
           arguments(logits, tokens, ctx->saved_data["ignore"].toInt(), ctx->saved_data["scale"].toDouble());
-      a.stats = desc(stats);
-      a.entropy = desc(entropy);
-      const saf_tensor_t dg = desc(g), dge = desc(ge), ddx = desc(dx);
+      a.stats = desc(kWhat, stats);
+      a.entropy = desc(kWhat, entropy);
+      const saf_tensor_t dg = desc(kWhat, g), dge = desc(kWhat, ge), ddx = desc(kWhat, dx);
       check(lib.backward(&a, &dg, &dge, &ddx, c10::hip::getCurrentHIPStream().stream()));
     }
-    if (at::GradMode::is_enabled()) {  // the gradient has no derivative of its own
-      auto once = std::make_shared<torch::autograd::DelayedError>("token_logprobs: twice differentiating is not supported", 1);
-      dx = (*once)({dx.detach().set_requires_grad(true)})[0];
-    }
+    dx = only_once("token_logprobs", dx);
     return {dx, at::Tensor(), at::Tensor()};
   }
 };
-
-// A leaf's autograd node belongs to the stream of the call that made it.  A
-// captured backward would make that stream wait for the capturing one, and with
-// it join the capture without ever leaving it: torch ends the process there.
-// So logits that are such a leaf, or come from one by operations of a single
-// input (views, slices, casts), are refused.
-void refuse_foreign_capture(const at::Tensor& logits) {
-  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  std::vector<std::shared_ptr<torch::autograd::Node>> leaves;
-  if (auto fn = logits.grad_fn()) {
-    for (;;) {
-      std::shared_ptr<torch::autograd::Node> only;
-      int n = 0;
-      for (const auto& e : fn->next_edges())
-        if (e.function) {
-          only = e.function;
-          ++n;
-        }
-      if (n != 1 || only->num_outputs() == 0) break;  // the leaf's own node has no next edges
-      fn = std::move(only);
-    }
-    for (const auto& e : fn->next_edges())
-      if (e.function && e.function->name() == "torch::autograd::AccumulateGrad") leaves.push_back(e.function);
-  } else if (auto node = torch::autograd::impl::try_get_grad_accumulator(logits)) {
-    leaves.push_back(std::move(node));
-  }
-  const c10::Stream now = c10::hip::getCurrentHIPStream().unwrap();
-  for (const auto& node : leaves) {
-    const auto made = node->stream();
-    TORCH_CHECK(!made || made->id() == now.id(),
-                "token_logprobs: an eager autograd graph of these logits, made on another stream, is still alive; release "
-                "it before capturing their gradient");
-  }
-}
-
-PyObject* wrap(const at::Tensor& t) {
-  if (!t.defined()) Py_RETURN_NONE;
-  return THPVariable_Wrap(t);
-}
 
 PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -297,7 +290,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   TORCH_CHECK_NOT_IMPLEMENTED(o.top >= 0 && o.top <= 32, "top = ", o.top, " outside 0..32 or above the vocabulary");
   Outputs r;
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
-    refuse_foreign_capture(logits);
+    refuse_foreign_capture("token_logprobs", "logits", logits);
     const auto out = TokenLogprobs::apply(logits, tokens, o);
     size_t k = 0;
     r.logp = out[k++];
@@ -328,7 +321,7 @@ PyObject* library(PyObject*, PyObject* const* args, Py_ssize_t n) {
   lib.forward = reinterpret_cast<decltype(lib.forward)>(p[0]);
   lib.workspace_bytes = reinterpret_cast<decltype(lib.workspace_bytes)>(p[1]);
   lib.backward = reinterpret_cast<decltype(lib.backward)>(p[2]);
-  lib.last_error = reinterpret_cast<decltype(lib.last_error)>(p[3]);
+  last_error = reinterpret_cast<decltype(last_error)>(p[3]);
   Py_RETURN_NONE;
 }
 
@@ -340,9 +333,18 @@ PyMethodDef methods[] = {
      "fill(what, block, offsets, rows, device, refuse_grad, *tensors) -> mask of tensors whose rows need a copy"},
     {"token_logprobs", method(token_logprobs), METH_FASTCALL,
      "token_logprobs(logits, tokens, top, entropy, scale, ignore_index) -> (logp, entropy, top_index, top_logp)"},
+    {"embed_tokens", method(embed_tokens), METH_FASTCALL, "embed_tokens(tokens, weight, scale, ignore_index, dtype) -> rows"},
+    {"add_layernorm", method(add_layernorm), METH_FASTCALL,
+     "add_layernorm(x, delta, weight, bias, eps, dtype) -> (r or None, y)"},
+    {"gelu_packed", method(gelu_packed), METH_FASTCALL, "gelu_packed(x, keep) -> y, or (y, q, exp) with keep"},
+    {"gelu_packed_bwd", method(gelu_packed_bwd), METH_FASTCALL, "gelu_packed_bwd(q, exp, dy, again) -> (dx, y or None)"},
+    {"pack_activation", method(pack_activation), METH_FASTCALL, "pack_activation(x) -> (q, exp)"},
+    {"unpack_activation", method(unpack_activation), METH_FASTCALL, "unpack_activation(q, exp, dtype) -> x"},
+    {"check_differentiable", method(check_differentiable), METH_FASTCALL, "check_differentiable(what, *tensors)"},
+    {"library_train", method(library_train), METH_FASTCALL, "library_train(addresses of the training operators)"},
     {"library", method(library), METH_FASTCALL, "library(forward, workspace_bytes, backward, last_error)"},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", "Host path of the decoding operators.", -1, methods};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", "Host path of the decoding and training operators.", -1, methods};
 
 }  // namespace
 

@@ -38,7 +38,10 @@ int fail(int code, const char* fmt, ...) {
 
 bool present(const saf_tensor_t& t) { return t.data != nullptr; }
 
-int elem_size(int dtype) { return dtype == SAF_I64 ? 8 : (dtype == SAF_F32 || dtype == SAF_I32 ? 4 : 2); }
+int elem_size(int dtype) {
+  if (dtype == SAF_I8 || dtype == SAF_U8) return 1;
+  return dtype == SAF_I64 ? 8 : (dtype == SAF_F32 || dtype == SAF_I32 ? 4 : 2);
+}
 
 const char* dtype_name(int d) {
   switch (d) {
@@ -47,6 +50,8 @@ const char* dtype_name(int d) {
     case SAF_BF16: return "bfloat16";
     case SAF_I32: return "int32";
     case SAF_I64: return "int64";
+    case SAF_I8: return "int8";
+    case SAF_U8: return "uint8";
     default: return "unknown";
   }
 }

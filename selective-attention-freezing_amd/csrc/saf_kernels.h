@@ -3,6 +3,7 @@
 // lives in include/saf_attn.h.
 #pragma once
 #include "saf_device.h"
+#include "saf_rowio.h"
 
 namespace saf {
 
@@ -336,6 +337,91 @@ struct LogprobBwdParams {
   int64_t g_st, ge_st;
 };
 
+// Residual addition and LayerNorm of a training step (layernorm_train.hip); r, y,
+// dx and ddelta are contiguous.
+struct LnTrainParams {
+  const void* x;
+  const void* delta;  // null: r is x, not written
+  void* r;
+  void* y;
+  const void* w;
+  const void* b;      // null: none
+  float* stats;       // (rows, 2) mean and 1 / deviation; null: not kept
+  int64_t rows, x_rs, d_rs;
+  int C, wb_dtype;
+  float eps;
+};
+struct LnTrainBwdParams {
+  const void* r;
+  const void* dy;
+  const void* dr;     // null: none
+  const void* w;
+  const float* stats;
+  void* dx;           // null: not wanted
+  void* ddelta;       // dx in the branch's type; null: not wanted
+  void* dw;           // null: not wanted
+  void* db;           // null: not wanted
+  float* part;        // (n_wg, 2, C); null: neither dw nor db
+  int64_t rows, r_rs, dy_rs, dr_rs;
+  int C, w_dtype, n_wg;
+};
+constexpr int kLnMaxC = 16384;
+int layernorm_bwd_groups(int64_t rows, int C, int n_cu);
+
+// Activations in 8 bits (act_pack.hip).  q and exp are contiguous; a unit is 8
+// channels, per_row.d of them a row (a multiple of 4).
+struct ActPackParams {
+  const void* x;   // the activation; dy in the backward pass
+  int64_t x_rs;
+  int8_t* q;
+  uint8_t* exp;
+  void* y;         // gelu(x) (contiguous); the unpacked activation; null in the backward pass: not wanted
+  int64_t y_rs;
+  void* dx;
+  int C;
+  FastDiv per_row;
+  uint32_t units;
+};
+enum class ActPackOp { kPack, kUnpack, kGelu, kGeluBwd };
+
+// Embedding lookup and gradient (embed.hip); a unit is 8 channels of a token, of
+// a chunk of sorted positions in the backward pass.
+constexpr int kEmbedTile = 8192;  // tokens that one workgroup sorts
+constexpr int kEmbedDigit = 9;    // bits of a sorting pass at most
+struct EmbedParams {
+  const void* tokens;
+  int tok_i64;
+  int64_t tok_st;
+  int64_t ignore, V;
+  const void* w;
+  int64_t w_rs;
+  void* y;
+  float scale;
+  int C;
+  FastDiv per_row;
+  uint32_t units;
+};
+struct EmbedBwdParams {
+  const void* tokens;
+  int tok_i64;
+  int64_t tok_st;
+  int64_t ignore, V, N;
+  const void* dy;
+  int64_t dy_rs;
+  void* dw;
+  int64_t dw_bytes;
+  float scale;
+  int C;
+  uint2* sorted;    // (N) token, position
+  uint2* sorted2;   // (N) with more than one tile and pass
+  uint32_t* counts; // (n_tiles, 2^kEmbedDigit) with more than one tile
+  float* head;      // (chunks, C) sums of a chunk's first word where that began before it
+  float* tail;      // (chunks, C) sums of its last word where that goes on
+  int n_tiles, n_clear, passes, bits, chunk;
+  FastDiv per_row;
+  uint32_t units;
+};
+
 // Rows of one scan chunk for a head dimension (must match ScanShape in the
 // kernel): 8 rows per thread, 32 KB of V per chunk for hd 64 / 128.
 inline int scan_chunk_rows(int hd) { return hd == 32 ? 512 : (hd == 64 ? 256 : 128); }
@@ -355,6 +441,11 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int hd, hipStr
 hipError_t launch_paged_append(const PagedAppendParams& p, int dtype, hipStream_t s);
 hipError_t launch_token_logprobs(const LogprobParams& p, int dtype, hipStream_t s);
 hipError_t launch_token_logprobs_bwd(const LogprobBwdParams& p, int dtype, hipStream_t s);
+hipError_t launch_layernorm_train(const LnTrainParams& p, int dtype, int branch, hipStream_t s);
+hipError_t launch_layernorm_train_bwd(const LnTrainBwdParams& p, int dtype, int branch, hipStream_t s);
+hipError_t launch_act_pack(const ActPackParams& p, int dtype, ActPackOp op, hipStream_t s);
+hipError_t launch_embed(const EmbedParams& p, int w_dtype, int y_dtype, hipStream_t s);
+hipError_t launch_embed_bwd(const EmbedBwdParams& p, int w_dtype, int y_dtype, hipStream_t s);
 bool proj_gemm_shape_ok(int64_t M, int64_t N, int64_t K);
 // exact GELU in place over n elements (n % 8 == 0, 16-byte aligned)
 hipError_t launch_gelu_inplace(void* x, int64_t n, int dtype, int n_cu, hipStream_t s);

@@ -15,7 +15,7 @@ LIB_NAME = "libsafattn.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 
 SAF_OK, SAF_EINVAL, SAF_EUNSUPPORTED, SAF_EALIGN, SAF_ELAUNCH, SAF_EWORKSPACE = 0, -1, -2, -3, -4, -5
-SAF_F32, SAF_F16, SAF_BF16, SAF_I32, SAF_I64 = 0, 1, 2, 3, 4
+SAF_F32, SAF_F16, SAF_BF16, SAF_I32, SAF_I64, SAF_I8, SAF_U8 = 0, 1, 2, 3, 4, 5, 6
 SAF_MAX_HEADS = 128
 
 _DTYPE_CODE = {torch.float32: SAF_F32, torch.float16: SAF_F16,
@@ -31,6 +31,8 @@ EXPORTS = ("saf_mixed_attn_fwd", "saf_mixed_attn_side_kernels", "saf_mixed_attn_
            "saf_decomposed_logz_bwd", "saf_workspace_bytes", "saf_mixed_attn_workspace_bytes", "saf_workspace_error",
            "saf_paged_append", "saf_paged_attn_fwd", "saf_paged_attn_workspace_bytes", "saf_token_logprobs",
            "saf_token_logprobs_workspace_bytes", "saf_token_logprobs_bwd",
+           "saf_embed_fwd", "saf_embed_bwd", "saf_embed_bwd_workspace_bytes", "saf_layernorm_fwd", "saf_layernorm_bwd",
+           "saf_layernorm_bwd_workspace_bytes", "saf_act_pack", "saf_act_unpack", "saf_gelu_pack_fwd", "saf_gelu_pack_bwd",
            "saf_time_next_kernel", "saf_last_error", "saf_version")
 
 
@@ -166,6 +168,19 @@ def lib():
             fn.restype = ctypes.c_int64
         L.saf_token_logprobs_bwd.argtypes = [P(SafTokenLogprobsArgs)] + [P(SafTensor)] * 3 + [ctypes.c_void_p]
         L.saf_token_logprobs_bwd.restype = ctypes.c_int
+        T, vp, i64 = P(SafTensor), ctypes.c_void_p, ctypes.c_int64
+        for name, rest in (("saf_embed_fwd", [T, T, ctypes.c_float, i64, T, vp]),
+                           ("saf_embed_bwd", [T, T, ctypes.c_float, i64, T, vp, i64, vp]),
+                           ("saf_layernorm_fwd", [T] * 4 + [ctypes.c_float] + [T] * 3 + [vp]),
+                           ("saf_layernorm_bwd", [T] * 9 + [vp, i64, vp]),
+                           ("saf_act_pack", [T] * 3 + [vp]), ("saf_act_unpack", [T] * 3 + [vp]),
+                           ("saf_gelu_pack_fwd", [T] * 4 + [vp]), ("saf_gelu_pack_bwd", [T] * 5 + [vp])):
+            fn = getattr(L, name)
+            fn.argtypes, fn.restype = rest, ctypes.c_int
+        L.saf_embed_bwd_workspace_bytes.argtypes = [i64] * 3
+        L.saf_embed_bwd_workspace_bytes.restype = i64
+        L.saf_layernorm_bwd_workspace_bytes.argtypes = [i64] * 2
+        L.saf_layernorm_bwd_workspace_bytes.restype = i64
         L.saf_time_next_kernel.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         L.saf_time_next_kernel.restype = ctypes.c_int
         L.saf_last_error.argtypes = []
@@ -234,6 +249,10 @@ def bind():
         module.library(*[ctypes.cast(getattr(L, n), ctypes.c_void_p).value
                          for n in ("saf_token_logprobs", "saf_token_logprobs_workspace_bytes", "saf_token_logprobs_bwd",
                                    "saf_last_error")])
+        module.library_train(*[ctypes.cast(getattr(L, n), ctypes.c_void_p).value
+                               for n in ("saf_embed_fwd", "saf_embed_bwd", "saf_embed_bwd_workspace_bytes",
+                                         "saf_layernorm_fwd", "saf_layernorm_bwd", "saf_layernorm_bwd_workspace_bytes",
+                                         "saf_act_pack", "saf_act_unpack", "saf_gelu_pack_fwd", "saf_gelu_pack_bwd")])
         _bind = module
     return _bind
 
@@ -293,6 +312,16 @@ def set_tables(args, n_heads, *tables):
 
 def set_workspace(args, ptr, nbytes):
     _WORKSPACE.pack_into(args, SafMixedAttnArgs.workspace.offset, ptr, nbytes)
+
+
+def dtype_code(what, dtype):
+    """Code of a floating dtype, -1 for None."""
+    if dtype is None:
+        return -1
+    code = _DTYPE_CODE.get(dtype, -1)
+    if not 0 <= code <= SAF_BF16:
+        raise NotImplementedError(f"{what}: unsupported dtype {dtype}")
+    return code
 
 
 def check(rc):

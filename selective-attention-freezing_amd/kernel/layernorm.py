@@ -8,6 +8,10 @@ sub-layer.  ``add_layernorm_`` does both in one pass over the residual
 to the activation dtype, then the LayerNorm of the rounded x in fp32, one
 rounding of the output.  Forward only.
 
+``add_layernorm`` is the differentiable form, out of place (``saf_layernorm_fwd``,
+``saf_layernorm_bwd``): the residual stream may be float32 beside 16-bit branches,
+and the weight gradients are sums in a fixed order.
+
 ``add_rmsnorm_`` is the same pass with transformers' Qwen3RMSNorm in place of
 the LayerNorm (the Qwen caller's decoder-block norms, ``saf_add_rmsnorm``).
 """
@@ -52,3 +56,18 @@ def add_rmsnorm_(x, delta, weight, eps=1e-6):
     if rc:
         _ext.check(rc)
     return out
+
+
+def add_layernorm(x, delta, weight, bias=None, eps=1e-5, dtype=None):
+    """(r, LayerNorm(r) * weight + bias) for the residual r = x + delta, both new
+    tensors (delta None: r is x itself).
+
+      x       (..., C), C up to 16384, float32, bfloat16 or float16; r has its dtype
+      delta   (..., C), x's shape, in the dtype of the normalised result
+      weight, bias  (C,), of one dtype of the three
+      dtype   of the normalised result; default delta's, without delta x's.  x's own,
+              or bfloat16 / float16 beside a float32 x
+    The norm is that of the rounded r; fp32 arithmetic, one rounding of each result.
+    Differentiable in x, delta, weight and bias (reverse mode, once)."""
+    r, y = _ext.bind().add_layernorm(x, delta, weight, bias, float(eps), _ext.dtype_code("add_layernorm", dtype))
+    return (x if r is None else r), y

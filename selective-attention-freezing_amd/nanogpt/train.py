@@ -1,0 +1,53 @@
+"""A training pass of the GPT of ``nanogpt.model`` on the framework's own operators
+around its products and attention.
+
+    logp = token_logprobs(model, idx, targets).logp      # (B, T)
+    (-logp.mean()).backward()
+
+computes what ``GPT.token_logprobs`` does, with ``kernel.embed_tokens`` for the
+embedding, each residual addition fused with the LayerNorm behind it
+(``kernel.add_layernorm``), and the MLPs' activations kept in 8 bits for the
+backward pass (``kernel.mlp_packed``; ``packed=False`` keeps them whole).  Under
+autocast the residual stream has the weights' float32 and the branches the
+autocast dtype.
+"""
+import torch
+
+import kernel as _kernel_mod
+from nanogpt.model import MLP
+
+
+def forward_hidden(model, idx, packed=True):
+    """Hidden states (B, T, C) of every position behind the last norm,
+    differentiable in every parameter of the model that the tokens reach."""
+    T = idx.size(1)
+    if T > model.config.block_size:
+        raise ValueError(f"sequences of {T} tokens exceed the model's block size {model.config.block_size}")
+    tr = model.transformer
+    x = _kernel_mod.embed_tokens(idx, tr.wte.weight)
+    dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+    rope = None
+    if model.rotary is None:
+        x = x + tr.wpe(torch.arange(T, device=idx.device))
+    else:
+        rope = model.rotary(T, dtype)
+    ln = tr.h[0].ln_1
+    h = _kernel_mod.add_layernorm(x, None, ln.weight, ln.bias, dtype=dtype)[1]
+    for i, block in enumerate(tr.h):
+        x, h = _kernel_mod.add_layernorm(x, block.attn(h, rope=rope), block.ln_2.weight, block.ln_2.bias)
+        ln = tr.h[i + 1].ln_1 if i + 1 < len(tr.h) else tr.ln_f
+        x, h = _kernel_mod.add_layernorm(x, _mlp(block.mlp, h, packed), ln.weight, ln.bias)
+    return h
+
+
+def _mlp(mlp, h, packed):
+    # a module of the caller's own, or another activation, runs as it is
+    if not packed or type(mlp) is not MLP or mlp.gelu.approximate != "none":
+        return mlp(h)
+    return _kernel_mod.mlp_packed(h, mlp.c_fc.weight, mlp.c_proj.weight, mlp.c_fc.bias, mlp.c_proj.bias)
+
+
+def token_logprobs(model, idx, tokens, packed=True, **kw):
+    """Log probabilities of tokens (B, T) as the next tokens of idx (B, T), with
+    kernel.token_logprobs' options; -logp.mean() is the training loss."""
+    return _kernel_mod.token_logprobs(model.lm_head(forward_hidden(model, idx, packed)), tokens, **kw)
