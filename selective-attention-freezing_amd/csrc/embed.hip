@@ -11,12 +11,12 @@
 // 1. The positions n are sorted by token, stable, least significant digit first
 //    (9 bits at most a pass), while the other workgroups of the same launches
 //    clear dW: the sort takes no time of its own as long as it is the shorter.
-//    Up to kTile tokens one workgroup sorts in LDS in one launch; more go tile by
-//    tile, each pass a launch that counts the digits of every tile and one that
+//    Up to kEmbedOnce tokens one workgroup sorts in LDS in one launch; more go tile
+//    by tile, each pass a launch that counts the digits of every tile and one that
 //    places every tile's keys.
-// 2. The sorted positions are cut into chunks; a thread sums 8 channels over
-//    a chunk and writes the rows whose tokens lie inside it.  A token that crosses
-//    chunks leaves float32 partial sums,
+// 2. The sorted positions are cut into chunks; a wave sums 256 channels over a chunk
+//    and writes the rows whose tokens lie inside it.  A token that crosses chunks
+//    leaves float32 partial sums,
 // 3. which the third launch adds in order.
 // Every sum is in the order of n whatever runs beside it: no atomic touches a
 // gradient, and each run gives the same bits.
@@ -29,39 +29,69 @@ namespace {
 
 constexpr int kSortThreads = 1024;
 constexpr int kWaves = kSortThreads / 64;
-constexpr int kKeys = kEmbedTile / kSortThreads;  // keys of a thread
 constexpr int kBins = 1 << kEmbedDigit;
+constexpr uint32_t kWideUnits = 1 << 19;  // units from which a thread of the lookup has four
 
-__device__ inline int64_t token_at(const void* tokens, int i64, int64_t st, int64_t n) {
-  return i64 ? reinterpret_cast<const int64_t*>(tokens)[n * st] : (int64_t)reinterpret_cast<const int32_t*>(tokens)[n * st];
-}
-
-template <typename TW, typename TY>
+// U units a thread, 256 apart; their tokens are read together, then their rows.
+template <typename TW, typename TY, int U, bool WHOLE>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const EmbedParams p) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= p.units) return;
-  const uint32_t n = p.per_row.div(i);
-  const int c = 8 * (int)(i - n * p.per_row.d), C = p.C;
-  const int64_t tok = token_at(p.tokens, p.tok_i64, p.tok_st, n);
-  float f[8];
-  if (tok >= 0 && tok < p.V && tok != p.ignore) {
-    load_row8(reinterpret_cast<const TW*>(p.w) + tok * p.w_rs, c, C, f);
+  const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
+  const int C = p.C;
+  uint32_t n[U];
+  int c[U];
+  int64_t tok[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] *= p.scale;
-  } else {
-    const float x = tok == p.ignore ? 0.f : __uint_as_float(0x7fc00000u);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = x;
+  for (int u = 0; u < U; ++u) {
+    const uint32_t i = first + 256 * u;
+    n[u] = p.per_row.div(i);
+    c[u] = i < p.units ? 8 * (int)(i - n[u] * p.per_row.d) : C;  // C: nothing to move
+    if (i >= p.units) n[u] = 0;
   }
-  store_row8(reinterpret_cast<TY*>(p.y) + (int64_t)n * C, c, C, f);
+  if (p.tok_i64) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) tok[u] = reinterpret_cast<const int64_t*>(p.tokens)[n[u] * p.tok_st];
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) tok[u] = reinterpret_cast<const int32_t*>(p.tokens)[n[u] * p.tok_st];
+  }
+  Row8<TW> w[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const bool word = tok[u] >= 0 && tok[u] < p.V;
+    w[u] = load_raw8<WHOLE>(reinterpret_cast<const TW*>(p.w) + (word ? tok[u] * p.w_rs : 0), c[u], C);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float f[8];
+    w[u].unpack(f);
+    const bool word = tok[u] >= 0 && tok[u] < p.V && tok[u] != p.ignore;
+    const float other = tok[u] == p.ignore ? 0.f : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = word ? f[e] * p.scale : other;
+    store_row8<WHOLE>(reinterpret_cast<TY*>(p.y) + (int64_t)n[u] * C, c[u], C, f);
+  }
 }
 
 // ---- sorting -----------------------------------------------------------------
 
-// Key of a token: itself, or V (behind every word) where it has no gradient.
-__device__ inline uint32_t key_of(const EmbedBwdParams& p, int64_t n) {
-  const int64_t t = token_at(p.tokens, p.tok_i64, p.tok_st, n);
-  return t >= 0 && t < p.V && t != p.ignore ? (uint32_t)t : (uint32_t)p.V;
+// Keys of positions at(0), at(1), ...: the token itself, or V (behind every word)
+// where it has no gradient; some value at and past `end`.  Every token is read
+// before the first is looked at.
+template <int KEYS, typename At>
+__device__ inline void keys_of(const EmbedBwdParams& p, int64_t end, At at, uint32_t (&key)[KEYS]) {
+  int64_t t[KEYS];
+  if (p.tok_i64) {
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) t[i] = at(i) < end ? reinterpret_cast<const int64_t*>(p.tokens)[at(i) * p.tok_st] : 0;
+  } else {
+    int32_t t32[KEYS];
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) t32[i] = at(i) < end ? reinterpret_cast<const int32_t*>(p.tokens)[at(i) * p.tok_st] : 0;
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) t[i] = t32[i];
+  }
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) key[i] = t[i] >= 0 && t[i] < p.V && t[i] != p.ignore ? (uint32_t)t[i] : (uint32_t)p.V;
 }
 
 // Zeros over this workgroup's part of bytes lo..hi of dW (16-byte aligned).
@@ -75,114 +105,151 @@ __device__ inline void clear_part(const EmbedBwdParams& p, int64_t lo, int64_t h
   if (wg == 0 && o < hi) *reinterpret_cast<uint16_t*>(base + o) = 0;
 }
 
-// Positions of a tile's keys among equal digits.  Wave w has keys
-// (w iters + i) 64 + lane in the order of i and lane; the lanes of one digit find
-// each other by a ballot per bit, and the first of them adds their number to the
-// digit's count in count[w], which afterwards holds the wave's keys per digit.
-__device__ inline void rank_keys(const uint32_t (&key)[kKeys], uint32_t (&rank)[kKeys], int iters, int valid, int shift,
-                                 int bits, uint32_t (*count)[kBins]) {
+// A workgroup places up to kEmbedOnce keys stably by a digit.  Each wave owns a run of
+// them; counts[w] first receives the number of wave w's keys of each digit, then
+// the place of the first of them, and a key takes its digit's place and moves it on
+// by one.  Places and numbers have 16 bits, two digits a word.
+typedef uint32_t Counts[kWaves][kBins / 2];
+
+__device__ inline void clear_counts(Counts& counts) {
+  for (int b = threadIdx.x; b < kWaves * kBins / 2; b += kSortThreads) (&counts[0][0])[b] = 0;
+  __syncthreads();
+}
+
+__device__ inline void count_key(Counts& counts, uint32_t d) {
+  atomicAdd(&counts[threadIdx.x >> 6][d >> 1], 1u << (16 * (d & 1)));
+}
+
+// Sum of v over the threads up to this one; `sums` is LDS of one value a wave.
+__device__ inline uint32_t running_sum(uint32_t v, uint32_t* sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int b = threadIdx.x; b < kWaves * kBins; b += kSortThreads) (&count[0][0])[b] = 0;
-  __syncthreads();
-  const uint64_t before = (uint64_t(1) << lane) - 1;
 #pragma unroll
-  for (int i = 0; i < kKeys; ++i) {
-    if (i >= iters) break;
-    const bool on = (wave * iters + i) * 64 + lane < valid;
-    const uint32_t d = (key[i] >> shift) & ((1u << bits) - 1);
-    uint64_t same = __ballot(on);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t m = __ballot((d >> b) & 1);
-      same &= (d >> b) & 1 ? m : ~m;
-    }
-    const bool first = on && (same & before) == 0;
-    uint32_t at = 0;
-    if (first) at = atomicAdd(&count[wave][d], (uint32_t)__popcll(same));
-    // lanes without a key take any lane's
-    rank[i] = __shfl(at, on ? __ffsll((unsigned long long)same) - 1 : lane, 64) + (uint32_t)__popcll(same & before);
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
   }
+  if (lane == 63) sums[wave] = v;
   __syncthreads();
+  for (int w = 0; w < wave; ++w) v += sums[w];
+  return v;
 }
 
-// Exclusive sums over bins and waves: count[w][d] becomes the first place of wave
-// w's keys of digit d, from the start start(d, total of the tile) on, or
-// from the running sum of the tile alone (start == null).
-__device__ inline void place_bins(uint32_t (*count)[kBins], uint32_t* total, const uint32_t* start) {
-  const int d = threadIdx.x;
-  if (d < kBins) {
-    uint32_t s = 0;
+// Numbers into places, in the order of digits, then waves.
+__device__ inline void places(Counts& counts, uint32_t* sums) {
+  __syncthreads();
+  const int d = threadIdx.x;  // a pair of digits
+  uint32_t n[kWaves] = {}, all = 0;
+  if (d < kBins / 2) {
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) n[w] = counts[w][d];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all += n[w];  // either half is 16384 at most: no carry
+  }
+  const uint32_t both = (all & 0xffff) + (all >> 16);
+  const uint32_t low = running_sum(both, sums) - both;
+  if (d < kBins / 2) {
+    uint32_t at = low | (low + (all & 0xffff)) << 16;
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const uint32_t n = count[w][d];
-      count[w][d] = s;
-      s += n;
+      counts[w][d] = at;
+      at += n[w];
     }
-    total[d] = s;
-  }
-  __syncthreads();
-  if (start == nullptr) {
-    // running sum over the bins, doubling the reach each round
-    for (int o = 1; o < kBins; o <<= 1) {
-      const uint32_t v = d < kBins && d >= o ? total[d - o] : 0;
-      __syncthreads();
-      if (d < kBins) total[d] += v;
-      __syncthreads();
-    }
-  }
-  if (d < kBins) {
-    const uint32_t first = start ? start[d] : (d ? total[d - 1] : 0);
-    for (int w = 0; w < kWaves; ++w) count[w][d] += first;
   }
   __syncthreads();
 }
 
-// Workgroup 0: all passes over up to kEmbedTile tokens in LDS.  The others clear dW.
+// The place of this lane's key of digit d, for the lanes that have one: lanes of
+// one digit find each other by a ballot per bit, and the first of them takes places
+// for all, which they fill in the order of lanes.
+__device__ inline uint32_t take_place(Counts& counts, uint32_t d, bool on) {
+  // other: the lanes whose digit differs in some bit, or that have none
+  const uint64_t some = __ballot(on);
+  uint32_t lo = ~(uint32_t)some, hi = ~(uint32_t)(some >> 32);
+#pragma unroll
+  for (int b = 0; b < kEmbedDigit; ++b) {  // a shorter digit's upper bits are zeros of all lanes
+    const uint32_t bit = (uint32_t)((int32_t)(d << (31 - b)) >> 31);
+    const uint64_t m = __ballot(bit != 0);
+    lo |= (uint32_t)m ^ bit;
+    hi |= (uint32_t)(m >> 32) ^ bit;
+  }
+  lo = ~lo;
+  hi = ~hi;
+  const uint32_t before = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
+  uint32_t at = 0;
+  if (on && before == 0) {
+    const uint32_t n = (uint32_t)(__popc(lo) + __popc(hi));
+    at = atomicAdd(&counts[threadIdx.x >> 6][d >> 1], n << (16 * (d & 1))) >> (16 * (d & 1)) & 0xffff;
+  }
+  const int first = lo ? __ffs((int)lo) - 1 : 31 + __ffs((int)hi);
+  return __shfl(at, on ? first : (int)(threadIdx.x & 63), 64) + before;
+}
+
+// Workgroup 0: all passes over up to kEmbedOnce tokens in LDS, the keys at their
+// positions and the positions in the order so far.  The others clear dW.
 __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const EmbedBwdParams p) {
-  __shared__ uint32_t count[kWaves][kBins];
-  __shared__ uint32_t total[kBins];
-  __shared__ uint2 held[kEmbedTile];
+  __shared__ Counts counts;
+  __shared__ uint32_t sums[kWaves];
+  __shared__ uint32_t keys[kEmbedOnce];
+  __shared__ uint16_t order[2][kEmbedOnce];
   if (blockIdx.x > 0) {
     clear_part(p, 0, p.dw_bytes, blockIdx.x - 1, gridDim.x - 1);
     return;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, N = (int)p.N;
-  const int iters = (N + kSortThreads - 1) / kSortThreads;
-  uint32_t key[kKeys], pos[kKeys], rank[kKeys];
+  for (int n0 = threadIdx.x; n0 < N; n0 += 4 * kSortThreads) {
+    const auto at = [&](int i) { return n0 + i * kSortThreads; };
+    uint32_t key[4];
+    keys_of(p, N, at, key);
 #pragma unroll
-  for (int i = 0; i < kKeys; ++i) {
-    const int at = (wave * iters + i) * 64 + lane;
-    pos[i] = at;
-    key[i] = i < iters && at < N ? key_of(p, at) : 0;
+    for (int i = 0; i < 4; ++i)
+      if (at(i) < N) {
+        keys[at(i)] = key[i];
+        order[0][at(i)] = (uint16_t)at(i);
+      }
   }
+  const int run = (N + kSortThreads - 1) / kSortThreads * 64, lo = wave * run;
+  const uint32_t mask = (1u << p.bits) - 1;
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.bits;
-    rank_keys(key, rank, iters, N, shift, p.bits, count);
-    place_bins(count, total, nullptr);
-#pragma unroll
-    for (int i = 0; i < kKeys; ++i)
-      if (i < iters && (wave * iters + i) * 64 + lane < N)
-        held[count[wave][(key[i] >> shift) & ((1u << p.bits) - 1)] + rank[i]] = make_uint2(key[i], pos[i]);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kKeys; ++i) {
-      const int at = (wave * iters + i) * 64 + lane;
-      if (i < iters && at < N) {
-        const uint2 h = held[at];
-        key[i] = h.x;
-        pos[i] = h.y;
-      }
+    const uint16_t* from = order[pass & 1];
+    uint16_t* to = order[~pass & 1];
+    clear_counts(counts);
+    for (int at = lo + lane; at < lo + run; at += 64)
+      if (at < N) count_key(counts, keys[from[at]] >> shift & mask);
+    places(counts, sums);
+    for (int at = lo + lane; at < lo + run; at += 64) {
+      const bool on = at < N;
+      const uint32_t pos = on ? from[at] : 0;
+      const uint32_t place = take_place(counts, keys[pos] >> shift & mask, on);
+      if (on) to[place] = (uint16_t)pos;
     }
     __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < kKeys; ++i) {
-    const int at = (wave * iters + i) * 64 + lane;
-    if (i < iters && at < N) p.sorted[at] = make_uint2(key[i], pos[i]);
+  for (int at = threadIdx.x; at < N; at += kSortThreads) {
+    const uint32_t pos = order[p.passes & 1][at];
+    p.sorted[at] = make_uint2(keys[pos], pos);
   }
 }
 
-// The tile's keys of one pass, from the tokens in the first.
-__device__ inline uint2 tile_key(const EmbedBwdParams& p, const uint2* from, int64_t n) {
-  return from ? from[n] : make_uint2(key_of(p, n), (uint32_t)n);
+// Keys and positions of a tile, from the tokens in the first pass.
+constexpr int kKeys = kEmbedTile / kSortThreads;
+template <typename At>
+__device__ inline void tile_keys(const EmbedBwdParams& p, const uint2* from, At at, uint32_t (&key)[kKeys],
+                                 uint32_t (&pos)[kKeys]) {
+  if (from) {
+    uint2 k[kKeys];
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) k[i] = at(i) < p.N ? from[at(i)] : make_uint2(0, 0);
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      key[i] = k[i].x;
+      pos[i] = k[i].y;
+    }
+  } else {
+    keys_of(p, p.N, at, key);
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) pos[i] = (uint32_t)at(i);
+  }
 }
 
 // Digit counts of every tile; workgroups behind the tiles clear their part.
@@ -196,11 +263,12 @@ __global__ __launch_bounds__(kSortThreads) void embed_count_kernel(const EmbedBw
   for (int b = threadIdx.x; b < kBins; b += kSortThreads) count[b] = 0;
   __syncthreads();
   const int64_t n0 = (int64_t)blockIdx.x * kEmbedTile;
+  const auto at = [&](int i) { return n0 + i * kSortThreads + threadIdx.x; };
+  uint32_t key[kKeys], pos[kKeys];
+  tile_keys(p, from, at, key, pos);
 #pragma unroll
-  for (int i = 0; i < kKeys; ++i) {
-    const int64_t n = n0 + i * kSortThreads + threadIdx.x;
-    if (n < p.N) atomicAdd(&count[(tile_key(p, from, n).x >> shift) & ((1u << p.bits) - 1)], 1u);
-  }
+  for (int i = 0; i < kKeys; ++i)
+    if (at(i) < p.N) atomicAdd(&count[key[i] >> shift & ((1u << p.bits) - 1)], 1u);
   __syncthreads();
   for (int b = threadIdx.x; b < kBins; b += kSortThreads) p.counts[(int64_t)blockIdx.x * kBins + b] = count[b];
 }
@@ -208,121 +276,185 @@ __global__ __launch_bounds__(kSortThreads) void embed_count_kernel(const EmbedBw
 // Every tile's keys to their places of this pass.
 __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(const EmbedBwdParams p, const uint2* from, uint2* to,
                                                                    int shift, int64_t lo, int64_t hi) {
-  __shared__ uint32_t count[kWaves][kBins];
-  __shared__ uint32_t total[kBins], start[kBins];
+  __shared__ Counts counts;
+  __shared__ uint32_t sums[2][kWaves], base[kBins];
   if ((int)blockIdx.x >= p.n_tiles) {
     clear_part(p, lo, hi, blockIdx.x - p.n_tiles, gridDim.x - p.n_tiles);
     return;
   }
-  // first place of each digit for this tile: all smaller digits, and this
-  // digit in the tiles before
-  const int d = threadIdx.x;
-  uint32_t mine = 0, all = 0;
-  if (d < kBins) {
-    for (int t = 0; t < p.n_tiles; ++t) {
-      const uint32_t n = p.counts[(int64_t)t * kBins + d];
-      if (t < (int)blockIdx.x) mine += n;
-      all += n;
-    }
-    total[d] = all;
-  }
-  __syncthreads();
-  for (int o = 1; o < kBins; o <<= 1) {
-    const uint32_t v = d < kBins && d >= o ? total[d - o] : 0;
-    __syncthreads();
-    if (d < kBins) total[d] += v;
-    __syncthreads();
-  }
-  if (d < kBins) start[d] = total[d] - all + mine;
-  __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t n0 = (int64_t)blockIdx.x * kEmbedTile;
-  const int valid = (int)(p.N - n0 < kEmbedTile ? p.N - n0 : kEmbedTile);
-  uint32_t key[kKeys], pos[kKeys], rank[kKeys];
-#pragma unroll
-  for (int i = 0; i < kKeys; ++i) {
-    const int at = (wave * kKeys + i) * 64 + lane;
-    const uint2 k = at < valid ? tile_key(p, from, n0 + at) : make_uint2(0, 0);
-    key[i] = k.x;
-    pos[i] = k.y;
-  }
-  rank_keys(key, rank, kKeys, valid, shift, p.bits, count);
-  place_bins(count, total, start);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const auto at = [&](int i) { return n0 + (wave * kKeys + i) * 64 + lane; };
+  const uint32_t mask = (1u << p.bits) - 1;
+  uint32_t key[kKeys], pos[kKeys];
+  tile_keys(p, from, at, key, pos);
+  clear_counts(counts);
 #pragma unroll
   for (int i = 0; i < kKeys; ++i)
-    if ((wave * kKeys + i) * 64 + lane < valid)
-      to[count[wave][(key[i] >> shift) & ((1u << p.bits) - 1)] + rank[i]] = make_uint2(key[i], pos[i]);
+    if (at(i) < p.N) count_key(counts, key[i] >> shift & mask);
+  // of each digit: the keys in the tiles before, and in all
+  const int d = threadIdx.x;
+  uint32_t before = 0, all = 0;
+  if (d < kBins) {
+    const uint32_t* of = p.counts + d;
+#pragma unroll 8
+    for (int t = 0; t < p.n_tiles; ++t) {
+      const uint32_t n = of[(int64_t)t * kBins];
+      before += t < (int)blockIdx.x ? n : 0;
+      all += n;
+    }
+  }
+  const uint32_t smaller = running_sum(all, sums[0]) - all;
+  places(counts, sums[1]);
+  // from a place among the tile's keys to one among all keys
+  if (d < kBins) base[d] = smaller + before - (counts[0][d >> 1] >> (16 * (d & 1)) & 0xffff);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kKeys; ++i) {
+    const uint32_t digit = key[i] >> shift & mask;
+    const uint32_t place = take_place(counts, digit, at(i) < p.N);
+    if (at(i) < p.N) to[base[digit] + place] = make_uint2(key[i], pos[i]);
+  }
 }
 
 // ---- sums --------------------------------------------------------------------
 
-template <typename TW, typename TY>
-__global__ __launch_bounds__(256) void embed_sum_kernel(const EmbedBwdParams p) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= p.units) return;
-  const uint32_t chunk = p.per_row.div(i);
-  const int c = 8 * (int)(i - chunk * p.per_row.d), C = p.C;
-  const int64_t lo = (int64_t)chunk * p.chunk, hi = lo + p.chunk < p.N ? lo + p.chunk : p.N;
-  uint32_t word = p.sorted[lo].x;
-  if (word == (uint32_t)p.V) return;
-  // the chunk's first word may have begun before it
-  bool head = lo > 0 && p.sorted[lo - 1].x == word;
-  const TY* dy = reinterpret_cast<const TY*>(p.dy);
-  TW* dw = reinterpret_cast<TW*>(p.dw);
-  float acc[8] = {};
-  auto finish = [&](bool open) {  // open: the word goes on in the next chunk
-    if (head) {
-      store_row8(p.head + (int64_t)chunk * C, c, C, acc);
-    } else if (open) {
-      store_row8(p.tail + (int64_t)chunk * C, c, C, acc);
-    } else {
-      float o[8];
+// A wave sums 256 channels of a chunk, four a lane.  Its lanes read the chunk's
+// positions in one piece; which word a row belongs to is the same for all of them,
+// so the rows' addresses and the branches at a word's end are scalar, and kRows rows
+// at a time are on their way before the first is added.
+constexpr int kRows = 16;
+
+template <bool WHOLE, typename T>
+__device__ inline void store4(T* p, const float (&f)[4], int n) {
+  if (n == 4) {
+    Row4<T>::store(p, f);
+  } else if (!WHOLE) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = acc[e] * p.scale;
-      store_row8(dw + (int64_t)word * C, c, C, o);
-    }
-  };
-  for (int64_t n = lo; n < hi; ++n) {
-    const uint2 k = p.sorted[n];
-    if (k.x != word) {
-      finish(false);
-      head = false;
-      word = k.x;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-      if (word == (uint32_t)p.V) return;
-    }
-    float f[8];
-    load_row8(dy + (int64_t)k.y * p.dy_rs, c, C, f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += f[e];
+    for (int e = 0; e < 3; ++e)
+      if (e < n) p[e] = static_cast<T>(f[e]);
   }
-  finish(hi < p.N && p.sorted[hi].x == word);
 }
 
-// Words that cross chunks: the chunk where one begins adds its partials.
-template <typename TW>
-__global__ __launch_bounds__(256) void embed_join_kernel(const EmbedBwdParams p) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+template <typename TW, typename TY, bool WHOLE>  // WHOLE: C is a multiple of 4
+__global__ __launch_bounds__(256) void embed_sum_kernel(const EmbedBwdParams p) {
+  const uint32_t i = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   if (i >= p.units) return;
   const uint32_t chunk = p.per_row.div(i);
-  const int c = 8 * (int)(i - chunk * p.per_row.d), C = p.C;
-  const int64_t lo = (int64_t)chunk * p.chunk, hi = lo + p.chunk;
-  if (hi >= p.N) return;
-  const uint32_t word = p.sorted[hi - 1].x;
+  const int lane = threadIdx.x & 63, C = p.C;
+  const int c = 256 * (int)(i - chunk * p.per_row.d) + 4 * lane;
+  // a lane behind the row's end reads its beginning and stores nothing
+  const int at = c < C ? c : 0, have = C - at < 4 ? C - at : 4, put = c < C ? have : 0;
+  const int64_t lo = (int64_t)chunk * p.chunk;
+  const int n = (int)(p.N - lo < p.chunk ? p.N - lo : p.chunk);
+  const uint32_t V = (uint32_t)p.V;
+  const uint2 mine = lane < n ? p.sorted[lo + lane] : make_uint2(V, 0);
+  const uint32_t left = lo > 0 ? p.sorted[lo - 1].x : V, right = lo + n < p.N ? p.sorted[lo + n].x : V;
+  const TY* dy = reinterpret_cast<const TY*>(p.dy);
+  TW* dw = reinterpret_cast<TW*>(p.dw);
+  const int live = __popcll(__ballot(mine.x != V));  // words come first
+  uint32_t word = V;  // none yet
+  bool head = false;  // the chunk's first word has begun before it
+  float acc[4] = {};
+  auto finish = [&](bool open) {  // open: the word goes on in the next chunk
+    if (head || open) {
+      store4<WHOLE>((head ? p.head : p.tail) + (int64_t)chunk * C + c, acc, put);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] *= p.scale;
+      store4<WHOLE>(dw + (int64_t)word * C + c, acc, put);
+    }
+  };
+  for (int j0 = 0; j0 < live; j0 += kRows) {
+    Row4<TY> rows[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const uint32_t row = __builtin_amdgcn_readlane(mine.y, j0 + j < live ? j0 + j : 0);
+      const TY* from = dy + (int64_t)row * p.dy_rs + at;
+      if (WHOLE || have == 4) rows[j] = Row4<TY>::load(from);
+      else rows[j] = Row4<TY>::load_part(from, have);
+    }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      if (j0 + j >= live) break;
+      const uint32_t w = __builtin_amdgcn_readlane(mine.x, j0 + j);
+      if (w != word) {
+        if (j0 + j == 0) head = w == __builtin_amdgcn_readfirstlane(left);
+        else finish(false), head = false;
+        word = w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = 0.f;
+      }
+      float f[4];
+      rows[j].unpack(f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += f[e];
+    }
+  }
+  if (word != V) finish(word == __builtin_amdgcn_readfirstlane(right));
+}
+
+// Words that cross chunks: the workgroups of the chunk where one begins add its
+// partials, kLanes of them at a time for 32 groups of 8 channels, each lane's in
+// order and then the lanes in order.
+constexpr int kLanes = 16;
+
+template <typename TW>
+__global__ __launch_bounds__(32 * kLanes) void embed_join_kernel(const EmbedBwdParams p) {
+  __shared__ float sums[kLanes][8][33];
+  const int64_t chunk = blockIdx.x, lo = chunk * p.chunk, hi = lo + p.chunk;
+  const uint32_t word = p.sorted[hi - 1].x;  // the grid has no workgroup of the last chunk
   if (word == (uint32_t)p.V || p.sorted[hi].x != word) return;
   if (lo > 0 && p.sorted[lo - 1].x == word) return;  // begun in an earlier chunk
-  float acc[8];
-  load_row8(p.tail + (int64_t)chunk * C, c, C, acc);
-  for (int64_t k = chunk + 1; k * p.chunk < p.N && p.sorted[k * p.chunk].x == word; ++k) {
-    float f[8];
-    load_row8(p.head + k * C, c, C, f);
+  // the last chunk whose first word it is, 64 candidates a step: near ones, then
+  // ones 64 times as far apart as long as all are, and back
+  const int64_t n_chunks = (p.N + p.chunk - 1) / p.chunk;
+  int64_t in = chunk + 1, step = 1;
+  for (bool out = true;;) {
+    const int64_t k = in + step * (1 + (threadIdx.x & 63));
+    const uint64_t is = __ballot(k < n_chunks && p.sorted[k < n_chunks ? k * p.chunk : 0].x == word);
+    const int more = ~is ? __builtin_ctzll(~is) : 64;
+    in += step * more;
+    if (out && more == 64) {
+      step *= 64;
+    } else if (step == 1) {
+      break;
+    } else {
+      out = false;
+      step /= 64;
+    }
+  }
+  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5;
+  const int c = 8 * (int)(blockIdx.y * 32 + col), C = p.C;
+  float acc[8] = {};
+  if (c < C) {
+    if (lane == 0) load_row8(p.tail + chunk * C, c, C, acc);
+#pragma unroll 4
+    for (int64_t k = chunk + 1 + lane; k <= in; k += kLanes) {
+      float f[8];
+      load_row8(p.head + k * C, c, C, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += f[e];
+      for (int e = 0; e < 8; ++e) acc[e] += f[e];
+    }
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] *= p.scale;
+  for (int e = 0; e < 8; ++e) sums[lane][e][col] = acc[e];
+  __syncthreads();
+  if (lane != 0 || c >= C) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float x = acc[e];
+    for (int l = 1; l < kLanes; ++l) x += sums[l][e][col];
+    acc[e] = x * p.scale;
+  }
   store_row8(reinterpret_cast<TW*>(p.dw) + (int64_t)word * C, c, C, acc);
+}
+
+template <typename TW, typename TY>
+void sum(const EmbedBwdParams& p, hipStream_t s) {
+  const dim3 grid((p.units + 3) / 4), wg(256);
+  if (p.C % 4 == 0) hipLaunchKernelGGL((embed_sum_kernel<TW, TY, true>), grid, wg, 0, s, p);
+  else hipLaunchKernelGGL((embed_sum_kernel<TW, TY, false>), grid, wg, 0, s, p);
 }
 
 template <typename TW>
@@ -333,7 +465,7 @@ hipError_t bwd_t(const EmbedBwdParams& p, int dtype, hipStream_t s) {
                        p.dw_bytes);
     return hipGetLastError();
   }
-  if (p.n_tiles == 1) {
+  if (p.N <= kEmbedOnce) {
     hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)(1 + p.n_clear)), sort_wg, 0, s, p);
   } else {
     // an equal part of the zeros beside each of the 2 x passes launches; the
@@ -355,21 +487,33 @@ hipError_t bwd_t(const EmbedBwdParams& p, int dtype, hipStream_t s) {
       from = to;
     }
   }
-  const dim3 grid((p.units + 255) / 256), wg(256);
-  if (dtype == kF32) hipLaunchKernelGGL((embed_sum_kernel<TW, float>), grid, wg, 0, s, p);
-  else if (dtype == kBF16) hipLaunchKernelGGL((embed_sum_kernel<TW, __bf16>), grid, wg, 0, s, p);
-  else hipLaunchKernelGGL((embed_sum_kernel<TW, _Float16>), grid, wg, 0, s, p);
-  if (p.N > p.chunk) hipLaunchKernelGGL((embed_join_kernel<TW>), grid, wg, 0, s, p);
+  if (dtype == kF32) sum<TW, float>(p, s);
+  else if (dtype == kBF16) sum<TW, __bf16>(p, s);
+  else sum<TW, _Float16>(p, s);
+  const int64_t n_chunks = (p.N + p.chunk - 1) / p.chunk;
+  if (n_chunks > 1)
+    hipLaunchKernelGGL((embed_join_kernel<TW>), dim3((unsigned)(n_chunks - 1), (unsigned)((p.C + 255) / 256)), dim3(32 * kLanes),
+                       0, s, p);
   return hipGetLastError();
 }
 
+template <typename TW, typename TY, bool WHOLE>
+hipError_t fwd_tt(const EmbedParams& p, hipStream_t s) {
+  if (p.units < kWideUnits)
+    hipLaunchKernelGGL((embed_fwd_kernel<TW, TY, 1, WHOLE>), dim3((p.units + 255) / 256), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((embed_fwd_kernel<TW, TY, 4, WHOLE>), dim3((p.units + 1023) / 1024), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+template <typename TW, typename TY>
+hipError_t fwd_tt(const EmbedParams& p, hipStream_t s) {
+  return p.C % 8 == 0 ? fwd_tt<TW, TY, true>(p, s) : fwd_tt<TW, TY, false>(p, s);
+}
 template <typename TW>
 hipError_t fwd_t(const EmbedParams& p, int dtype, hipStream_t s) {
-  const dim3 grid((p.units + 255) / 256), wg(256);
-  if (dtype == kF32) hipLaunchKernelGGL((embed_fwd_kernel<TW, float>), grid, wg, 0, s, p);
-  else if (dtype == kBF16) hipLaunchKernelGGL((embed_fwd_kernel<TW, __bf16>), grid, wg, 0, s, p);
-  else hipLaunchKernelGGL((embed_fwd_kernel<TW, _Float16>), grid, wg, 0, s, p);
-  return hipGetLastError();
+  if (dtype == kF32) return fwd_tt<TW, float>(p, s);
+  if (dtype == kBF16) return fwd_tt<TW, __bf16>(p, s);
+  return fwd_tt<TW, _Float16>(p, s);
 }
 
 }  // namespace

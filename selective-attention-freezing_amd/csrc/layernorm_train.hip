@@ -17,8 +17,8 @@
 // 8 (TPR k + thread): every load and store of the group is one run.
 //
 // Backward: a workgroup walks rows a grid apart and keeps its share of dw and db
-// of its threads' channels in registers; at the end it adds its row groups in LDS
-// and writes one (2, C) float32 partial, and a second kernel adds the partials in
+// of its threads' channels in registers; at the end it adds its waves in LDS and
+// writes one (2, C) float32 partial, and a second kernel adds the partials in
 // a fixed order, so the weight gradients are the same in every run.
 #include "saf_kernels.h"
 #include "saf_rowio.h"
@@ -62,22 +62,32 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTr
   if (row >= p.rows) return;
   const int C = p.C;
   const TX* xr = reinterpret_cast<const TX*>(p.x) + row * p.x_rs;
+  Row8<TX> x[NCH];
   float v[NCH][8];
 #pragma unroll
-  for (int k = 0; k < NCH; ++k) load_row8(xr, 8 * (TPR * k + t), C, v[k]);
+  for (int k = 0; k < NCH; ++k) x[k] = load_raw8(xr, 8 * (TPR * k + t), C);
+  float w[NCH][8], b[NCH][8] = {};
+  load_vec<NCH>(p.w, p.wb_dtype, 8 * t, 8 * TPR, C, w);
+  if (p.b) load_vec<NCH>(p.b, p.wb_dtype, 8 * t, 8 * TPR, C, b);
   if (p.delta) {
     const TB* dr = reinterpret_cast<const TB*>(p.delta) + row * p.d_rs;
     TX* rr = reinterpret_cast<TX*>(p.r) + row * C;
+    Row8<TB> a[NCH];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) a[k] = load_raw8(dr, 8 * (TPR * k + t), C);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = 8 * (TPR * k + t);
       float d[8];
-      load_row8(dr, c, C, d);
+      x[k].unpack(v[k]);
+      a[k].unpack(d);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[k][e] = (float)static_cast<TX>(v[k][e] + d[e]);
-      store_row8(rr, c, C, v[k]);
+      for (int e = 0; e < 8; ++e) v[k][e] += d[e];
+      store_row8(rr, 8 * (TPR * k + t), C, v[k]);
+      x[k] = Row8<TX>::pack(v[k]);
     }
   }
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) x[k].unpack(v[k]);
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < NCH; ++k)
@@ -100,41 +110,45 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTr
   TB* yr = reinterpret_cast<TB*>(p.y) + row * C;
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
-    const int c = 8 * (TPR * k + t);
-    if (c >= C) continue;
-    float w[8], b[8] = {};
-    load_vec8(p.w, p.wb_dtype, c, C, w);
-    if (p.b) load_vec8(p.b, p.wb_dtype, c, C, b);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = fmaf((v[k][e] - mean) * rstd, w[e], b[e]);
-    store_row8(yr, c, C, w);
+    for (int e = 0; e < 8; ++e) w[k][e] = fmaf((v[k][e] - mean) * rstd, w[k][e], b[k][e]);
+    store_row8(yr, 8 * (TPR * k + t), C, w[k]);
   }
 }
 
 template <typename TX, typename TB, int TPR, int NCH>
 __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTrainBwdParams p) {
   __shared__ float slots[2][TPR > 64 ? TPR / 64 : 1];
-  __shared__ float2 part[TPR >= 256 ? 1 : 8 * TPR * NCH];
+  // dw and db of the four waves of a workgroup whose rows are a wave's or less
+  constexpr int kCols = 8 * TPR * NCH;
+  __shared__ float2 part[TPR >= 256 ? 1 : 4][TPR >= 256 ? 1 : kCols];
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int C = p.C;
-  float w[NCH][8], aw[NCH][8], ab[NCH][8];
-#pragma unroll
-  for (int k = 0; k < NCH; ++k) {
-    const int c = 8 * (TPR * k + t);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[k][e] = aw[k][e] = ab[k][e] = 0.f;
-    if (c < C) load_vec8(p.w, p.w_dtype, c, C, w[k]);
-  }
+  float w[NCH][8], aw[NCH][8] = {}, ab[NCH][8] = {};
+  load_vec<NCH>(p.w, p.w_dtype, 8 * t, 8 * TPR, C, w);
   for (int64_t row = (int64_t)blockIdx.x * kGroups<TPR> + group; row < p.rows;
        row += (int64_t)gridDim.x * kGroups<TPR>) {
     const TX* rr = reinterpret_cast<const TX*>(p.r) + row * p.r_rs;
     const TB* gr = reinterpret_cast<const TB*>(p.dy) + row * p.dy_rs;
     const float mean = p.stats[2 * row], rstd = p.stats[2 * row + 1];
+    constexpr bool kTogether = TPR <= 256;  // sixteen waves have no registers for dr as well
+    Row8<TX> r[NCH], add[NCH];
+    Row8<TB> dy[NCH];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) r[k] = load_raw8(rr, 8 * (TPR * k + t), C);
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) dy[k] = load_raw8(gr, 8 * (TPR * k + t), C);
+    const TX* er = reinterpret_cast<const TX*>(p.dr) + row * p.dr_rs;
+    if (kTogether && p.dr) {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) add[k] = load_raw8(er, 8 * (TPR * k + t), C);
+    }
     float xh[NCH][8], g[NCH][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) load_row8(rr, 8 * (TPR * k + t), C, xh[k], mean);
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) load_row8(gr, 8 * (TPR * k + t), C, g[k]);
+    for (int k = 0; k < NCH; ++k) {
+      r[k].unpack(xh[k]);
+      dy[k].unpack(g[k]);
+    }
 #pragma unroll
     for (int k = 0; k < NCH; ++k)
 #pragma unroll
@@ -156,7 +170,10 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
       const int c = 8 * (TPR * k + t);
       if (c >= C) continue;
       float d[8] = {};
-      if (p.dr) load_row8(reinterpret_cast<const TX*>(p.dr) + row * p.dr_rs, c, C, d);
+      if (p.dr) {
+        if constexpr (!kTogether) add[k] = load_raw8(er, c, C);
+        add[k].unpack(d);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = fmaf(rstd, g[k][e] - c1 - xh[k][e] * c2, d[e]);
       if (p.dx) store_row8(dxr, c, C, d);
@@ -165,27 +182,27 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
   }
   if (!p.part) return;
   float* out = p.part + (int64_t)blockIdx.x * 2 * C;
-  if constexpr (kGroups<TPR> > 1) {
-    for (int i = 0; i < kGroups<TPR>; ++i) {
-      if (group == i)
-#pragma unroll
-        for (int k = 0; k < NCH; ++k)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float2& a = part[(8 * k + e) * TPR + t];
-            a = i == 0 ? make_float2(aw[k][e], ab[k][e]) : make_float2(a.x + aw[k][e], a.y + ab[k][e]);
-          }
-      __syncthreads();
-    }
-    if (group != 0) return;
+  if constexpr (TPR < 256) {
+    const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int k = 0; k < NCH; ++k)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float2 a = part[(8 * k + e) * TPR + t];
-        aw[k][e] = a.x;
-        ab[k][e] = a.y;
+        if constexpr (TPR == 32) {  // the wave's two rows
+          aw[k][e] = half_swap_sum(aw[k][e]);
+          ab[k][e] = half_swap_sum(ab[k][e]);
+        }
+        if (TPR == 64 || group % 2 == 0) part[wave][(8 * k + e) * TPR + t] = make_float2(aw[k][e], ab[k][e]);
       }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kCols; i += 256) {
+      const int c = 8 * (i / (8 * TPR) * TPR + i % TPR) + i / TPR % 8;
+      if (c >= C) continue;
+      const float2 p0 = part[0][i], p1 = part[1][i], p2 = part[2][i], p3 = part[3][i];
+      out[c] = (p0.x + p1.x) + (p2.x + p3.x);
+      out[C + c] = (p0.y + p1.y) + (p2.y + p3.y);
+    }
+    return;
   }
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {

@@ -10,7 +10,8 @@ using namespace saf;
 namespace {
 
 constexpr int64_t kMaxUnits = 0x7fffffff;
-constexpr int64_t kMaxC = int64_t(1) << 24;
+constexpr int64_t kEmbedWaves = 4096;
+constexpr int64_t kMaxC = int64_t(1) << 23;
 
 bool float_dtype(int d) { return d == SAF_F32 || d == SAF_F16 || d == SAF_BF16; }
 bool given(const saf_tensor_t* t) { return t != nullptr && t->ndim > 0; }
@@ -75,7 +76,7 @@ int check_tokens(const saf_tensor_t* t) {
 
 int check_table(int64_t V, int64_t C) {
   if (V < 1 || C < 1) return fail(SAF_EINVAL, "the embedding must have rows and channels");
-  if (V >= kMaxUnits || C > kMaxC) return fail(SAF_EUNSUPPORTED, "an embedding of 2^31 rows, or of more than 2^24 channels");
+  if (V >= kMaxUnits || C > kMaxC) return fail(SAF_EUNSUPPORTED, "an embedding of 2^31 rows, or of more than 2^23 channels");
   return SAF_OK;
 }
 
@@ -86,10 +87,11 @@ struct EmbedPlan {
   int64_t n_chunks, at_sorted2, at_counts, at_head, at_tail, bytes;
 };
 
-// Positions per chunk.  Few, so that short batches fill the card; more from 2^17
-// positions on, where the partial sums of the words that cross chunks would
-// otherwise be what the pass reads.
-int chunk_of(int64_t N) { return N < (int64_t(1) << 17) ? 16 : 64; }
+// Positions per chunk: as many as leave the card 4096 waves, from 16 to 64.
+int chunk_of(int64_t N, int64_t C) {
+  const int64_t waves = (N + 63) / 64 * ((C + 255) / 256);
+  return waves >= kEmbedWaves ? 64 : (2 * waves >= kEmbedWaves ? 32 : 16);
+}
 
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
@@ -100,13 +102,13 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int64_t C) {
   while ((V >> key_bits) != 0) ++key_bits;
   e.passes = (key_bits + kEmbedDigit - 1) / kEmbedDigit;
   e.bits = (key_bits + e.passes - 1) / e.passes;
-  e.chunk = chunk_of(N);
+  e.chunk = chunk_of(N, C);
   e.n_chunks = (N + e.chunk - 1) / e.chunk;
   int64_t at = up256(8 * N);
   e.at_sorted2 = at;
-  if (e.n_tiles > 1 && e.passes > 1) at += up256(8 * N);
+  if (N > kEmbedOnce && e.passes > 1) at += up256(8 * N);
   e.at_counts = at;
-  if (e.n_tiles > 1) at += up256(4 * ((int64_t)e.n_tiles << kEmbedDigit));
+  if (N > kEmbedOnce) at += up256(4 * ((int64_t)e.n_tiles << kEmbedDigit));
   e.at_head = at;
   if (e.n_chunks > 1) at += up256(4 * e.n_chunks * C);
   e.at_tail = at;
@@ -122,7 +124,7 @@ int pack_params(const char* what, const saf_tensor_t* x, const char* x_name, con
   if (int rc = check_float(x, x_name)) return rc;
   if (x->ndim != 2) return fail(SAF_EINVAL, "%s must be 2-D (rows, C)", x_name);
   const int64_t R = x->size[0], C = x->size[1];
-  if (C < 1 || C > kMaxC) return fail(SAF_EUNSUPPORTED, "%s: C = %lld is not supported (1 to 2^24)", what, (long long)C);
+  if (C < 1 || C > kMaxC) return fail(SAF_EUNSUPPORTED, "%s: C = %lld is not supported (1 to 2^23)", what, (long long)C);
   if (int rc = check_rows(x, x_name, R, C, false)) return rc;
   const int64_t nb = (C + 31) / 32;
   if (int rc = check_rows(q, "q", R, C, true)) return rc;
@@ -197,7 +199,7 @@ int saf_embed_bwd(const saf_tensor_t* tokens, const saf_tensor_t* dout, float sc
   if (!types_meet(dweight->dtype, dout->dtype)) return fail(SAF_EUNSUPPORTED, "embed: bf16 beside fp16");
   const EmbedPlan e = embed_plan(N, V, C);
   EmbedBwdParams p{};
-  if (int rc = units_of("embed", e.n_chunks, (C + 7) / 8, p.per_row, p.units)) return rc;
+  if (int rc = units_of("embed", e.n_chunks, (C + 255) / 256, p.per_row, p.units)) return rc;
   if (int rc = check_workspace("embed_bwd", workspace, workspace_bytes, e.bytes)) return rc;
   char* ws = reinterpret_cast<char*>(workspace);
   p.tokens = tokens->data;

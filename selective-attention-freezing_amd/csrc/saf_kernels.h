@@ -384,9 +384,10 @@ struct ActPackParams {
 };
 enum class ActPackOp { kPack, kUnpack, kGelu, kGeluBwd };
 
-// Embedding lookup and gradient (embed.hip); a unit is 8 channels of a token, of
-// a chunk of sorted positions in the backward pass.
-constexpr int kEmbedTile = 8192;  // tokens that one workgroup sorts
+// Embedding lookup and gradient (embed.hip); a unit is 8 channels of a token, in the
+// backward pass 256 channels of a chunk of at most 64 sorted positions.
+constexpr int kEmbedOnce = 8192;   // tokens that one workgroup sorts by itself
+constexpr int kEmbedTile = 2048;  // a workgroup's part of more
 constexpr int kEmbedDigit = 9;    // bits of a sorting pass at most
 struct EmbedParams {
   const void* tokens;
@@ -413,8 +414,8 @@ struct EmbedBwdParams {
   float scale;
   int C;
   uint2* sorted;    // (N) token, position
-  uint2* sorted2;   // (N) with more than one tile and pass
-  uint32_t* counts; // (n_tiles, 2^kEmbedDigit) with more than one tile
+  uint2* sorted2;   // (N) with more than kEmbedOnce tokens and one pass
+  uint32_t* counts; // (n_tiles, 2^kEmbedDigit) with more than kEmbedOnce tokens
   float* head;      // (chunks, C) sums of a chunk's first word where that began before it
   float* tail;      // (chunks, C) sums of its last word where that goes on
   int n_tiles, n_clear, passes, bits, chunk;

@@ -13,68 +13,150 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
+// Eight elements as they lie in memory, and as float32.  Kernels load all the
+// pieces that they need before they unpack the first, so that they wait for memory
+// once and not once a piece.
 template <typename T> struct Row8 {
-  static __device__ inline void load(const T* p, float (&f)[8]) {
-    const u32x4_any r = *reinterpret_cast<const u32x4_any*>(p);
+  u32x4_any raw;
+  __device__ inline void unpack(float (&f)[8]) const {
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      f[2 * m] = Elem<T>::lo(r[m]);
-      f[2 * m + 1] = Elem<T>::hi(r[m]);
+      f[2 * m] = Elem<T>::lo(raw[m]);
+      f[2 * m + 1] = Elem<T>::hi(raw[m]);
     }
   }
-  static __device__ inline void store(T* p, const float (&f)[8]) {
-    u32x4_any r;
+  static __device__ inline Row8 pack(const float (&f)[8]) {
+    Row8 r;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) r[m] = Elem<T>::pack2(f[2 * m], f[2 * m + 1]);
-    *reinterpret_cast<u32x4_any*>(p) = r;
+    for (int m = 0; m < 4; ++m) r.raw[m] = Elem<T>::pack2(f[2 * m], f[2 * m + 1]);
+    return r;
+  }
+  static __device__ inline Row8 load(const T* p) { return {*reinterpret_cast<const u32x4_any*>(p)}; }
+  __device__ inline void store(T* p) const { *reinterpret_cast<u32x4_any*>(p) = raw; }
+  // its first n < 8 elements, the rest zero
+  static __device__ inline Row8 load_part(const T* p, int n) {
+    Row8 r{};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) r.raw[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+    return r;
+  }
+  __device__ inline void store_part(T* p, int n) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(raw[e / 2] >> (16 * (e & 1)));
   }
 };
 template <> struct Row8<float> {
-  static __device__ inline void load(const float* p, float (&f)[8]) {
-    const f32x4_any a = *reinterpret_cast<const f32x4_any*>(p), b = *reinterpret_cast<const f32x4_any*>(p + 4);
+  f32x4_any raw[2];
+  __device__ inline void unpack(float (&f)[8]) const {
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      f[m] = a[m];
-      f[m + 4] = b[m];
-    }
+    for (int e = 0; e < 8; ++e) f[e] = raw[e / 4][e % 4];
   }
-  static __device__ inline void store(float* p, const float (&f)[8]) {
-    f32x4_any a, b;
+  static __device__ inline Row8 pack(const float (&f)[8]) {
+    Row8 r;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      a[m] = f[m];
-      b[m] = f[m + 4];
-    }
-    *reinterpret_cast<f32x4_any*>(p) = a;
-    *reinterpret_cast<f32x4_any*>(p + 4) = b;
+    for (int e = 0; e < 8; ++e) r.raw[e / 4][e % 4] = f[e];
+    return r;
+  }
+  static __device__ inline Row8 load(const float* p) {
+    return {{*reinterpret_cast<const f32x4_any*>(p), *reinterpret_cast<const f32x4_any*>(p + 4)}};
+  }
+  __device__ inline void store(float* p) const {
+    *reinterpret_cast<f32x4_any*>(p) = raw[0];
+    *reinterpret_cast<f32x4_any*>(p + 4) = raw[1];
+  }
+  static __device__ inline Row8 load_part(const float* p, int n) {
+    Row8 r{};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) r.raw[e / 4][e % 4] = p[e];
+    return r;
+  }
+  __device__ inline void store_part(float* p, int n) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = raw[e / 4][e % 4];
   }
 };
 
-// Elements c..c+7 of a row of C; those past it are `past` / not stored.
-template <typename T>
-__device__ inline void load_row8(const T* row, int c, int C, float (&f)[8], float past = 0.f) {
-  if (c + 8 <= C) {
-    Row8<T>::load(row + c, f);
-  } else {
+// Four elements.
+typedef uint32_t u32x2_e2 __attribute__((ext_vector_type(2), aligned(2)));
+template <typename T> struct Row4 {
+  u32x2_e2 raw;
+  __device__ inline void unpack(float (&f)[4]) const {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = c + e < C ? (float)row[c + e] : past;
+    for (int m = 0; m < 2; ++m) {
+      f[2 * m] = Elem<T>::lo(raw[m]);
+      f[2 * m + 1] = Elem<T>::hi(raw[m]);
+    }
   }
+  static __device__ inline Row4 load(const T* p) { return {*reinterpret_cast<const u32x2_e2*>(p)}; }
+  // the first n < 4
+  static __device__ inline Row4 load_part(const T* p, int n) {
+    Row4 r{};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < n) r.raw[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+    return r;
+  }
+  static __device__ inline void store(T* p, const float (&f)[4]) {
+    *reinterpret_cast<u32x2_e2*>(p) = u32x2_e2{Elem<T>::pack2(f[0], f[1]), Elem<T>::pack2(f[2], f[3])};
+  }
+};
+template <> struct Row4<float> {
+  f32x4_any raw;
+  __device__ inline void unpack(float (&f)[4]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = raw[e];
+  }
+  static __device__ inline Row4 load(const float* p) { return {*reinterpret_cast<const f32x4_any*>(p)}; }
+  static __device__ inline Row4 load_part(const float* p, int n) {
+    Row4 r{};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < n) r.raw[e] = p[e];
+    return r;
+  }
+  static __device__ inline void store(float* p, const float (&f)[4]) {
+    *reinterpret_cast<f32x4_any*>(p) = f32x4_any{f[0], f[1], f[2], f[3]};
+  }
+};
+
+// Elements c..c+7 of a row of C; those past it are zero / not stored.  WHOLE: C is a
+// multiple of 8 (kernels whose code is large are built for both: what a launch
+// reads of it is read anew, and part chunks are most of it).
+template <bool WHOLE = false, typename T>
+__device__ inline Row8<T> load_raw8(const T* row, int c, int C) {
+  Row8<T> r{};
+  if (WHOLE ? c < C : c + 8 <= C) r = Row8<T>::load(row + c);
+  else if (!WHOLE && c < C) r = Row8<T>::load_part(row + c, C - c);
+  return r;
 }
-template <typename T>
+template <bool WHOLE = false, typename T>
+__device__ inline void load_row8(const T* row, int c, int C, float (&f)[8]) {
+  load_raw8<WHOLE>(row, c, C).unpack(f);
+}
+template <bool WHOLE = false, typename T>
 __device__ inline void store_row8(T* row, int c, int C, const float (&f)[8]) {
-  if (c + 8 <= C) {
-    Row8<T>::store(row + c, f);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c + e < C) row[c + e] = static_cast<T>(f[e]);
-  }
+  const Row8<T> r = Row8<T>::pack(f);
+  if (WHOLE ? c < C : c + 8 <= C) r.store(row + c);
+  else if (!WHOLE && c < C) r.store_part(row + c, C - c);
 }
-// The same of a vector of run-time type.
-__device__ inline void load_vec8(const void* v, int dtype, int c, int C, float (&f)[8]) {
-  if (dtype == 0) load_row8(reinterpret_cast<const float*>(v), c, C, f);
-  else if (dtype == 2) load_row8(reinterpret_cast<const __bf16*>(v), c, C, f);
-  else load_row8(reinterpret_cast<const _Float16*>(v), c, C, f);
+// N chunks of 8 elements of a vector of C, of a run-time type, at c, c + step, ...
+template <typename T, int N>
+__device__ inline void load_vec(const void* v, int c, int step, int C, float (&f)[N][8]) {
+  Row8<T> r[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) r[k] = load_raw8(reinterpret_cast<const T*>(v), c + step * k, C);
+#pragma unroll
+  for (int k = 0; k < N; ++k) r[k].unpack(f[k]);
+}
+template <int N>
+__device__ inline void load_vec(const void* v, int dtype, int c, int step, int C, float (&f)[N][8]) {
+  if (dtype == 0) load_vec<float, N>(v, c, step, C, f);
+  else if (dtype == 2) load_vec<__bf16, N>(v, c, step, C, f);
+  else load_vec<_Float16, N>(v, c, step, C, f);
 }
 __device__ inline void store_elem(void* v, int dtype, int64_t i, float x) {
   if (dtype == 0) reinterpret_cast<float*>(v)[i] = x;

@@ -115,6 +115,7 @@ def test_embed_workspace():
     assert f(-1, 9, 16) == f(3, 0, 16) == f(3, 9, 0) == f(1 << 32, 9, 16) == f(3, 1 << 31, 16) == -1
     # a second buffer and digit counts only with several tiles (and passes)
     assert f(8193, 600, 8) - f(8193, 500, 8) == (8 * 8193 + 255) // 256 * 256
+    assert f(8192, 600, 8) == f(8192, 500, 8)
 
 
 @pytest.mark.parametrize("change,code,text", [
