@@ -27,8 +27,8 @@ namespace saf {
 
 namespace {
 
-template <int TPR> constexpr int kGroups = TPR >= 256 ? 1 : 256 / TPR;
-template <int TPR> constexpr int kThreads = TPR >= 256 ? TPR : 256;
+template <int TPR> constexpr int kGroups = TPR > 64 ? 1 : 256 / TPR;  // rows of a workgroup at a time
+template <int TPR> constexpr int kThreads = TPR > 64 ? TPR : 256;
 
 // Sum over the TPR threads of a row, in a fixed order.  `slot` is LDS of the
 // reduction's own (one per sum of a row) where several waves share a row.
@@ -66,9 +66,6 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTr
   float v[NCH][8];
 #pragma unroll
   for (int k = 0; k < NCH; ++k) x[k] = load_raw8(xr, 8 * (TPR * k + t), C);
-  float w[NCH][8], b[NCH][8] = {};
-  load_vec<NCH>(p.w, p.wb_dtype, 8 * t, 8 * TPR, C, w);
-  if (p.b) load_vec<NCH>(p.b, p.wb_dtype, 8 * t, 8 * TPR, C, b);
   if (p.delta) {
     const TB* dr = reinterpret_cast<const TB*>(p.delta) + row * p.d_rs;
     TX* rr = reinterpret_cast<TX*>(p.r) + row * C;
@@ -88,6 +85,11 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTr
   }
 #pragma unroll
   for (int k = 0; k < NCH; ++k) x[k].unpack(v[k]);
+  // behind the row, which then needs no registers for its pieces any more, and ahead of
+  // the sums that hide them
+  float w[NCH][8], b[NCH][8] = {};
+  load_vec<NCH>(p.w, p.wb_dtype, 8 * t, 8 * TPR, C, w);
+  if (p.b) load_vec<NCH>(p.b, p.wb_dtype, 8 * t, 8 * TPR, C, b);
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < NCH; ++k)
@@ -241,6 +243,8 @@ hipError_t by_width(int C, A... a) {
   if (n <= 64) return F<TX, TB, 32, 2>::run(a...);
   if (n <= 96) return F<TX, TB, 32, 3>::run(a...);
   if (n <= 128) return F<TX, TB, 32, 4>::run(a...);
+  if constexpr (F<TX, TB, 64, 4>::kForward)
+    if (n <= 256) return F<TX, TB, 128, 2>::run(a...);
   if (n <= 192) return F<TX, TB, 64, 3>::run(a...);
   if (n <= 256) return F<TX, TB, 64, 4>::run(a...);
   if (n <= 512) return F<TX, TB, 256, 2>::run(a...);
@@ -251,6 +255,7 @@ hipError_t by_width(int C, A... a) {
 }
 
 template <typename TX, typename TB, int TPR, int NCH> struct Fwd {
+  static constexpr bool kForward = true;
   static hipError_t run(const LnTrainParams& p, hipStream_t s) {
     constexpr int G = kGroups<TPR>;
     hipLaunchKernelGGL((layernorm_fwd_kernel<TX, TB, TPR, NCH>), dim3((unsigned)((p.rows + G - 1) / G)), dim3(kThreads<TPR>),
@@ -259,6 +264,7 @@ template <typename TX, typename TB, int TPR, int NCH> struct Fwd {
   }
 };
 template <typename TX, typename TB, int TPR, int NCH> struct Bwd {
+  static constexpr bool kForward = false;
   static hipError_t run(const LnTrainBwdParams& p, hipStream_t s) {
     if (p.n_wg > 0)
       hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TB, TPR, NCH>), dim3((unsigned)p.n_wg), dim3(kThreads<TPR>), 0, s, p);
