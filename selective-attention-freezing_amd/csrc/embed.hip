@@ -30,7 +30,9 @@ namespace {
 constexpr int kSortThreads = 1024;
 constexpr int kWaves = kSortThreads / 64;
 constexpr int kBins = 1 << kEmbedDigit;
-constexpr uint32_t kWideUnits = 1 << 19;  // units from which a thread of the lookup has four
+// Units from which a thread of the lookup has two: 131072 tokens of 896 bf16 channels 44 us
+// against 46, 4096 the same 6.7 either way.
+constexpr uint32_t kWideUnits = 1 << 19;
 
 // U units a thread, 256 apart; their tokens are read together, then their rows.
 template <typename TW, typename TY, int U, bool WHOLE>
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const EmbedParams p) {
     const float other = tok[u] == p.ignore ? 0.f : __uint_as_float(0x7fc00000u);
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = word ? f[e] * p.scale : other;
-    store_row8<WHOLE>(reinterpret_cast<TY*>(p.y) + (int64_t)n[u] * C, c[u], C, f);
+    stream_row8<WHOLE>(reinterpret_cast<TY*>(p.y) + (int64_t)n[u] * C, c[u], C, f);
   }
 }
 
@@ -502,7 +504,7 @@ hipError_t fwd_tt(const EmbedParams& p, hipStream_t s) {
   if (p.units < kWideUnits)
     hipLaunchKernelGGL((embed_fwd_kernel<TW, TY, 1, WHOLE>), dim3((p.units + 255) / 256), dim3(256), 0, s, p);
   else
-    hipLaunchKernelGGL((embed_fwd_kernel<TW, TY, 4, WHOLE>), dim3((p.units + 1023) / 1024), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((embed_fwd_kernel<TW, TY, 2, WHOLE>), dim3((p.units + 511) / 512), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <typename TW, typename TY>

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTr
       a[k].unpack(d);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[k][e] += d[e];
-      store_row8(rr, 8 * (TPR * k + t), C, v[k]);
+      stream_row8(rr, 8 * (TPR * k + t), C, v[k]);
       x[k] = Row8<TX>::pack(v[k]);
     }
   }
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTr
   for (int k = 0; k < NCH; ++k) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[k][e] = fmaf((v[k][e] - mean) * rstd, w[k][e], b[k][e]);
-    store_row8(yr, 8 * (TPR * k + t), C, w[k]);
+    stream_row8(yr, 8 * (TPR * k + t), C, w[k]);
   }
 }
 

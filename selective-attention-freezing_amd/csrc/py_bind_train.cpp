@@ -401,7 +401,7 @@ PyObject* pack_activation(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!counted("pack_activation(x)", n, 1)) return nullptr;
   const at::Tensor& x = tensor(what, args[0]);
   same_device(what, x, x);
-  at::NoGradGuard no_grad;
+  TORCH_CHECK_NOT_IMPLEMENTED(!recorded(x), what, " has no backward: call it under torch.no_grad()");
   const c10::hip::HIPGuard guard(x.get_device());
   const Packed p = packed_like(x);
   const at::Tensor x2 = rows(x);

@@ -33,6 +33,7 @@ template <typename T> struct Row8 {
   }
   static __device__ inline Row8 load(const T* p) { return {*reinterpret_cast<const u32x4_any*>(p)}; }
   __device__ inline void store(T* p) const { *reinterpret_cast<u32x4_any*>(p) = raw; }
+  __device__ inline void stream(T* p) const { __builtin_nontemporal_store(raw, reinterpret_cast<u32x4_any*>(p)); }
   // its first n < 8 elements, the rest zero
   static __device__ inline Row8 load_part(const T* p, int n) {
     Row8 r{};
@@ -65,6 +66,10 @@ template <> struct Row8<float> {
   __device__ inline void store(float* p) const {
     *reinterpret_cast<f32x4_any*>(p) = raw[0];
     *reinterpret_cast<f32x4_any*>(p + 4) = raw[1];
+  }
+  __device__ inline void stream(float* p) const {
+    __builtin_nontemporal_store(raw[0], reinterpret_cast<f32x4_any*>(p));
+    __builtin_nontemporal_store(raw[1], reinterpret_cast<f32x4_any*>(p + 4));
   }
   static __device__ inline Row8 load_part(const float* p, int n) {
     Row8 r{};
@@ -143,6 +148,15 @@ __device__ inline void store_row8(T* row, int c, int C, const float (&f)[8]) {
   if (WHOLE ? c < C : c + 8 <= C) r.store(row + c);
   else if (!WHOLE && c < C) r.store_part(row + c, C - c);
 }
+// store_row8 of a result that this launch does not read again: past the L2, which
+// keeps it for what is read.
+template <bool WHOLE = false, typename T>
+__device__ inline void stream_row8(T* row, int c, int C, const float (&f)[8]) {
+  const Row8<T> r = Row8<T>::pack(f);
+  if (WHOLE ? c < C : c + 8 <= C) r.stream(row + c);
+  else if (!WHOLE && c < C) r.store_part(row + c, C - c);
+}
+
 // N chunks of 8 elements of a vector of C, of a run-time type, at c, c + step, ...
 template <typename T, int N>
 __device__ inline void load_vec(const void* v, int c, int step, int C, float (&f)[N][8]) {

@@ -29,8 +29,8 @@ def pack_activation(x):
     """x (..., C) in 8 bits.  For a block of 32 channels (a row's last one may be
     short) with the largest magnitude m the step is 2^(floor(log2 m) - 6), and each
     value its nearest multiple (half to even), at most 127 steps.  A block with an
-    infinity or NaN comes back as NaN.  Not differentiable: the result is what a
-    backward pass keeps."""
+    infinity or NaN comes back as NaN.  Without derivative (the result is what a
+    backward pass keeps): an x that needs a gradient is refused while grad mode is on."""
     return PackedActivation(*_ext.bind().pack_activation(x), x.dtype)
 
 

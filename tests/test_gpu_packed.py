@@ -288,6 +288,8 @@ def test_refusals():
             call(x[:, :0])
         with pytest.raises(ValueError, match="at least one channel"):
             call(x[0, 0])
+    with pytest.raises(NotImplementedError, match="no backward"):
+        kernel.pack_activation(x.clone().requires_grad_())
     p = kernel.pack_activation(x)
     for bad in (p._replace(exp=p.exp[:2]), p._replace(q=p.q.short()), p._replace(q=p.q[:, :31].contiguous(), exp=p.exp[:, :0]),
                 p._replace(q=p.q[:, ::2])):

@@ -121,6 +121,20 @@ def test_same_bits_every_time():
         assert torch.equal(runs[0][1][n], runs[1][1][n])
 
 
+def test_trainable_patterns():
+    """alpha and rho of a layer that trains them: the same gradients on both paths (the
+    bound of test_bf16_model)."""
+    import supplement
+    m = _model(dtype=BF16, bias=False)
+    supplement.enable(m)
+    idx, nxt = _batch(m)
+    a, ga = _loss_and_grads(m, lambda: m.token_logprobs(idx, nxt).logp)
+    b, gb = _loss_and_grads(m, lambda: train.token_logprobs(m, idx, nxt).logp)
+    assert sum("alpha" in n or "rho" in n for n in gb) == 4
+    assert (a - b).abs().max() <= 20 * 2.0 ** -8 * 4
+    _near(gb, ga, 20 * 2.0 ** -8 + 0.1)
+
+
 def test_modules_of_the_callers_own(monkeypatch):
     """Another MLP, or another activation, runs as it is."""
     m = _model()

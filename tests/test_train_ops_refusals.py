@@ -180,6 +180,7 @@ def test_packed_arguments(change, code, text):
     L = _ext.lib()
     a = dict(dict(x=_t((3, 40), _BF16), q=_t((3, 40), _I8), exp=_t((3, 2), _U8), y=_t((3, 40), _BF16)), **change)
     _refused(L.saf_gelu_pack_fwd(a["x"], a["y"], a["q"], a["exp"], None), code, text)
+    _refused(L.saf_act_unpack(_t((3, 40), _I8), _t((3, 2), _U8), _t((3, 40), _BF16, (39, 1)), None), _ext.SAF_EINVAL, "overlap")
     if "y" not in change:
         _refused(L.saf_act_pack(a["x"], a["q"], a["exp"], None), code, text)
         _refused(L.saf_act_unpack(a["q"], a["exp"], a["x"], None), code, text.replace("x", "out") if "2-D" in text else text)
