@@ -12,9 +12,11 @@
 // (the row stays in registers, so the second sum costs no second read).  Both
 // kernels move bytes and nothing else bounds them.
 //
-// A row belongs to TPR threads (a half wave up to 1024 channels, a wave, four
-// waves, sixteen), each with NCH chunks of 8 channels, chunk k at channel
-// 8 (TPR k + thread): every load and store of the group is one run.
+// A row belongs to TPR threads (from eight lanes for 64 channels to sixteen waves for
+// 16384), each with NCH chunks of 8 channels, chunk k at channel 8 (TPR k + thread):
+// every load and store of the group is one run.  2^25 elements take 41 us forward and
+// 62 backward in bf16, 97 and 110 in float32 (6.6 and 4.3, 5.5 and 4.9 TB/s; a copy
+// reaches 5.2), at most a third more at widths that fill the last chunks badly.
 //
 // Backward: a workgroup walks rows a grid apart and keeps its share of dw and db
 // of its threads' channels in registers; at the end it adds its waves in LDS and
@@ -34,12 +36,13 @@ template <int TPR> constexpr int kThreads = TPR > 64 ? TPR : 256;
 // reduction's own (one per sum of a row) where several waves share a row.
 template <int TPR>
 __device__ inline float row_sum(float v, float* slot) {
-  if constexpr (TPR == 32) {
+  if constexpr (TPR <= 32) {
     v = dpp_add<0xb1, 0xf>(v);
     v = dpp_add<0x4e, 0xf>(v);
-    v = dpp_add<0x141, 0xf>(v);
-    v = dpp_add<0x140, 0xf>(v);
-    return v + __shfl_xor(v, 16, 64);
+    v = dpp_add<0x141, 0xf>(v);                   // eight lanes
+    if constexpr (TPR > 8) v = dpp_add<0x140, 0xf>(v);
+    if constexpr (TPR > 16) v += __shfl_xor(v, 16, 64);
+    return v;
   } else {
     v = dpp_wave_sum(v);
     if constexpr (TPR > 64) {
@@ -190,11 +193,16 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
     for (int k = 0; k < NCH; ++k)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if constexpr (TPR == 32) {  // the wave's two rows
+#pragma unroll
+        for (int o = TPR; o < 32; o <<= 1) {  // the wave's rows
+          aw[k][e] += __shfl_xor(aw[k][e], o, 64);
+          ab[k][e] += __shfl_xor(ab[k][e], o, 64);
+        }
+        if constexpr (TPR < 64) {
           aw[k][e] = half_swap_sum(aw[k][e]);
           ab[k][e] = half_swap_sum(ab[k][e]);
         }
-        if (TPR == 64 || group % 2 == 0) part[wave][(8 * k + e) * TPR + t] = make_float2(aw[k][e], ab[k][e]);
+        if ((threadIdx.x & 63) < TPR) part[wave][(8 * k + e) * TPR + t] = make_float2(aw[k][e], ab[k][e]);
       }
     __syncthreads();
     for (int i = threadIdx.x; i < kCols; i += 256) {
@@ -235,27 +243,46 @@ __global__ __launch_bounds__(1024) void layernorm_dw_kernel(const LnTrainBwdPara
   store_elem(out, p.w_dtype, c, s);
 }
 
-// C up to 1024: a half wave a row; 2048: a wave; 8192: four waves; 16384: sixteen.
-template <template <typename, typename, int, int> class F, typename TX, typename TB, typename... A>
-hipError_t by_width(int C, A... a) {
-  const int n = (C + 7) / 8;
-  if (n <= 32) return F<TX, TB, 32, 1>::run(a...);
-  if (n <= 64) return F<TX, TB, 32, 2>::run(a...);
-  if (n <= 96) return F<TX, TB, 32, 3>::run(a...);
-  if (n <= 128) return F<TX, TB, 32, 4>::run(a...);
-  if constexpr (F<TX, TB, 64, 4>::kForward)
-    if (n <= 256) return F<TX, TB, 128, 2>::run(a...);
-  if (n <= 192) return F<TX, TB, 64, 3>::run(a...);
-  if (n <= 256) return F<TX, TB, 64, 4>::run(a...);
-  if (n <= 512) return F<TX, TB, 256, 2>::run(a...);
-  if (n <= 768) return F<TX, TB, 256, 3>::run(a...);
-  if (n <= 1024) return F<TX, TB, 256, 4>::run(a...);
-  if (n <= 2048) return F<TX, TB, 1024, 2>::run(a...);
+// Threads of a row and chunks of a thread for n chunks of 8 channels.  Forward: at
+// most two chunks a thread up to 2048 channels, more threads of a row rather than more
+// registers of a thread (2^25 float32 elements, rows of 1024: two waves' halves with
+// four chunks 116 us, a wave with two 97; rows of 2048 beside bf16 branches: a wave
+// with four 71 us, two waves with two 64).  Backward: a thread keeps dw and db of its
+// channels over the rows, and rows inside a wave need no barrier: up to four chunks.
+// Rows of 64 channels by half waves, a quarter of the lanes at work, took 106 and 189
+// us where eight lanes a row take 42 and 63.
+template <typename TX, typename TB, template <typename, typename, int, int> class F, typename P>
+hipError_t fwd_width(int n, const P& p, hipStream_t s) {
+  if (n <= 8) return F<TX, TB, 8, 1>::run(p, s);
+  if (n <= 16) return F<TX, TB, 16, 1>::run(p, s);
+  if (n <= 32) return F<TX, TB, 32, 1>::run(p, s);
+  if (n <= 64) return F<TX, TB, 64, 1>::run(p, s);
+  if (n <= 128) return F<TX, TB, 64, 2>::run(p, s);
+  if (n <= 256) return F<TX, TB, 128, 2>::run(p, s);
+  if (n <= 512) return F<TX, TB, 256, 2>::run(p, s);
+  if (n <= 768) return F<TX, TB, 256, 3>::run(p, s);
+  if (n <= 1024) return F<TX, TB, 256, 4>::run(p, s);
+  if (n <= 2048) return F<TX, TB, 1024, 2>::run(p, s);
+  return hipErrorInvalidValue;
+}
+template <typename TX, typename TB, template <typename, typename, int, int> class F, typename P>
+hipError_t bwd_width(int n, const P& p, hipStream_t s) {
+  if (n <= 8) return F<TX, TB, 8, 1>::run(p, s);
+  if (n <= 16) return F<TX, TB, 16, 1>::run(p, s);
+  if (n <= 32) return F<TX, TB, 32, 1>::run(p, s);
+  if (n <= 64) return F<TX, TB, 32, 2>::run(p, s);
+  if (n <= 96) return F<TX, TB, 32, 3>::run(p, s);
+  if (n <= 128) return F<TX, TB, 32, 4>::run(p, s);
+  if (n <= 192) return F<TX, TB, 64, 3>::run(p, s);
+  if (n <= 256) return F<TX, TB, 64, 4>::run(p, s);
+  if (n <= 512) return F<TX, TB, 256, 2>::run(p, s);
+  if (n <= 768) return F<TX, TB, 256, 3>::run(p, s);
+  if (n <= 1024) return F<TX, TB, 256, 4>::run(p, s);
+  if (n <= 2048) return F<TX, TB, 1024, 2>::run(p, s);
   return hipErrorInvalidValue;
 }
 
 template <typename TX, typename TB, int TPR, int NCH> struct Fwd {
-  static constexpr bool kForward = true;
   static hipError_t run(const LnTrainParams& p, hipStream_t s) {
     constexpr int G = kGroups<TPR>;
     hipLaunchKernelGGL((layernorm_fwd_kernel<TX, TB, TPR, NCH>), dim3((unsigned)((p.rows + G - 1) / G)), dim3(kThreads<TPR>),
@@ -264,7 +291,6 @@ template <typename TX, typename TB, int TPR, int NCH> struct Fwd {
   }
 };
 template <typename TX, typename TB, int TPR, int NCH> struct Bwd {
-  static constexpr bool kForward = false;
   static hipError_t run(const LnTrainBwdParams& p, hipStream_t s) {
     if (p.n_wg > 0)
       hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TB, TPR, NCH>), dim3((unsigned)p.n_wg), dim3(kThreads<TPR>), 0, s, p);
@@ -274,15 +300,18 @@ template <typename TX, typename TB, int TPR, int NCH> struct Bwd {
   }
 };
 
-template <template <typename, typename, int, int> class F, typename P>
+template <typename TX, typename TB>
+hipError_t run(const LnTrainParams& p, hipStream_t s) { return fwd_width<TX, TB, Fwd>((p.C + 7) / 8, p, s); }
+template <typename TX, typename TB>
+hipError_t run(const LnTrainBwdParams& p, hipStream_t s) { return bwd_width<TX, TB, Bwd>((p.C + 7) / 8, p, s); }
+
+template <typename P>
 hipError_t by_types(const P& p, int dtype, int branch, hipStream_t s) {
   if (dtype == kF32) {
-    if (branch == kF32) return by_width<F, float, float, const P&, hipStream_t>(p.C, p, s);
-    if (branch == kBF16) return by_width<F, float, __bf16, const P&, hipStream_t>(p.C, p, s);
-    return by_width<F, float, _Float16, const P&, hipStream_t>(p.C, p, s);
+    if (branch == kF32) return run<float, float>(p, s);
+    return branch == kBF16 ? run<float, __bf16>(p, s) : run<float, _Float16>(p, s);
   }
-  if (dtype == kBF16) return by_width<F, __bf16, __bf16, const P&, hipStream_t>(p.C, p, s);
-  return by_width<F, _Float16, _Float16, const P&, hipStream_t>(p.C, p, s);
+  return dtype == kBF16 ? run<__bf16, __bf16>(p, s) : run<_Float16, _Float16>(p, s);
 }
 
 }  // namespace
@@ -291,17 +320,17 @@ hipError_t by_types(const P& p, int dtype, int branch, hipStream_t s) {
 // one round of rows.
 int layernorm_bwd_groups(int64_t rows, int C, int n_cu) {
   const int n = (C + 7) / 8;
-  const int per = n <= 128 ? 8 : (n <= 256 ? 4 : 1);
+  const int per = n <= 8 ? 32 : (n <= 16 ? 16 : (n <= 128 ? 8 : (n <= 256 ? 4 : 1)));
   const int64_t rounds = (rows + per - 1) / per;
   const int64_t most = (int64_t)n_cu * (n <= 1024 ? 2 : 1);
   return (int)(rounds < most ? rounds : most);
 }
 
 hipError_t launch_layernorm_train(const LnTrainParams& p, int dtype, int branch, hipStream_t s) {
-  return by_types<Fwd>(p, dtype, branch, s);
+  return by_types(p, dtype, branch, s);
 }
 hipError_t launch_layernorm_train_bwd(const LnTrainBwdParams& p, int dtype, int branch, hipStream_t s) {
-  return by_types<Bwd>(p, dtype, branch, s);
+  return by_types(p, dtype, branch, s);
 }
 
 }  // namespace saf

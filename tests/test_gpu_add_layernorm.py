@@ -49,9 +49,9 @@ def _case(R, C, xt, yt, wt, delta=True, bias=True, seed=0):
 
 
 @pytest.mark.parametrize("xt,yt", TYPES)
-@pytest.mark.parametrize("C", [1, 7, 8, 33, 256, 257, 511, 768, 1000, 1024, 1025, 1536, 2047, 2048, 2049, 4100, 6144, 8191])
+@pytest.mark.parametrize("C", [1, 7, 8, 33, 64, 65, 128, 129, 256, 257, 511, 768, 1000, 1024, 1025, 1536, 2047, 2048, 2049, 4100, 6144, 8191])
 def test_widths_and_types(xt, yt, C):
-    """Every layout of a row: half a wave with 1 to 4 chunks, a wave, four waves."""
+    """Every layout of a row: eight lanes to four waves, 1 to 4 chunks a thread."""
     c = _case(37, C, xt, yt, yt if C % 2 else F32, delta=C % 3 != 0, bias=C % 4 != 0, seed=C)
     _check(**c, dtype=yt)
 
@@ -63,7 +63,7 @@ def test_widest(xt, yt, C):
 
 
 @pytest.mark.parametrize("R", [1, 2, 7, 8, 9, 4095, 4096, 5001])
-@pytest.mark.parametrize("C", [64, 1280, 2100])
+@pytest.mark.parametrize("C", [40, 100, 64, 1280, 2100])
 def test_rows(R, C):
     """Fewer rows than workgroups, and more: ragged last rounds."""
     _check(**_case(R, C, BF16, BF16, BF16, seed=R))
