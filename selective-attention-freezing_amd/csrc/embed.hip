@@ -11,9 +11,10 @@
 // 1. The positions n are sorted by token, stable, least significant digit first
 //    (9 bits at most a pass), while the other workgroups of the same launches
 //    clear dW: the sort takes no time of its own as long as it is the shorter.
-//    Up to kEmbedOnce tokens one workgroup sorts in LDS in one launch; more go tile
-//    by tile, each pass a launch that counts the digits of every tile and one that
-//    places every tile's keys.
+//    Up to kEmbedOnce tokens one workgroup sorts in LDS in one launch.  More go tile
+//    by tile, a launch a pass that places every tile's keys; each workgroup counts the
+//    digits of all keys for itself, from kEmbedCounted tokens on a launch before it
+//    counts them once.
 // 2. The sorted positions are cut into chunks; a wave sums 256 channels over a chunk
 //    and writes the rows whose tokens lie inside it.  A token that crosses chunks
 //    leaves float32 partial sums,
@@ -233,24 +234,24 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const EmbedBwd
   }
 }
 
-// Keys and positions of a tile, from the tokens in the first pass.
+// Keys and positions at(0), at(1), ..., from the tokens in the first pass.
 constexpr int kKeys = kEmbedTile / kSortThreads;
-template <typename At>
-__device__ inline void tile_keys(const EmbedBwdParams& p, const uint2* from, At at, uint32_t (&key)[kKeys],
-                                 uint32_t (&pos)[kKeys]) {
+template <int KEYS, typename At>
+__device__ inline void tile_keys(const EmbedBwdParams& p, const uint2* from, At at, uint32_t (&key)[KEYS],
+                                 uint32_t (&pos)[KEYS]) {
   if (from) {
-    uint2 k[kKeys];
+    uint2 k[KEYS];
 #pragma unroll
-    for (int i = 0; i < kKeys; ++i) k[i] = at(i) < p.N ? from[at(i)] : make_uint2(0, 0);
+    for (int i = 0; i < KEYS; ++i) k[i] = at(i) < p.N ? from[at(i)] : make_uint2(0, 0);
 #pragma unroll
-    for (int i = 0; i < kKeys; ++i) {
+    for (int i = 0; i < KEYS; ++i) {
       key[i] = k[i].x;
       pos[i] = k[i].y;
     }
   } else {
     keys_of(p, p.N, at, key);
 #pragma unroll
-    for (int i = 0; i < kKeys; ++i) pos[i] = (uint32_t)at(i);
+    for (int i = 0; i < KEYS; ++i) pos[i] = (uint32_t)at(i);
   }
 }
 
@@ -279,7 +280,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_count_kernel(const EmbedBw
 __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(const EmbedBwdParams p, const uint2* from, uint2* to,
                                                                    int shift, int64_t lo, int64_t hi) {
   __shared__ Counts counts;
-  __shared__ uint32_t sums[2][kWaves], base[kBins];
+  __shared__ uint32_t sums[2][kWaves], part[2][kBins], base[kBins];
   if ((int)blockIdx.x >= p.n_tiles) {
     clear_part(p, lo, hi, blockIdx.x - p.n_tiles, gridDim.x - p.n_tiles);
     return;
@@ -297,9 +298,25 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(const EmbedBw
   // of each digit: the keys in the tiles before, and in all
   const int d = threadIdx.x;
   uint32_t before = 0, all = 0;
-  if (d < kBins) {
+  if (p.counts == nullptr) {
+    for (int b = d; b < 2 * kBins; b += kSortThreads) (&part[0][0])[b] = 0;
+    __syncthreads();
+    for (int64_t first = 0; first < p.N; first += 8 * kSortThreads) {
+      const auto any = [&](int i) { return first + i * kSortThreads + threadIdx.x; };
+      uint32_t other[8], unused[8];
+      tile_keys(p, from, any, other, unused);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (any(i) < p.N) atomicAdd(&part[any(i) < n0][other[i] >> shift & mask], 1u);
+    }
+    __syncthreads();
+    if (d < kBins) {
+      before = part[1][d];
+      all = before + part[0][d];
+    }
+  } else if (d < kBins) {
     const uint32_t* of = p.counts + d;
-#pragma unroll 8
+#pragma unroll 16
     for (int t = 0; t < p.n_tiles; ++t) {
       const uint32_t n = of[(int64_t)t * kBins];
       before += t < (int)blockIdx.x ? n : 0;
@@ -470,22 +487,22 @@ hipError_t bwd_t(const EmbedBwdParams& p, int dtype, hipStream_t s) {
   if (p.N <= kEmbedOnce) {
     hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)(1 + p.n_clear)), sort_wg, 0, s, p);
   } else {
-    // an equal part of the zeros beside each of the 2 x passes launches; the
-    // pass that comes last writes `sorted`
-    const int64_t step = (p.dw_bytes / (2 * p.passes) + 15) / 16 * 16;
+    // an equal part of the zeros beside each of the launches; the pass that comes
+    // last writes `sorted`
+    const int launches = (p.counts ? 2 : 1) * p.passes;
+    const int64_t step = (p.dw_bytes / launches + 15) / 16 * 16;
     const uint2* from = nullptr;
-    for (int i = 0; i < p.passes; ++i) {
-      uint2* to = (p.passes - 1 - i) & 1 ? p.sorted2 : p.sorted;
-      for (int half = 0; half < 2; ++half) {
-        const int64_t lo = (2 * i + half) * step;
-        int64_t hi = 2 * i + half == 2 * p.passes - 1 ? p.dw_bytes : lo + step;
-        if (hi > p.dw_bytes) hi = p.dw_bytes;
-        const dim3 grid((unsigned)(p.n_tiles + (lo < hi ? p.n_clear : 0)));
-        if (half == 0)
-          hipLaunchKernelGGL(embed_count_kernel, grid, sort_wg, 0, s, p, from, i * p.bits, lo, hi);
-        else
-          hipLaunchKernelGGL(embed_place_kernel, grid, sort_wg, 0, s, p, from, to, i * p.bits, lo, hi);
+    for (int i = 0; i < launches; ++i) {
+      const int64_t lo = i * step < p.dw_bytes ? i * step : p.dw_bytes;
+      const int64_t hi = i + 1 < launches && lo + step < p.dw_bytes ? lo + step : p.dw_bytes;
+      const dim3 grid((unsigned)(p.n_tiles + (lo < hi ? p.n_clear : 0)));
+      const int pass = p.counts ? i / 2 : i;
+      if (p.counts && i % 2 == 0) {
+        hipLaunchKernelGGL(embed_count_kernel, grid, sort_wg, 0, s, p, from, pass * p.bits, lo, hi);
+        continue;
       }
+      uint2* to = (p.passes - 1 - pass) & 1 ? p.sorted2 : p.sorted;
+      hipLaunchKernelGGL(embed_place_kernel, grid, sort_wg, 0, s, p, from, to, pass * p.bits, lo, hi);
       from = to;
     }
   }

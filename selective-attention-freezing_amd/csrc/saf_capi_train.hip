@@ -111,7 +111,7 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int64_t C) {
   e.at_sorted2 = at;
   if (N > kEmbedOnce && e.passes > 1) at += up256(8 * N);
   e.at_counts = at;
-  if (N > kEmbedOnce) at += up256(4 * ((int64_t)e.n_tiles << kEmbedDigit));
+  if (N >= kEmbedCounted) at += up256(4 * ((int64_t)e.n_tiles << kEmbedDigit));
   e.at_head = at;
   if (e.n_chunks > 1) at += up256(4 * e.n_chunks * C);
   e.at_tail = at;
@@ -219,7 +219,7 @@ int saf_embed_bwd(const saf_tensor_t* tokens, const saf_tensor_t* dout, float sc
   p.C = (int)C;
   p.sorted = reinterpret_cast<uint2*>(ws);
   p.sorted2 = reinterpret_cast<uint2*>(ws + e.at_sorted2);
-  p.counts = reinterpret_cast<uint32_t*>(ws + e.at_counts);
+  p.counts = N >= kEmbedCounted ? reinterpret_cast<uint32_t*>(ws + e.at_counts) : nullptr;
   p.head = reinterpret_cast<float*>(ws + e.at_head);
   p.tail = reinterpret_cast<float*>(ws + e.at_tail);
   p.n_tiles = e.n_tiles;

@@ -386,11 +386,13 @@ enum class ActPackOp { kPack, kUnpack, kGelu, kGeluBwd };
 
 // Embedding lookup and gradient (embed.hip); a unit is 8 channels of a token, in the
 // backward pass 256 channels of a chunk of at most 64 sorted positions.
-// Tokens that one workgroup sorts by itself (25 us for 8192 in two passes, against 29
-// us and three more launches by tiles; 44 us against 29 for 16384), and a workgroup's
-// part of more.
+// Tokens that one workgroup sorts by itself (8192 in two passes: 25 us, one launch;
+// by tiles 24 in two, 44 against 29 for 16384), a workgroup's part of more, and the
+// number from which their digits are counted once in launches of their own (16384: 29
+// us in two launches, 29 in four; 32768: 37 and 30).
 constexpr int kEmbedOnce = 8192;
 constexpr int kEmbedTile = 2048;
+constexpr int kEmbedCounted = 16385;
 constexpr int kEmbedDigit = 9;    // bits of a sorting pass at most
 struct EmbedParams {
   const void* tokens;
@@ -418,7 +420,7 @@ struct EmbedBwdParams {
   int C;
   uint2* sorted;    // (N) token, position
   uint2* sorted2;   // (N) with more than kEmbedOnce tokens and one pass
-  uint32_t* counts; // (n_tiles, 2^kEmbedDigit) with more than kEmbedOnce tokens
+  uint32_t* counts; // (n_tiles, 2^kEmbedDigit) from kEmbedCounted tokens on, else null
   float* head;      // (chunks, C) sums of a chunk's first word where that began before it
   float* tail;      // (chunks, C) sums of its last word where that goes on
   int n_tiles, n_clear, passes, bits, chunk;
