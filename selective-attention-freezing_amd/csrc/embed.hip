@@ -14,7 +14,7 @@
 //    Up to kEmbedOnce tokens one workgroup sorts in LDS in one launch.  More go tile
 //    by tile, a launch a pass that places every tile's keys; each workgroup counts the
 //    digits of all keys for itself, from kEmbedCounted tokens on a launch before it
-//    counts them once.
+//    counts them once, and past kEmbedScanned tiles another sums the counts up.
 // 2. The sorted positions are cut into chunks; a wave sums 256 channels over a chunk
 //    and writes the rows whose tokens lie inside it.  A token that crosses chunks
 //    leaves float32 partial sums,
@@ -150,7 +150,7 @@ __device__ inline void places(Counts& counts, uint32_t* sums) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) n[w] = counts[w][d];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) all += n[w];  // either half is 16384 at most: no carry
+    for (int w = 0; w < kWaves; ++w) all += n[w];  // either half is kEmbedOnce at most: no carry
   }
   const uint32_t both = (all & 0xffff) + (all >> 16);
   const uint32_t low = running_sum(both, sums) - both;
@@ -280,6 +280,30 @@ __global__ __launch_bounds__(kSortThreads) void embed_count_kernel(const EmbedBw
   for (int b = threadIdx.x; b < kBins; b += kSortThreads) p.counts[(int64_t)blockIdx.x * kBins + b] = count[b];
 }
 
+// Counts of very many tiles summed up, once: a tile's become those of the tiles before
+// it, the row behind the last the totals.  Workgroups of 64 digits, each of their waves
+// with a run of tiles.
+__global__ __launch_bounds__(1024) void embed_scan_kernel(const EmbedBwdParams p) {
+  __shared__ uint32_t sums[16][64];
+  const int col = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t* of = p.counts + blockIdx.x * 64 + col;
+  const int run = (p.n_tiles + 15) / 16, lo = wave * run, hi = lo + run < p.n_tiles ? lo + run : p.n_tiles;
+  uint32_t s = 0;
+#pragma unroll 16
+  for (int t = lo; t < hi; ++t) s += of[(int64_t)t * kBins];
+  sums[wave][col] = s;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < wave; ++w) before += sums[w][col];
+#pragma unroll 16
+  for (int t = lo; t < hi; ++t) {
+    const uint32_t n = of[(int64_t)t * kBins];
+    of[(int64_t)t * kBins] = before;
+    before += n;
+  }
+  if (wave == 15) of[(int64_t)p.n_tiles * kBins] = before;
+}
+
 // Every tile's keys to their places of this pass.
 __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(const EmbedBwdParams p, const uint2* from, uint2* to,
                                                                    int shift, int64_t lo, int64_t hi) {
@@ -318,6 +342,9 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(const EmbedBw
       before = part[1][d];
       all = before + part[0][d];
     }
+  } else if (d < kBins && p.n_tiles > kEmbedScanned) {
+    before = p.counts[(int64_t)blockIdx.x * kBins + d];
+    all = p.counts[(int64_t)p.n_tiles * kBins + d];
   } else if (d < kBins) {
     const uint32_t* of = p.counts + d;
 #pragma unroll 16
@@ -479,6 +506,18 @@ void sum(const EmbedBwdParams& p, hipStream_t s) {
   if (p.C % 4 == 0) hipLaunchKernelGGL((embed_sum_kernel<TW, TY, true>), grid, wg, 0, s, p);
   else hipLaunchKernelGGL((embed_sum_kernel<TW, TY, false>), grid, wg, 0, s, p);
 }
+// bf16 and fp16 do not meet (the C entry refuses them).
+template <typename TW>
+void sum(const EmbedBwdParams& p, int dtype, hipStream_t s) {
+  if constexpr (sizeof(TW) == 4) {
+    if (dtype == kF32) sum<float, float>(p, s);
+    else if (dtype == kBF16) sum<float, __bf16>(p, s);
+    else sum<float, _Float16>(p, s);
+  } else {
+    if (dtype == kF32) sum<TW, float>(p, s);
+    else sum<TW, TW>(p, s);
+  }
+}
 
 template <typename TW>
 hipError_t bwd_t(const EmbedBwdParams& p, int dtype, hipStream_t s) {
@@ -503,6 +542,7 @@ hipError_t bwd_t(const EmbedBwdParams& p, int dtype, hipStream_t s) {
       const int pass = p.counts ? i / 2 : i;
       if (p.counts && i % 2 == 0) {
         hipLaunchKernelGGL(embed_count_kernel, grid, sort_wg, 0, s, p, from, pass * p.bits, lo, hi);
+        if (p.n_tiles > kEmbedScanned) hipLaunchKernelGGL(embed_scan_kernel, dim3(kBins / 64), sort_wg, 0, s, p);
         continue;
       }
       uint2* to = (p.passes - 1 - pass) & 1 ? p.sorted2 : p.sorted;
@@ -510,9 +550,7 @@ hipError_t bwd_t(const EmbedBwdParams& p, int dtype, hipStream_t s) {
       from = to;
     }
   }
-  if (dtype == kF32) sum<TW, float>(p, s);
-  else if (dtype == kBF16) sum<TW, __bf16>(p, s);
-  else sum<TW, _Float16>(p, s);
+  sum<TW>(p, dtype, s);
   const int64_t n_chunks = (p.N + p.chunk - 1) / p.chunk;
   if (n_chunks > 1)
     hipLaunchKernelGGL((embed_join_kernel<TW>), dim3((unsigned)(n_chunks - 1), (unsigned)((p.C + 255) / 256)), dim3(32 * kLanes),
@@ -534,9 +572,12 @@ hipError_t fwd_tt(const EmbedParams& p, hipStream_t s) {
 }
 template <typename TW>
 hipError_t fwd_t(const EmbedParams& p, int dtype, hipStream_t s) {
-  if (dtype == kF32) return fwd_tt<TW, float>(p, s);
-  if (dtype == kBF16) return fwd_tt<TW, __bf16>(p, s);
-  return fwd_tt<TW, _Float16>(p, s);
+  if constexpr (sizeof(TW) == 4) {
+    if (dtype == kF32) return fwd_tt<float, float>(p, s);
+    return dtype == kBF16 ? fwd_tt<float, __bf16>(p, s) : fwd_tt<float, _Float16>(p, s);
+  } else {
+    return dtype == kF32 ? fwd_tt<TW, float>(p, s) : fwd_tt<TW, TW>(p, s);
+  }
 }
 
 }  // namespace

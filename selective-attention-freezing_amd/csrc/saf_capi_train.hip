@@ -111,7 +111,7 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int64_t C) {
   e.at_sorted2 = at;
   if (N > kEmbedOnce && e.passes > 1) at += up256(8 * N);
   e.at_counts = at;
-  if (N >= kEmbedCounted) at += up256(4 * ((int64_t)e.n_tiles << kEmbedDigit));
+  if (N >= kEmbedCounted) at += up256(4 * ((int64_t)(e.n_tiles + 1) << kEmbedDigit));
   e.at_head = at;
   if (e.n_chunks > 1) at += up256(4 * e.n_chunks * C);
   e.at_tail = at;

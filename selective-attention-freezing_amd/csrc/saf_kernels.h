@@ -393,6 +393,9 @@ enum class ActPackOp { kPack, kUnpack, kGelu, kGeluBwd };
 constexpr int kEmbedOnce = 8192;
 constexpr int kEmbedTile = 2048;
 constexpr int kEmbedCounted = 16385;
+// Tiles up to which every workgroup adds the counts of all tiles for itself (a pass over
+// 262144 tokens places them in 12.5 us so, in 7.6 behind a sum of 6; 1048576: 47, 14.5 and 6).
+constexpr int kEmbedScanned = 128;
 constexpr int kEmbedDigit = 9;    // bits of a sorting pass at most
 struct EmbedParams {
   const void* tokens;
@@ -420,7 +423,7 @@ struct EmbedBwdParams {
   int C;
   uint2* sorted;    // (N) token, position
   uint2* sorted2;   // (N) with more than kEmbedOnce tokens and one pass
-  uint32_t* counts; // (n_tiles, 2^kEmbedDigit) from kEmbedCounted tokens on, else null
+  uint32_t* counts; // (n_tiles + 1, 2^kEmbedDigit) from kEmbedCounted tokens on, else null
   float* head;      // (chunks, C) sums of a chunk's first word where that began before it
   float* tail;      // (chunks, C) sums of its last word where that goes on
   int n_tiles, n_clear, passes, bits, chunk;

@@ -75,6 +75,16 @@ def test_many_tokens():
     _check(t, rnd(1000, 24, seed=7), rnd(200003, 24, seed=8, dtype=F32), 1.0)
 
 
+@pytest.mark.parametrize("V", [300, 70000])
+def test_very_many_tokens(V):
+    """More tiles than a workgroup adds up by itself; an odd number of them."""
+    N = 2048 * 150 + 77
+    t = _tokens(N, V, 8, skew=5.0)
+    t[::5] = 3
+    t[1::50] = -100
+    _check(t, rnd(V, 3, seed=7), rnd(N, 3, seed=8, dtype=F32), 1.0)
+
+
 @pytest.mark.parametrize("tt", [torch.long, torch.int32])
 def test_tokens_out_of_range(tt):
     t = _tokens(100, 50, 9, dtype=tt)
