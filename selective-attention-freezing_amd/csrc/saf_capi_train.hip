@@ -92,6 +92,7 @@ struct EmbedPlan {
 // 16384 tokens of a natural distribution at 768 channels, 25 and 20 for 32768, 35 and
 // 31 for 65536.
 int chunk_of(int64_t N, int64_t C) {
+  if (N <= 64) return 64;  // one chunk: no parts to join, a launch less
   const int64_t waves = (N + 63) / 64 * ((C + 255) / 256);
   return waves >= 1024 ? 64 : (waves >= 512 ? 32 : 16);
 }

@@ -111,7 +111,7 @@ def test_embed_bwd_arguments(change, code, text):
 def test_embed_workspace():
     f = _ext.lib().saf_embed_bwd_workspace_bytes
     assert f(0, 9, 16) == 0
-    assert f(3, 9, 16) == 256                        # one chunk: the sorted positions alone
+    assert f(3, 9, 16) == 256 and f(64, 9, 16) == 512   # one chunk: the sorted positions alone
     assert f(-1, 9, 16) == f(3, 0, 16) == f(3, 9, 0) == f(1 << 32, 9, 16) == f(3, 1 << 31, 16) == -1
     # a second buffer and digit counts only with several tiles (and passes)
     assert f(8193, 600, 8) - f(8193, 500, 8) == (8 * 8193 + 255) // 256 * 256
