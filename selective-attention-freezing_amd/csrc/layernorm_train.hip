@@ -15,8 +15,13 @@
 // A row belongs to TPR threads (from eight lanes for 64 channels to sixteen waves for
 // 16384), each with NCH chunks of 8 channels, chunk k at channel 8 (TPR k + thread):
 // every load and store of the group is one run.  2^25 elements take 41 us forward and
-// 62 backward in bf16, 97 and 110 in float32 (6.6 and 4.3, 5.5 and 4.9 TB/s; a copy
+// 50 backward in bf16, 97 and 95 in float32 (6.6 and 5.4, 5.5 and 5.6 TB/s; a copy
 // reaches 5.2), at most a third more at widths that fill the last chunks badly.
+//
+// What nothing reads again goes past the caches: dy and dr (8192 x 2048, float32
+// beside bf16, both directions: 105 us through them, 99 past them), r and y (44 and 41
+// forward; a training step is the same either way).  delta so read costs rows that fit
+// the caches more than it gives (bf16 forward: 41 us, 48).
 //
 // Backward: a workgroup walks rows a grid apart and keeps its share of dw and db
 // of its threads' channels in registers; at the end it adds its waves in LDS and
@@ -142,11 +147,11 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
 #pragma unroll
     for (int k = 0; k < NCH; ++k) r[k] = load_raw8(rr, 8 * (TPR * k + t), C);
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) dy[k] = load_raw8(gr, 8 * (TPR * k + t), C);
+    for (int k = 0; k < NCH; ++k) dy[k] = once_raw8(gr, 8 * (TPR * k + t), C);
     const TX* er = reinterpret_cast<const TX*>(p.dr) + row * p.dr_rs;
     if (kTogether && p.dr) {
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) add[k] = load_raw8(er, 8 * (TPR * k + t), C);
+      for (int k = 0; k < NCH; ++k) add[k] = once_raw8(er, 8 * (TPR * k + t), C);
     }
     float xh[NCH][8], g[NCH][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -176,7 +181,7 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
       if (c >= C) continue;
       float d[8] = {};
       if (p.dr) {
-        if constexpr (!kTogether) add[k] = load_raw8(er, c, C);
+        if constexpr (!kTogether) add[k] = once_raw8(er, c, C);
         add[k].unpack(d);
       }
 #pragma unroll

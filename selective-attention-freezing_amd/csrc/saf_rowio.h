@@ -32,6 +32,9 @@ template <typename T> struct Row8 {
     return r;
   }
   static __device__ inline Row8 load(const T* p) { return {*reinterpret_cast<const u32x4_any*>(p)}; }
+  static __device__ inline Row8 load_once(const T* p) {
+    return {__builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p))};
+  }
   __device__ inline void store(T* p) const { *reinterpret_cast<u32x4_any*>(p) = raw; }
   __device__ inline void stream(T* p) const { __builtin_nontemporal_store(raw, reinterpret_cast<u32x4_any*>(p)); }
   // its first n < 8 elements, the rest zero
@@ -62,6 +65,10 @@ template <> struct Row8<float> {
   }
   static __device__ inline Row8 load(const float* p) {
     return {{*reinterpret_cast<const f32x4_any*>(p), *reinterpret_cast<const f32x4_any*>(p + 4)}};
+  }
+  static __device__ inline Row8 load_once(const float* p) {
+    return {{__builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(p)),
+             __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(p + 4))}};
   }
   __device__ inline void store(float* p) const {
     *reinterpret_cast<f32x4_any*>(p) = raw[0];
@@ -136,6 +143,14 @@ __device__ inline Row8<T> load_raw8(const T* row, int c, int C) {
   Row8<T> r{};
   if (WHOLE ? c < C : c + 8 <= C) r = Row8<T>::load(row + c);
   else if (!WHOLE && c < C) r = Row8<T>::load_part(row + c, C - c);
+  return r;
+}
+// The same of a row that nothing reads again soon: it takes no other's place in the caches.
+template <typename T>
+__device__ inline Row8<T> once_raw8(const T* row, int c, int C) {
+  Row8<T> r{};
+  if (c + 8 <= C) r = Row8<T>::load_once(row + c);
+  else if (c < C) r = Row8<T>::load_part(row + c, C - c);
   return r;
 }
 template <bool WHOLE = false, typename T>
