@@ -21,7 +21,8 @@
 // What nothing reads again goes past the caches: dy and dr (8192 x 2048, float32
 // beside bf16, both directions: 105 us through them, 99 past them), r and y (44 and 41
 // forward; a training step is the same either way).  delta so read costs rows that fit
-// the caches more than it gives (bf16 forward: 41 us, 48).
+// the caches more than it gives (bf16 forward: 41 us, 48), and so do dy and dr whose
+// pieces cross lines, which are then fetched twice (rows of 2047: 76 and 91).
 //
 // Backward: a workgroup walks rows a grid apart and keeps its share of dw and db
 // of its threads' channels in registers; at the end it adds its waves in LDS and
@@ -146,12 +147,22 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
     Row8<TB> dy[NCH];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) r[k] = load_raw8(rr, 8 * (TPR * k + t), C);
+    if (p.once) {
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) dy[k] = once_raw8(gr, 8 * (TPR * k + t), C);
+      for (int k = 0; k < NCH; ++k) dy[k] = once_raw8(gr, 8 * (TPR * k + t), C);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) dy[k] = load_raw8(gr, 8 * (TPR * k + t), C);
+    }
     const TX* er = reinterpret_cast<const TX*>(p.dr) + row * p.dr_rs;
     if (kTogether && p.dr) {
+      if (p.once) {
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) add[k] = once_raw8(er, 8 * (TPR * k + t), C);
+        for (int k = 0; k < NCH; ++k) add[k] = once_raw8(er, 8 * (TPR * k + t), C);
+      } else {
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) add[k] = load_raw8(er, 8 * (TPR * k + t), C);
+      }
     }
     float xh[NCH][8], g[NCH][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -181,7 +192,7 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
       if (c >= C) continue;
       float d[8] = {};
       if (p.dr) {
-        if constexpr (!kTogether) add[k] = once_raw8(er, c, C);
+        if constexpr (!kTogether) add[k] = load_raw8(er, c, C);
         add[k].unpack(d);
       }
 #pragma unroll

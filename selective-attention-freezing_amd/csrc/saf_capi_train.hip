@@ -336,6 +336,10 @@ int saf_layernorm_bwd(const saf_tensor_t* r, const saf_tensor_t* stats, const sa
     p.dr = dr->data;
     p.dr_rs = dr->stride[0];
   }
+  auto al16 = [](const saf_tensor_t& t) {
+    return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && (t.size[0] <= 1 || t.stride[0] * elem_size(t.dtype) % 16 == 0);
+  };
+  p.once = al16(*dy) && (!given(dr) || al16(*dr));
   p.dx = given(dx) ? dx->data : nullptr;
   p.ddelta = given(ddelta) ? ddelta->data : nullptr;
   p.w = weight->data;

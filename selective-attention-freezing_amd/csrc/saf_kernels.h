@@ -364,6 +364,7 @@ struct LnTrainBwdParams {
   float* part;        // (n_wg, 2, C); null: neither dw nor db
   int64_t rows, r_rs, dy_rs, dr_rs;
   int C, w_dtype, n_wg;
+  int once;           // dy's and dr's rows are 16-byte aligned
 };
 constexpr int kLnMaxC = 16384;
 int layernorm_bwd_groups(int64_t rows, int C, int n_cu);
