@@ -480,7 +480,8 @@ int saf_embed_fwd(const saf_tensor_t* tokens, const saf_tensor_t* weight, float 
 
 /* Gradient of saf_embed_fwd: dweight[v] = scale sum of dout[n] over the n with
  * tokens[n] = v, added in the order of n; every row of dweight (V, C) is written,
- * 16-byte aligned.  The workspace (256-byte aligned) is that of N tokens, V and C. */
+ * 16-byte aligned.  The workspace (256-byte aligned) is that of N tokens (at most 2^28), V
+ * and C. */
 int saf_embed_bwd(const saf_tensor_t* tokens, const saf_tensor_t* dout, float scale, int64_t ignore_index,
                   const saf_tensor_t* dweight, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t saf_embed_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t channels);

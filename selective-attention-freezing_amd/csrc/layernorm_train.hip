@@ -332,6 +332,12 @@ hipError_t by_types(const P& p, int dtype, int branch, hipStream_t s) {
 
 }  // namespace
 
+// Threads of a row in the forward pass (fwd_width).
+int layernorm_row_threads(int C) {
+  const int n = (C + 7) / 8;
+  return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : n <= 128 ? 64 : n <= 256 ? 128 : n <= 1024 ? 256 : 1024;
+}
+
 // Workgroups of the backward pass: as many as are resident, each with at least
 // one round of rows.
 int layernorm_bwd_groups(int64_t rows, int C, int n_cu) {

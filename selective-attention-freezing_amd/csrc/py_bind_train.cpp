@@ -146,7 +146,7 @@ struct EmbedTokens : public torch::autograd::Function<EmbedTokens> {
       const int64_t V = ctx->saved_data["V"].toInt(), C = g.size(1);
       dw = at::empty({V, C}, plain(g).dtype((at::ScalarType)ctx->saved_data["type"].toInt()));
       const int64_t bytes = lib.embed_bytes(t.numel(), V, C);
-      if (bytes < 0) check(SAF_EINVAL);
+      if (bytes < 0) check(SAF_EUNSUPPORTED);
       const at::Tensor ws = workspace(bytes, g);
       const saf_tensor_t td = desc(kEmbed, t), gd = rows_desc(kEmbed, g), dd = rows_desc(kEmbed, dw);
       check(lib.embed_bwd(&td, &gd, (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["ignore"].toInt(), &dd,

@@ -11,6 +11,8 @@ namespace {
 
 constexpr int64_t kMaxUnits = 0x7fffffff;
 constexpr int64_t kMaxC = int64_t(1) << 23;
+constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1024;  // of a launch, whose workgroups have 1024 at most
+constexpr int64_t kMaxTokens = int64_t(1) << 28;             // of an embedding's gradient
 
 bool float_dtype(int d) { return d == SAF_F32 || d == SAF_F16 || d == SAF_BF16; }
 bool given(const saf_tensor_t* t) { return t != nullptr && t->ndim > 0; }
@@ -180,8 +182,8 @@ int saf_embed_fwd(const saf_tensor_t* tokens, const saf_tensor_t* weight, float 
 }
 
 int64_t saf_embed_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t channels) {
-  if (n_tokens < 0 || n_tokens > kMaxUnits) {
-    fail(SAF_EINVAL, "embed: %lld tokens", (long long)n_tokens);
+  if (n_tokens < 0 || n_tokens > kMaxTokens) {
+    fail(SAF_EUNSUPPORTED, "embed_bwd: %lld tokens (at most 2^28)", (long long)n_tokens);
     return -1;
   }
   if (check_table(vocab, channels) != SAF_OK) return -1;
@@ -196,7 +198,7 @@ int saf_embed_bwd(const saf_tensor_t* tokens, const saf_tensor_t* dout, float sc
   if (dweight->ndim != 2) return fail(SAF_EINVAL, "dweight must be (V, C)");
   const int64_t N = tokens->size[0], V = dweight->size[0], C = dweight->size[1];
   if (int rc = check_table(V, C)) return rc;
-  if (N > kMaxUnits) return fail(SAF_EUNSUPPORTED, "embed: more than 2^31 tokens");
+  if (N > kMaxTokens) return fail(SAF_EUNSUPPORTED, "embed_bwd: %lld tokens (at most 2^28)", (long long)N);
   if (int rc = check_rows(dweight, "dweight", V, C, true)) return rc;
   if (reinterpret_cast<uintptr_t>(dweight->data) % 16 != 0) return fail(SAF_EALIGN, "dweight must be 16-byte aligned");
   if (int rc = check_rows(dout, "dout", N, C, false)) return rc;
@@ -204,6 +206,7 @@ int saf_embed_bwd(const saf_tensor_t* tokens, const saf_tensor_t* dout, float sc
   const EmbedPlan e = embed_plan(N, V, C);
   EmbedBwdParams p{};
   if (int rc = units_of("embed", e.n_chunks, (C + 255) / 256, p.per_row, p.units)) return rc;
+  if (p.units > kMaxThreads / 64) return fail(SAF_EUNSUPPORTED, "embed_bwd: too many tokens of %lld channels", (long long)C);
   if (int rc = check_workspace("embed_bwd", workspace, workspace_bytes, e.bytes)) return rc;
   char* ws = reinterpret_cast<char*>(workspace);
   p.tokens = tokens->data;
@@ -241,7 +244,8 @@ int saf_layernorm_fwd(const saf_tensor_t* x, const saf_tensor_t* delta, const sa
   if (x->ndim != 2) return fail(SAF_EINVAL, "x must be 2-D (rows, C)");
   const int64_t R = x->size[0], C = x->size[1];
   if (C < 1 || C > kLnMaxC) return fail(SAF_EUNSUPPORTED, "layernorm: C = %lld is not supported (1 to %d)", (long long)C, kLnMaxC);
-  if (R > kMaxUnits) return fail(SAF_EUNSUPPORTED, "layernorm: more than 2^31 rows");
+  if (R > kMaxThreads / layernorm_row_threads((int)C))
+    return fail(SAF_EUNSUPPORTED, "layernorm: too many rows (%lld) of %lld channels", (long long)R, (long long)C);
   if (int rc = check_rows(x, "x", R, C, false)) return rc;
   if (int rc = check_rows(y, "y", R, C, true)) return rc;
   if (y->dtype != x->dtype && x->dtype != SAF_F32)

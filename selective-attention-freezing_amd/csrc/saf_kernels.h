@@ -367,6 +367,7 @@ struct LnTrainBwdParams {
   int once;           // dy's and dr's rows are 16-byte aligned
 };
 constexpr int kLnMaxC = 16384;
+int layernorm_row_threads(int C);
 int layernorm_bwd_groups(int64_t rows, int C, int n_cu);
 
 // Activations in 8 bits (act_pack.hip).  q and exp are contiguous; a unit is 8

@@ -244,6 +244,29 @@ def test_mlp_parts():
     assert torch.equal(kernel.mlp_packed(*args), y.detach())
 
 
+def test_mlp_shapes():
+    """One row without a leading dimension, no rows at all, weights of other strides."""
+    x, ws, bs, gy = _mlp_case(F32, (20,), 32, 64, 32, True)
+    leaves = [t.detach().requires_grad_() for t in (x[0], *ws, *bs)]
+    y = kernel.mlp_packed(*leaves)
+    rows = [t.detach().requires_grad_() for t in (x[:1], *ws, *bs)]
+    want = kernel.mlp_packed(*rows)
+    assert y.shape == (32,)
+    tol = 64 * U * 32                                         # two library products of 64 terms of magnitude up to 4
+    close(y.detach(), want.detach()[0], tol)
+    for a, b in zip(torch.autograd.grad(y, leaves, gy[0]), torch.autograd.grad(want, rows, gy[:1])):
+        close(a.reshape(b.shape), b, tol * 4)
+    for lead in ((0,), (3, 0)):
+        none = [t.detach().requires_grad_() for t in (x.new_zeros(*lead, 32), *ws, *bs)]
+        y = kernel.mlp_packed(*none)
+        assert y.shape == (*lead, 32)
+        for t, g in zip(none, torch.autograd.grad(y, none, torch.zeros_like(y))):
+            assert g.shape == t.shape and not g.any()
+    turned = [t.detach().t().contiguous().t().requires_grad_() for t in ws]
+    y = kernel.mlp_packed(x, *turned, *bs)
+    assert torch.autograd.grad(y, turned, gy)[0].shape == ws[0].shape
+
+
 def test_mlp_under_autocast():
     x, ws, bs, gy = _mlp_case(F32, (20,), 32, 64, 32, True)
     leaves = [t.detach().requires_grad_() for t in (x, *ws, *bs)]

@@ -48,7 +48,7 @@ def _together(seed, B=3, T=500, V=333, C=64):
     return leaves, run, [torch.full((B, T), -1.0 / (B * T), device=DEV)]
 
 
-CASES = dict(embed=_embed, norm=_norm, gelu=_gelu, mlp=_mlp, together=_together)
+CASES = dict(embed=_embed, embed_counted=lambda seed: _embed(seed, N=20000, C=40), norm=_norm, gelu=_gelu, mlp=_mlp, together=_together)
 
 
 def _eager(leaves, run, seeds):

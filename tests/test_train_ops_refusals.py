@@ -108,11 +108,20 @@ def test_embed_bwd_arguments(change, code, text):
     _refused(L.saf_embed_bwd(_t((3,), _I64), a["dout"], 1.0, -100, a["dweight"], a["ws"], n, None), code, text)
 
 
+def test_embed_bwd_sizes():
+    """More threads than a launch has are refused, not cut short."""
+    L, n, C = _ext.lib(), 1 << 28, 8192
+    _refused(L.saf_embed_bwd(_t((n,), _I64), _t((n, C), _BF16), 1.0, -100, _t((9, C), _BF16), 0x100000, 1 << 60, None),
+             _ext.SAF_EUNSUPPORTED, "too many tokens")
+    _refused(L.saf_embed_bwd(_t((n + 1,), _I64), _t((n + 1, 8), _BF16), 1.0, -100, _t((9, 8), _BF16), 0x100000, 1 << 60, None),
+             _ext.SAF_EUNSUPPORTED, "at most 2^28")
+
+
 def test_embed_workspace():
     f = _ext.lib().saf_embed_bwd_workspace_bytes
     assert f(0, 9, 16) == 0
     assert f(3, 9, 16) == 256 and f(64, 9, 16) == 512   # one chunk: the sorted positions alone
-    assert f(-1, 9, 16) == f(3, 0, 16) == f(3, 9, 0) == f(1 << 32, 9, 16) == f(3, 1 << 31, 16) == -1
+    assert f(-1, 9, 16) == f(3, 0, 16) == f(3, 9, 0) == f((1 << 28) + 1, 9, 16) == f(3, 1 << 31, 16) == -1
     # a second buffer and digit counts only with several tiles (and passes)
     assert f(8193, 600, 8) - f(8193, 500, 8) == (8 * 8193 + 255) // 256 * 256
     assert f(8192, 600, 8) == f(8192, 500, 8)
@@ -122,6 +131,8 @@ def test_embed_workspace():
     (dict(x=_t((3, 16), _I32)), _ext.SAF_EUNSUPPORTED, "unsupported dtype int32"),
     (dict(x=_t((3, 16385), _BF16)), _ext.SAF_EUNSUPPORTED, "C = 16385"),
     (dict(x=_t((3, 0), _BF16)), _ext.SAF_EUNSUPPORTED, "C = 0"),
+    (dict(x=_t((1 << 29, 16), _BF16)), _ext.SAF_EUNSUPPORTED, "too many rows"),
+    (dict(x=_t((1 << 22, 16384), _BF16)), _ext.SAF_EUNSUPPORTED, "too many rows"),
     (dict(y=_t((3, 16), _F32)), _ext.SAF_EUNSUPPORTED, "bfloat16 x with float32 y"),
     (dict(x=_t((3, 16), _F16)), _ext.SAF_EUNSUPPORTED, "float16 x with bfloat16 y"),
     (dict(delta=_t((3, 16), _F32)), _ext.SAF_EINVAL, "r must have x's dtype and delta y's"),
