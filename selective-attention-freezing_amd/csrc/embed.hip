@@ -11,7 +11,8 @@
 // 1. The positions n are sorted by token, stable, least significant digit first
 //    (9 bits at most a pass), while the other workgroups of the same launches
 //    clear dW: the sort takes no time of its own as long as it is the shorter.
-//    Up to kEmbedOnce tokens one workgroup sorts in LDS in one launch.  More go tile
+//    Up to kEmbedFew tokens nothing is sorted: each workgroup looks for the words of its
+//    rows in the list of tokens.  Up to kEmbedOnce tokens one workgroup sorts in LDS in one launch.  More go tile
 //    by tile, a launch a pass that places every tile's keys; each workgroup counts the
 //    digits of all keys for itself, from kEmbedCounted tokens on a launch before it
 //    counts them once, and past kEmbedScanned tiles another sums the counts up.
@@ -444,6 +445,75 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const EmbedBwdParams p) 
   if (word != V) finish(word == __builtin_amdgcn_readfirstlane(right));
 }
 
+// Up to kEmbedFew tokens, as many as a wave has lanes: a workgroup owns a run of rows
+// of dW, clears them, finds the words among them in the list of all tokens, and sums
+// their rows of dy, a wave 256 channels of a word.  One launch, no workspace.
+constexpr int kFewThreads = 512;
+
+template <typename TW, typename TY>
+__global__ __launch_bounds__(kFewThreads) void embed_few_kernel(const EmbedBwdParams p) {
+  static_assert(kEmbedFew == 64, "a lane a token");
+  const int N = (int)p.N, C = p.C, t = threadIdx.x, lane = t & 63;
+  const int64_t per = (p.V + gridDim.x - 1) / gridDim.x, v0 = blockIdx.x * per;
+  if (v0 >= p.V) return;
+  const int64_t v1 = v0 + per < p.V ? v0 + per : p.V;
+  uint32_t key[1];  // every wave has all of them
+  keys_of(p, N, [&](int) { return lane; }, key);
+  // rows as bytes: whole pieces of 16, and what is left before and behind them
+  char* base = reinterpret_cast<char*>(p.dw);
+  const int64_t lo = v0 * C * (int64_t)sizeof(TW), hi = v1 * C * (int64_t)sizeof(TW);
+  const int64_t a = (lo + 15) / 16 * 16 < hi ? (lo + 15) / 16 * 16 : hi, b = hi / 16 * 16 > a ? hi / 16 * 16 : a;
+  for (int64_t o = a + 16 * t; o < b; o += 16 * kFewThreads)
+    __builtin_nontemporal_store(u32x4_any{0, 0, 0, 0}, reinterpret_cast<u32x4_any*>(base + o));
+  if (lo + 2 * t < a) *reinterpret_cast<uint16_t*>(base + lo + 2 * t) = 0;
+  if (b + 2 * t < hi) *reinterpret_cast<uint16_t*>(base + b + 2 * t) = 0;
+  __builtin_amdgcn_s_waitcnt(0);  // a row's zeros are written before another wave writes its sums
+  __syncthreads();
+  const TY* dy = reinterpret_cast<const TY*>(p.dy);
+  const int blocks = (C + 255) / 256;
+  // the words of these rows one after the other, their channels dealt out to the waves
+  uint64_t left = __ballot(lane < N && key[0] >= (uint32_t)v0 && key[0] < (uint32_t)v1);
+  for (int unit = 0; left; unit += blocks) {
+    const uint32_t word = __builtin_amdgcn_readlane(key[0], __builtin_ctzll(left));
+    const uint64_t all = __ballot(lane < N && key[0] == word);
+    left &= ~all;
+    for (int block = 0; block < blocks; ++block) {
+      if ((unit + block) % (kFewThreads / 64) != t >> 6) continue;
+      const int c = 256 * block + 4 * lane;
+      const int at = c < C ? c : 0, have = C - at < 4 ? C - at : 4, put = c < C ? have : 0;
+      float acc[4] = {};
+      for (uint64_t is = all; is;) {
+        // eight rows on their way before the first is added; behind the last a repeat of it
+        constexpr int G = 8;
+        const int live = __popcll(is);
+        int n[G];
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          n[j] = is ? __builtin_ctzll(is) : n[j ? j - 1 : 0];
+          is &= is - 1;
+        }
+        Row4<TY> rows[G];
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          const TY* from = dy + (int64_t)n[j] * p.dy_rs + at;
+          if (have == 4) rows[j] = Row4<TY>::load(from);
+          else rows[j] = Row4<TY>::load_part(from, have);
+        }
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          float f[4];
+          rows[j].unpack(f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = j < live ? acc[e] + f[e] : acc[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] *= p.scale;
+      store4<false>(reinterpret_cast<TW*>(p.dw) + (int64_t)word * C + c, acc, put);
+    }
+  }
+}
+
 // Words that cross chunks: the workgroups of the chunk where one begins add its
 // partials, kLanes of them at a time for 32 groups of 8 channels, each lane's in
 // order and then the lanes in order.
@@ -506,25 +576,33 @@ void sum(const EmbedBwdParams& p, hipStream_t s) {
   if (p.C % 4 == 0) hipLaunchKernelGGL((embed_sum_kernel<TW, TY, true>), grid, wg, 0, s, p);
   else hipLaunchKernelGGL((embed_sum_kernel<TW, TY, false>), grid, wg, 0, s, p);
 }
+template <typename TW, typename TY>
+void few(const EmbedBwdParams& p, hipStream_t s) {
+  hipLaunchKernelGGL((embed_few_kernel<TW, TY>), dim3((unsigned)p.n_clear), dim3(kFewThreads), 0, s, p);
+}
+template <typename TW, typename TY>
+void few_or_sum(const EmbedBwdParams& p, hipStream_t s) {
+  if (p.N <= kEmbedFew) few<TW, TY>(p, s);
+  else sum<TW, TY>(p, s);
+}
 // bf16 and fp16 do not meet (the C entry refuses them).
 template <typename TW>
-void sum(const EmbedBwdParams& p, int dtype, hipStream_t s) {
+void few_or_sum(const EmbedBwdParams& p, int dtype, hipStream_t s) {
   if constexpr (sizeof(TW) == 4) {
-    if (dtype == kF32) sum<float, float>(p, s);
-    else if (dtype == kBF16) sum<float, __bf16>(p, s);
-    else sum<float, _Float16>(p, s);
+    if (dtype == kF32) few_or_sum<float, float>(p, s);
+    else if (dtype == kBF16) few_or_sum<float, __bf16>(p, s);
+    else few_or_sum<float, _Float16>(p, s);
   } else {
-    if (dtype == kF32) sum<TW, float>(p, s);
-    else sum<TW, TW>(p, s);
+    if (dtype == kF32) few_or_sum<TW, float>(p, s);
+    else few_or_sum<TW, TW>(p, s);
   }
 }
 
 template <typename TW>
 hipError_t bwd_t(const EmbedBwdParams& p, int dtype, hipStream_t s) {
   const dim3 sort_wg(kSortThreads);
-  if (p.n_tiles == 0) {  // nothing but zeros
-    hipLaunchKernelGGL(embed_count_kernel, dim3((unsigned)p.n_clear), sort_wg, 0, s, p, (const uint2*)nullptr, 0, (int64_t)0,
-                       p.dw_bytes);
+  if (p.N <= kEmbedFew) {
+    few_or_sum<TW>(p, dtype, s);
     return hipGetLastError();
   }
   if (p.N <= kEmbedOnce) {
@@ -550,7 +628,7 @@ hipError_t bwd_t(const EmbedBwdParams& p, int dtype, hipStream_t s) {
       from = to;
     }
   }
-  sum<TW>(p, dtype, s);
+  few_or_sum<TW>(p, dtype, s);
   const int64_t n_chunks = (p.N + p.chunk - 1) / p.chunk;
   if (n_chunks > 1)
     hipLaunchKernelGGL((embed_join_kernel<TW>), dim3((unsigned)(n_chunks - 1), (unsigned)((p.C + 255) / 256)), dim3(32 * kLanes),

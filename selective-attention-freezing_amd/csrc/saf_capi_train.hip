@@ -94,7 +94,6 @@ struct EmbedPlan {
 // 16384 tokens of a natural distribution at 768 channels, 25 and 20 for 32768, 35 and
 // 31 for 65536.
 int chunk_of(int64_t N, int64_t C) {
-  if (N <= 64) return 64;  // one chunk: no parts to join, a launch less
   const int64_t waves = (N + 63) / 64 * ((C + 255) / 256);
   return waves >= 1024 ? 64 : (waves >= 512 ? 32 : 16);
 }
@@ -103,6 +102,7 @@ int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 EmbedPlan embed_plan(int64_t N, int64_t V, int64_t C) {
   EmbedPlan e{};
+  if (N <= kEmbedFew) return e;
   e.n_tiles = (int)((N + kEmbedTile - 1) / kEmbedTile);
   int key_bits = 1;  // of the words and of the key behind them, V
   while ((V >> key_bits) != 0) ++key_bits;
@@ -230,8 +230,8 @@ int saf_embed_bwd(const saf_tensor_t* tokens, const saf_tensor_t* dout, float sc
   p.passes = e.passes;
   p.bits = e.bits;
   p.chunk = e.chunk;
-  // workgroups that clear: 64 KB each, at most one a CU
-  const int64_t want = (p.dw_bytes + 65535) / 65536;
+  // workgroups that clear: 64 KB each, 16 of a few tokens', at most one a CU
+  const int64_t part = N <= kEmbedFew ? 16384 : 65536, want = (p.dw_bytes + part - 1) / part;
   p.n_clear = (int)(want < cu_count() ? want : cu_count());
   return launched(launch_embed_bwd(p, dweight->dtype, dout->dtype, stream_of(stream)), "embed_bwd");
 }

@@ -388,6 +388,9 @@ enum class ActPackOp { kPack, kUnpack, kGelu, kGeluBwd };
 
 // Embedding lookup and gradient (embed.hip); a unit is 8 channels of a token, in the
 // backward pass 256 channels of a chunk of at most 64 sorted positions.
+// Tokens that nothing is sorted for (64, 50304 x 768 bf16: 18 us in one launch, 22 in
+// three with the sort; 256: 23 and 23, all of one word 38 and 24).
+constexpr int kEmbedFew = 64;
 // Tokens that one workgroup sorts by itself (8192 in two passes: 25 us, one launch;
 // by tiles 24 in two, 44 against 29 for 16384), a workgroup's part of more, and the
 // number from which their digits are counted once in launches of their own (16384: 29

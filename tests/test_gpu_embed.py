@@ -51,17 +51,17 @@ def test_types_and_sizes(wt, yt, N, V, C):
     _check(t, rnd(V, C, seed=1, dtype=wt), rnd(N, C, seed=2, dtype=yt), 1.0 if C % 2 else 3.3, dtype=yt)
 
 
-@pytest.mark.parametrize("N", [15, 16, 17, 63, 64, 65, 1023, 8191, 8192, 8193, 10240, 16384, 16385, 40000])
+@pytest.mark.parametrize("N", [15, 16, 17, 63, 64, 65, 255, 256, 257, 1023, 8191, 8192, 8193, 10240, 16384, 16385, 40000])
 @pytest.mark.parametrize("V", [2, 511, 512, 40000, 262143, 300000])
 def test_sorting(N, V):
-    """One to three passes, one tile and several, chunks of 16 and 32 positions, words
+    """Few tokens, one to three passes, one tile and several, chunks of 16 and 32 positions, words
     of one position and of thousands."""
     t = _tokens(N, V, N + V, skew=3.0)
     t[5::11] = -100
     _check(t, rnd(V, 5, seed=3), rnd(N, 5, seed=4), 1.0)
 
 
-@pytest.mark.parametrize("N", [1, 16, 40, 64, 65, 9000, 140001])
+@pytest.mark.parametrize("N", [1, 16, 40, 64, 65, 256, 257, 9000, 140001])
 @pytest.mark.parametrize("word", [0, 96])
 def test_one_word(N, word):
     t = torch.full((N,), word, device=DEV)

@@ -93,8 +93,8 @@ def test_embed_arguments(change, code, text):
 
 
 @pytest.mark.parametrize("change,code,text", [
-    (dict(dout=_t((4, 16), _BF16)), _ext.SAF_EINVAL, "dout must be (3, 16)"),
-    (dict(dout=_t((3, 16), _F16)), _ext.SAF_EUNSUPPORTED, "bf16 beside fp16"),
+    (dict(dout=_t((301, 16), _BF16)), _ext.SAF_EINVAL, "dout must be (300, 16)"),
+    (dict(dout=_t((300, 16), _F16)), _ext.SAF_EUNSUPPORTED, "bf16 beside fp16"),
     (dict(dweight=_t((9, 16), _BF16, (32, 1))), _ext.SAF_EALIGN, "dweight must be contiguous"),
     (dict(dweight=_t((9, 16), _BF16, ptr=0x100008)), _ext.SAF_EALIGN, "dweight must be 16-byte aligned"),
     (dict(ws=None), _ext.SAF_EWORKSPACE, "workspace"),
@@ -103,9 +103,9 @@ def test_embed_arguments(change, code, text):
 ])
 def test_embed_bwd_arguments(change, code, text):
     L = _ext.lib()
-    a = dict(dict(dout=_t((3, 16), _BF16), dweight=_t((9, 16), _BF16), ws=0x100000, short=0), **change)
-    n = L.saf_embed_bwd_workspace_bytes(3, 9, 16) - a["short"]
-    _refused(L.saf_embed_bwd(_t((3,), _I64), a["dout"], 1.0, -100, a["dweight"], a["ws"], n, None), code, text)
+    a = dict(dict(dout=_t((300, 16), _BF16), dweight=_t((9, 16), _BF16), ws=0x100000, short=0), **change)
+    n = L.saf_embed_bwd_workspace_bytes(300, 9, 16) - a["short"]
+    _refused(L.saf_embed_bwd(_t((300,), _I64), a["dout"], 1.0, -100, a["dweight"], a["ws"], n, None), code, text)
 
 
 def test_embed_bwd_sizes():
@@ -119,8 +119,8 @@ def test_embed_bwd_sizes():
 
 def test_embed_workspace():
     f = _ext.lib().saf_embed_bwd_workspace_bytes
-    assert f(0, 9, 16) == 0
-    assert f(3, 9, 16) == 256 and f(64, 9, 16) == 512   # one chunk: the sorted positions alone
+    assert f(0, 9, 16) == 0 and f(65, 9, 16) > 8 * 65
+    assert f(3, 9, 16) == f(64, 9, 16) == 0          # nothing is sorted
     assert f(-1, 9, 16) == f(3, 0, 16) == f(3, 9, 0) == f((1 << 28) + 1, 9, 16) == f(3, 1 << 31, 16) == -1
     # a second buffer and digit counts only with several tiles (and passes)
     assert f(8193, 600, 8) - f(8193, 500, 8) == (8 * 8193 + 255) // 256 * 256
