@@ -201,8 +201,10 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
       if (p.ddelta) store_row8(reinterpret_cast<TB*>(p.ddelta) + row * C, c, C, d);
     }
   }
-  if (!p.part) return;
+  if (!p.dw && !p.db) return;
+  // a workgroup by itself has the sums; the others' parts are added by the next launch
   float* out = p.part + (int64_t)blockIdx.x * 2 * C;
+  const bool alone = p.part == nullptr;
   if constexpr (TPR < 256) {
     const int wave = threadIdx.x >> 6;
 #pragma unroll
@@ -225,15 +227,31 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
       const int c = 8 * (i / (8 * TPR) * TPR + i % TPR) + i / TPR % 8;
       if (c >= C) continue;
       const float2 p0 = part[0][i], p1 = part[1][i], p2 = part[2][i], p3 = part[3][i];
-      out[c] = (p0.x + p1.x) + (p2.x + p3.x);
-      out[C + c] = (p0.y + p1.y) + (p2.y + p3.y);
+      const float sw = (p0.x + p1.x) + (p2.x + p3.x), sb = (p0.y + p1.y) + (p2.y + p3.y);
+      if (!alone) {
+        out[c] = sw;
+        out[C + c] = sb;
+      } else {
+        if (p.dw) store_elem(p.dw, p.w_dtype, c, sw);
+        if (p.db) store_elem(p.db, p.w_dtype, c, sb);
+      }
     }
     return;
   }
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
-    store_row8(out, 8 * (TPR * k + t), C, aw[k]);
-    store_row8(out + C, 8 * (TPR * k + t), C, ab[k]);
+    const int c = 8 * (TPR * k + t);
+    if (!alone) {
+      store_row8(out, c, C, aw[k]);
+      store_row8(out + C, c, C, ab[k]);
+      continue;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < C) {
+        if (p.dw) store_elem(p.dw, p.w_dtype, c + e, aw[k][e]);
+        if (p.db) store_elem(p.db, p.w_dtype, c + e, ab[k][e]);
+      }
   }
 }
 
@@ -310,7 +328,7 @@ template <typename TX, typename TB, int TPR, int NCH> struct Bwd {
   static hipError_t run(const LnTrainBwdParams& p, hipStream_t s) {
     if (p.n_wg > 0)
       hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TB, TPR, NCH>), dim3((unsigned)p.n_wg), dim3(kThreads<TPR>), 0, s, p);
-    if (p.dw || p.db)
+    if ((p.dw || p.db) && p.n_wg != 1)
       hipLaunchKernelGGL(layernorm_dw_kernel, dim3((unsigned)((p.C + 31) / 32), 2), dim3(1024), 0, s, p, p.n_wg);
     return hipGetLastError();
   }
@@ -338,12 +356,14 @@ int layernorm_row_threads(int C) {
   return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : n <= 128 ? 64 : n <= 256 ? 128 : n <= 1024 ? 256 : 1024;
 }
 
-// Workgroups of the backward pass: as many as are resident, each with at least
-// one round of rows.
+// Workgroups of the backward pass: as many as are resident, each with at least one
+// round of rows.  One for up to four rounds of rows of a wave or less, which needs no
+// second launch (32 x 768: 9 us, 6 + 3 and the gap between in two; 4 x 8192 17 and 9).
 int layernorm_bwd_groups(int64_t rows, int C, int n_cu) {
   const int n = (C + 7) / 8;
   const int per = n <= 8 ? 32 : (n <= 16 ? 16 : (n <= 128 ? 8 : (n <= 256 ? 4 : 1)));
   const int64_t rounds = (rows + per - 1) / per;
+  if (rounds <= (n <= 256 ? 4 : 1)) return 1;
   const int64_t most = (int64_t)n_cu * (n <= 1024 ? 2 : 1);
   return (int)(rounds < most ? rounds : most);
 }

@@ -290,7 +290,8 @@ int64_t saf_layernorm_bwd_workspace_bytes(int64_t rows, int64_t channels) {
     fail(SAF_EINVAL, "layernorm: rows of %lld channels are not supported", (long long)channels);
     return -1;
   }
-  return rows == 0 ? 0 : (int64_t)layernorm_bwd_groups(rows, (int)channels, cu_count()) * 2 * channels * 4;
+  const int n_wg = rows == 0 ? 0 : layernorm_bwd_groups(rows, (int)channels, cu_count());
+  return n_wg > 1 ? (int64_t)n_wg * 2 * channels * 4 : 0;
 }
 
 int saf_layernorm_bwd(const saf_tensor_t* r, const saf_tensor_t* stats, const saf_tensor_t* weight,
@@ -330,7 +331,7 @@ int saf_layernorm_bwd(const saf_tensor_t* r, const saf_tensor_t* stats, const sa
   if (R == 0 && !p.dw && !p.db) return SAF_OK;
   if (p.dw || p.db) {
     if (int rc = check_workspace("layernorm_bwd", workspace, workspace_bytes, ws_bytes)) return rc;
-    p.part = reinterpret_cast<float*>(workspace);
+    if (ws_bytes > 0) p.part = reinterpret_cast<float*>(workspace);
   }
   p.r = r->data;
   p.r_rs = r->stride[0];

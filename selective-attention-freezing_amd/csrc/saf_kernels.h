@@ -361,7 +361,7 @@ struct LnTrainBwdParams {
   void* ddelta;       // dx in the branch's type; null: not wanted
   void* dw;           // null: not wanted
   void* db;           // null: not wanted
-  float* part;        // (n_wg, 2, C); null: neither dw nor db
+  float* part;        // (n_wg, 2, C) with several workgroups, else null
   int64_t rows, r_rs, dy_rs, dr_rs;
   int C, w_dtype, n_wg;
   int once;           // dy's and dr's rows are 16-byte aligned

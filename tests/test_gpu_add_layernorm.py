@@ -62,10 +62,10 @@ def test_widest(xt, yt, C):
     _check(**_case(5, C, xt, yt, F32, seed=C), dtype=yt)
 
 
-@pytest.mark.parametrize("R", [1, 2, 7, 8, 9, 4095, 4096, 5001])
+@pytest.mark.parametrize("R", [1, 2, 4, 5, 7, 8, 9, 16, 17, 31, 32, 33, 63, 64, 65, 128, 129, 4095, 4096, 5001])
 @pytest.mark.parametrize("C", [40, 100, 64, 1280, 2100])
 def test_rows(R, C):
-    """Fewer rows than workgroups, and more: ragged last rounds."""
+    """One workgroup, fewer rows than workgroups, and more: ragged last rounds."""
     _check(**_case(R, C, BF16, BF16, BF16, seed=R))
 
 

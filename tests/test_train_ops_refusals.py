@@ -152,22 +152,22 @@ def test_layernorm_arguments(change, code, text):
 
 
 @pytest.mark.parametrize("change,code,text", [
-    (dict(dy=_t((3, 16), _F32)), _ext.SAF_EUNSUPPORTED, "bfloat16 r with float32 dy"),
+    (dict(dy=_t((300, 16), _F32)), _ext.SAF_EUNSUPPORTED, "bfloat16 r with float32 dy"),
     (dict(stats=_NONE), _ext.SAF_EINVAL, "stats is required"),
-    (dict(dr=_t((3, 16), _F32)), _ext.SAF_EINVAL, "dr and dx must have r's dtype"),
-    (dict(dx=_t((3, 16), _BF16, (20, 1))), _ext.SAF_EALIGN, "dx must be contiguous"),
-    (dict(ddelta=_t((3, 16), _F32)), _ext.SAF_EINVAL, "ddelta must have dy's dtype"),
+    (dict(dr=_t((300, 16), _F32)), _ext.SAF_EINVAL, "dr and dx must have r's dtype"),
+    (dict(dx=_t((300, 16), _BF16, (20, 1))), _ext.SAF_EALIGN, "dx must be contiguous"),
+    (dict(ddelta=_t((300, 16), _F32)), _ext.SAF_EINVAL, "ddelta must have dy's dtype"),
     (dict(dw=_t((16,), _BF16)), _ext.SAF_EINVAL, "of the weight's dtype"),
     (dict(ws=None), _ext.SAF_EWORKSPACE, "workspace"),
     (dict(ws=0x100010), _ext.SAF_EALIGN, "256-byte aligned"),
 ])
 def test_layernorm_bwd_arguments(change, code, text):
-    a = dict(dict(dy=_t((3, 16), _BF16), stats=_t((3, 2), _F32), dr=_NONE, dx=_t((3, 16), _BF16), ddelta=_NONE,
+    a = dict(dict(dy=_t((300, 16), _BF16), stats=_t((300, 2), _F32), dr=_NONE, dx=_t((300, 16), _BF16), ddelta=_NONE,
                   dw=_t((16,), _F32), ws=0x100000), **change)
     L = _ext.lib()
-    n = L.saf_layernorm_bwd_workspace_bytes(3, 16)
+    n = L.saf_layernorm_bwd_workspace_bytes(300, 16)
     assert n > 0
-    _refused(L.saf_layernorm_bwd(_t((3, 16), _BF16), a["stats"], _t((16,), _F32), a["dy"], a["dr"], a["dx"], a["ddelta"],
+    _refused(L.saf_layernorm_bwd(_t((300, 16), _BF16), a["stats"], _t((16,), _F32), a["dy"], a["dr"], a["dx"], a["ddelta"],
                                  a["dw"], _NONE, a["ws"], n, None), code, text)
 
 
@@ -175,7 +175,7 @@ def test_layernorm_workspace():
     f = _ext.lib().saf_layernorm_bwd_workspace_bytes
     assert f(0, 16) == 0
     assert f(-1, 16) == f(3, 0) == f(3, 16385) == -1
-    assert f(1, 16) == 2 * 16 * 4
+    assert f(1, 16) == f(128, 16) == 0 and f(129, 16) == 5 * 2 * 16 * 4    # rounds of 32 rows, four by one workgroup
 
 
 @pytest.mark.parametrize("change,code,text", [
