@@ -14,6 +14,7 @@ autocast dtype.
 import torch
 
 import kernel as _kernel_mod
+from kernel import _ext
 from nanogpt.model import MLP
 
 
@@ -25,6 +26,9 @@ def forward_hidden(model, idx, packed=True):
         raise ValueError(f"sequences of {T} tokens exceed the model's block size {model.config.block_size}")
     tr = model.transformer
     x = _kernel_mod.embed_tokens(idx, tr.wte.weight)
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        # weights of torch's own operators as well, which would not refuse the capture
+        _ext.bind().check_differentiable("nanogpt.train", *model.parameters())
     dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
     rope = None
     if model.rotary is None:

@@ -7,7 +7,7 @@ import torch
 import torch.nn.functional as F
 
 import kernel
-from train_cases import BF16, DEV, F16, F32, HALF, LEAST, U, cdf, close, gelu_tol, held, pdf, rnd, slope_tol
+from train_cases import BF16, DEV, F16, F32, HALF, LEAST, U, cdf, close, gelu_tol, held, in_use, pdf, rnd, slope_tol
 
 pytestmark = pytest.mark.gpu
 
@@ -169,9 +169,9 @@ def test_what_is_kept():
     x = rnd(1 << 12, 1 << 10, seed=1, dtype=BF16)
     leaf = x.requires_grad_()
     torch.cuda.synchronize()
-    before = torch.cuda.memory_allocated()
+    before = in_use()
     y = kernel.gelu_packed(leaf)
-    assert torch.cuda.memory_allocated() - before <= y.numel() * (2 + 1 + 1 / 32) + 4096
+    assert in_use() - before <= y.numel() * (2 + 1 + 1 / 32) + 4096
 
 
 # ---- the whole MLP ------------------------------------------------------------------
@@ -287,9 +287,9 @@ def test_mlp_keeps_8_bits():
     leaves = [t.detach().requires_grad_() for t in (x, *ws)]
     kernel.mlp_packed(*leaves).sum().backward()              # workspaces of the products
     torch.cuda.synchronize()
-    before = torch.cuda.memory_allocated()
+    before = in_use()
     y = kernel.mlp_packed(*leaves)
-    assert torch.cuda.memory_allocated() - before <= y.numel() * 2 + R * 5 * C * (1 + 1 / 32) + 8192
+    assert in_use() - before <= y.numel() * 2 + R * 5 * C * (1 + 1 / 32) + 8192
 
 
 def test_mlp_is_differentiated_once():

@@ -6,7 +6,7 @@ import torch
 import kernel
 from nanogpt import train
 from nanogpt.model import GPT, GPTConfig
-from train_cases import BF16, DEV, F32
+from train_cases import BF16, DEV, F32, in_use
 
 pytestmark = pytest.mark.gpu
 
@@ -154,6 +154,23 @@ def test_refusals():
         train.forward_hidden(m, torch.zeros(1, 129, dtype=torch.long, device=DEV))
 
 
+def test_capture_is_refused_while_an_eager_graph_lives():
+    """Also where only weights of torch's own operators are trained."""
+    m = _model(dtype=BF16, frozen=False)
+    m.requires_grad_(False)
+    for b in m.transformer.h:
+        b.attn.q_proj.requires_grad_()
+        b.attn.k_proj.requires_grad_()
+    idx, nxt = _batch(m)
+    alive = train.token_logprobs(m, idx, nxt).logp
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            train.token_logprobs(m, idx, nxt)
+    torch.cuda.synchronize()
+    assert torch.isfinite(alive).all()
+
+
 def test_memory():
     """The packed step keeps less: the MLPs' activations in 8 bits."""
     m = _model(dtype=BF16, layers=4, frozen=False)
@@ -162,9 +179,9 @@ def test_memory():
     for packed in (False, True):
         _loss_and_grads(m, lambda: train.token_logprobs(m, idx, nxt, packed=packed).logp)   # workspaces
         torch.cuda.synchronize()
-        before = torch.cuda.memory_allocated()
+        before = in_use()
         h = train.forward_hidden(m, idx, packed)
-        held[packed] = torch.cuda.memory_allocated() - before
+        held[packed] = in_use() - before
         del h
     rows, C = 32 * 128, 128
     # 4 layers x (8 + 8 C) bytes of u and gelu(u) against 4 (1 + 1/32) C; x is kept by no

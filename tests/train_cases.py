@@ -28,6 +28,13 @@ def close(got, want, tol, what=""):
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()}, worst excess {float((d - tol)[bad].max()):.3e}"
 
 
+def in_use():
+    """Bytes that the live tensors asked for.  memory_allocated() counts the blocks that
+    serve them: a free one that is up to 1 MiB larger is handed out whole, so what it
+    shows depends on what ran before."""
+    return torch.cuda.memory_stats()["requested_bytes.all.current"]
+
+
 # ---- LayerNorm --------------------------------------------------------------------
 
 def norm_exact(x, delta, w, b, eps, dy=None, dr=None):
