@@ -427,7 +427,7 @@ struct EmbedBwdParams {
   float scale;
   int C;
   uint2* sorted;    // (N) token, position
-  uint2* sorted2;   // (N) with more than kEmbedOnce tokens and one pass
+  uint2* sorted2;   // (N) with more tokens than kEmbedOnce and more passes than one
   uint32_t* counts; // (n_tiles + 1, 2^kEmbedDigit) from kEmbedCounted tokens on, else null
   float* head;      // (chunks, C) sums of a chunk's first word where that began before it
   float* tail;      // (chunks, C) sums of its last word where that goes on
