@@ -27,16 +27,35 @@ namespace saf {
 
 namespace {
 
-// Phi(u) and exp(-u^2 / 2).  float32: the library's erfc and exp.  16-bit types:
-// for a = |u| the tail Phi(-a) = exp(-a^2 / 2) t P(t), t = 1 / (1 + 0.3 a), P of
-// degree 5 fitted to erfcx(a / sqrt 2) / (2 t) for its largest relative error over
-// 0 <= a <= 14.5 (9.2e-6 evaluated in float32: 1/50 of half an fp16 step),
-// so that small results far below zero keep their digits.
+// Phi(u) and exp(-u^2 / 2): for a = |u| the tail Phi(-a) = exp(-a^2 / 2) t P(t),
+// t = 1 / (1 + c a), P fitted to erfcx(a / sqrt 2) / (2 t) for its largest relative
+// error over 0 <= a <= 14.5, so that small results far below zero keep their digits.
+// 16-bit types: degree 5, 9.2e-6 evaluated in float32 (1/50 of half an fp16 step).
+// float32: degree 8, 3.2e-8; the tail is within 12 float32 roundings (2^-24), as what
+// the square and the product lose is given back to the exponential.  With the library's
+// erfc and exp in its place 16384 x 4096 float32 took 146 us forward and 166 backward,
+// 113 and 112 so (5.4 TB/s).
 template <bool EXACT>
 __device__ inline float normal_cdf(float u, float& e) {
   if constexpr (EXACT) {
-    e = expf(-0.5f * u * u);
-    return 0.5f * erfcf(u * -0.70710678118654752f);
+    constexpr float kHi = -0.7213475108146667f, kLo = -9.629815167500055e-09f;  // -log2(e) / 2
+    const float a = fminf(fabsf(u), 20.f);  // behind it nothing is left, and the square stays finite
+    const float s = a * a, x = s * kHi;
+    const float rest = fmaf(s, kHi, -x) + fmaf(s, kLo, fmaf(a, a, -s) * kHi);
+    e = fast_exp2(x);
+    e = fmaf(e, rest * 0.6931471805599453f, e);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, a, 1.f));
+    float h = -0.029157886281609535f;
+    h = fmaf(h, t, 0.14403091371059418f);
+    h = fmaf(h, t, -0.2558389902114868f);
+    h = fmaf(h, t, 0.1593196988105774f);
+    h = fmaf(h, t, -0.023212352767586708f);
+    h = fmaf(h, t, 0.10555250197649002f);
+    h = fmaf(h, t, 0.11982128769159317f);
+    h = fmaf(h, t, 0.139863520860672f);
+    h = fmaf(h, t, 0.139621302485466f);
+    h *= t * e;
+    return u < 0.f ? h : 1.f - h;
   } else {
     const float a = fabsf(u);
     e = fast_exp2(u * u * (-0.5f * kLog2e));

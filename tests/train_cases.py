@@ -102,7 +102,7 @@ def pdf(z):
 
 def gelu_tol(z, dtype):
     """Error of z Phi(z) before its rounding.  The tail Phi(-|z|) is off relatively
-    by the fit (9.2e-6, 16-bit types) or the library's erfc (16 U), by the rounding
+    by the fit (9.2e-6, 16-bit types; 16 U, float32), by the rounding
     of its exponent z^2 / 2 (z^2 U, twice: the square and the product) and a few
     operations; for z > 0 the tail is subtracted from 1 (one U of the result).
     Results under 2^-120 may be zero."""
