@@ -14,9 +14,11 @@
 //
 // A row belongs to TPR threads (from eight lanes for 64 channels to sixteen waves for
 // 16384), each with NCH chunks of 8 channels, chunk k at channel 8 (TPR k + thread):
-// every load and store of the group is one run.  2^25 elements take 41 us forward and
-// 50 backward in bf16, 97 and 95 in float32 (6.6 and 5.4, 5.5 and 5.6 TB/s; a copy
-// reaches 5.2), at most a third more at widths that fill the last chunks badly.
+// every load and store of the group is one run.  2^25 elements take 40 us forward and
+// 52 backward in bf16, 93 and 96 in float32 (6.7 and 5.2, 5.8 and 5.6 TB/s; a copy
+// reaches 5.2).  At odd widths a row's last chunk is read as its last 8 channels and
+// moved into place in registers (333 channels of bf16: element by element 79 and 98 us,
+// so 57 and 68; 2047 of float32 backward 134 and 111).
 //
 // What nothing reads again goes past the caches: dy and dr (8192 x 2048, float32
 // beside bf16, both directions: 105 us through them, 99 past them), r and y (44 and 41
@@ -37,6 +39,8 @@ namespace {
 
 template <int TPR> constexpr int kGroups = TPR > 64 ? 1 : 256 / TPR;  // rows of a workgroup at a time
 template <int TPR> constexpr int kThreads = TPR > 64 ? TPR : 256;
+// Rows of less than 8 channels are among the narrowest form's only (fwd_width, bwd_width).
+template <int TPR, int NCH> constexpr RowEnd kEnd = TPR * NCH == 8 ? RowEnd::kAny : RowEnd::kEdge;
 
 // Sum over the TPR threads of a row, in a fixed order.  `slot` is LDS of the
 // reduction's own (one per sum of a row) where several waves share a row.
@@ -64,6 +68,7 @@ __device__ inline float row_sum(float v, float* slot) {
 
 template <typename TX, typename TB, int TPR, int NCH>
 __global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTrainParams p) {
+  constexpr RowEnd END = kEnd<TPR, NCH>;
   __shared__ float slots[2][TPR > 64 ? TPR / 64 : 1];
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * kGroups<TPR> + threadIdx.x / TPR;
@@ -74,31 +79,32 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTr
   Row8<TX> x[NCH];
   float v[NCH][8];
 #pragma unroll
-  for (int k = 0; k < NCH; ++k) x[k] = load_raw8(xr, 8 * (TPR * k + t), C);
+  for (int k = 0; k < NCH; ++k) x[k] = edge_raw8<END>(xr, 8 * (TPR * k + t), C);
   if (p.delta) {
     const TB* dr = reinterpret_cast<const TB*>(p.delta) + row * p.d_rs;
     TX* rr = reinterpret_cast<TX*>(p.r) + row * C;
     Row8<TB> a[NCH];
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) a[k] = load_raw8(dr, 8 * (TPR * k + t), C);
+    for (int k = 0; k < NCH; ++k) a[k] = edge_raw8<END>(dr, 8 * (TPR * k + t), C);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       float d[8];
-      x[k].unpack(v[k]);
-      a[k].unpack(d);
+      edge_unpack<END>(x[k], 8 * (TPR * k + t), C, v[k]);
+      edge_unpack<END>(a[k], 8 * (TPR * k + t), C, d);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[k][e] += d[e];
       stream_row8(rr, 8 * (TPR * k + t), C, v[k]);
-      x[k] = Row8<TX>::pack(v[k]);
+      Row8<TX>::pack(v[k]).unpack(v[k]);  // the norm is that of the rounded sum
     }
-  }
+  } else {
 #pragma unroll
-  for (int k = 0; k < NCH; ++k) x[k].unpack(v[k]);
+    for (int k = 0; k < NCH; ++k) edge_unpack<END>(x[k], 8 * (TPR * k + t), C, v[k]);
+  }
   // behind the row, which then needs no registers for its pieces any more, and ahead of
   // the sums that hide them
   float w[NCH][8], b[NCH][8] = {};
-  load_vec<NCH>(p.w, p.wb_dtype, 8 * t, 8 * TPR, C, w);
-  if (p.b) load_vec<NCH>(p.b, p.wb_dtype, 8 * t, 8 * TPR, C, b);
+  load_vec<END>(p.w, p.wb_dtype, 8 * t, 8 * TPR, C, w);
+  if (p.b) load_vec<END>(p.b, p.wb_dtype, 8 * t, 8 * TPR, C, b);
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < NCH; ++k)
@@ -127,16 +133,20 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_fwd_kernel(const LnTr
   }
 }
 
-template <typename TX, typename TB, int TPR, int NCH>
+template <typename TX, typename TB, int TPR, int NCH, bool WHOLE>  // WHOLE: C is a multiple of 8
 __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTrainBwdParams p) {
+  // rows of whole chunks go through the checks of both kinds of chunk all the same: they
+  // space a wave's requests out (8192 x 4096 float32: 98 us, 109 with one check; bf16
+  // the same either way)
+  constexpr RowEnd END = WHOLE ? RowEnd::kAny : kEnd<TPR, NCH>;
   __shared__ float slots[2][TPR > 64 ? TPR / 64 : 1];
   // dw and db of the four waves of a workgroup whose rows are a wave's or less
   constexpr int kCols = 8 * TPR * NCH;
-  __shared__ float2 part[TPR >= 256 ? 1 : 4][TPR >= 256 ? 1 : kCols];
+  __shared__ float2 part[TPR > 64 ? 1 : 4][TPR > 64 ? 1 : kCols];
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int C = p.C;
   float w[NCH][8], aw[NCH][8] = {}, ab[NCH][8] = {};
-  load_vec<NCH>(p.w, p.w_dtype, 8 * t, 8 * TPR, C, w);
+  load_vec<END>(p.w, p.w_dtype, 8 * t, 8 * TPR, C, w);
   for (int64_t row = (int64_t)blockIdx.x * kGroups<TPR> + group; row < p.rows;
        row += (int64_t)gridDim.x * kGroups<TPR>) {
     const TX* rr = reinterpret_cast<const TX*>(p.r) + row * p.r_rs;
@@ -146,29 +156,29 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
     Row8<TX> r[NCH], add[NCH];
     Row8<TB> dy[NCH];
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) r[k] = load_raw8(rr, 8 * (TPR * k + t), C);
+    for (int k = 0; k < NCH; ++k) r[k] = edge_raw8<END>(rr, 8 * (TPR * k + t), C);
     if (p.once) {
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) dy[k] = once_raw8(gr, 8 * (TPR * k + t), C);
+      for (int k = 0; k < NCH; ++k) dy[k] = edge_raw8<END, true>(gr, 8 * (TPR * k + t), C);
     } else {
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) dy[k] = load_raw8(gr, 8 * (TPR * k + t), C);
+      for (int k = 0; k < NCH; ++k) dy[k] = edge_raw8<END>(gr, 8 * (TPR * k + t), C);
     }
     const TX* er = reinterpret_cast<const TX*>(p.dr) + row * p.dr_rs;
     if (kTogether && p.dr) {
       if (p.once) {
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) add[k] = once_raw8(er, 8 * (TPR * k + t), C);
+        for (int k = 0; k < NCH; ++k) add[k] = edge_raw8<END, true>(er, 8 * (TPR * k + t), C);
       } else {
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) add[k] = load_raw8(er, 8 * (TPR * k + t), C);
+        for (int k = 0; k < NCH; ++k) add[k] = edge_raw8<END>(er, 8 * (TPR * k + t), C);
       }
     }
     float xh[NCH][8], g[NCH][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      r[k].unpack(xh[k]);
-      dy[k].unpack(g[k]);
+      edge_unpack<END>(r[k], 8 * (TPR * k + t), C, xh[k]);
+      edge_unpack<END>(dy[k], 8 * (TPR * k + t), C, g[k]);
     }
 #pragma unroll
     for (int k = 0; k < NCH; ++k)
@@ -192,8 +202,8 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
       if (c >= C) continue;
       float d[8] = {};
       if (p.dr) {
-        if constexpr (!kTogether) add[k] = load_raw8(er, c, C);
-        add[k].unpack(d);
+        if constexpr (!kTogether) add[k] = edge_raw8<END>(er, c, C);
+        edge_unpack<END>(add[k], c, C, d);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = fmaf(rstd, g[k][e] - c1 - xh[k][e] * c2, d[e]);
@@ -205,7 +215,7 @@ __global__ __launch_bounds__(kThreads<TPR>) void layernorm_bwd_kernel(const LnTr
   // a workgroup by itself has the sums; the others' parts are added by the next launch
   float* out = p.part + (int64_t)blockIdx.x * 2 * C;
   const bool alone = p.part == nullptr;
-  if constexpr (TPR < 256) {
+  if constexpr (TPR <= 64) {
     const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int k = 0; k < NCH; ++k)
@@ -282,7 +292,10 @@ __global__ __launch_bounds__(1024) void layernorm_dw_kernel(const LnTrainBwdPara
 // registers of a thread (2^25 float32 elements, rows of 1024: two waves' halves with
 // four chunks 116 us, a wave with two 97; rows of 2048 beside bf16 branches: a wave
 // with four 71 us, two waves with two 64).  Backward: a thread keeps dw and db of its
-// channels over the rows, and rows inside a wave need no barrier: up to four chunks.
+// channels over the rows, and rows inside a wave need no barrier: up to four chunks,
+// two at odd widths, whose last chunk takes registers of its own (1001 channels of bf16:
+// half a wave with four 72 us, a wave with two 55); three for two waves from 2049
+// channels on, where four waves with two stood half idle (2560: 77 us, 61).
 // Rows of 64 channels by half waves, a quarter of the lanes at work, took 106 and 189
 // us where eight lanes a row take 42 and 63.
 template <typename TX, typename TB, template <typename, typename, int, int> class F, typename P>
@@ -299,45 +312,48 @@ hipError_t fwd_width(int n, const P& p, hipStream_t s) {
   if (n <= 2048) return F<TX, TB, 1024, 2>::run(p, s);
   return hipErrorInvalidValue;
 }
-template <typename TX, typename TB, template <typename, typename, int, int> class F, typename P>
-hipError_t bwd_width(int n, const P& p, hipStream_t s) {
-  if (n <= 8) return F<TX, TB, 8, 1>::run(p, s);
-  if (n <= 16) return F<TX, TB, 16, 1>::run(p, s);
-  if (n <= 32) return F<TX, TB, 32, 1>::run(p, s);
-  if (n <= 64) return F<TX, TB, 32, 2>::run(p, s);
-  if (n <= 96) return F<TX, TB, 32, 3>::run(p, s);
-  if (n <= 128) return F<TX, TB, 32, 4>::run(p, s);
-  if (n <= 192) return F<TX, TB, 64, 3>::run(p, s);
-  if (n <= 256) return F<TX, TB, 64, 4>::run(p, s);
-  if (n <= 512) return F<TX, TB, 256, 2>::run(p, s);
-  if (n <= 768) return F<TX, TB, 256, 3>::run(p, s);
-  if (n <= 1024) return F<TX, TB, 256, 4>::run(p, s);
-  if (n <= 2048) return F<TX, TB, 1024, 2>::run(p, s);
-  return hipErrorInvalidValue;
-}
-
 template <typename TX, typename TB, int TPR, int NCH> struct Fwd {
   static hipError_t run(const LnTrainParams& p, hipStream_t s) {
     constexpr int G = kGroups<TPR>;
-    hipLaunchKernelGGL((layernorm_fwd_kernel<TX, TB, TPR, NCH>), dim3((unsigned)((p.rows + G - 1) / G)), dim3(kThreads<TPR>),
-                       0, s, p);
+    const dim3 grid((unsigned)((p.rows + G - 1) / G)), wg(kThreads<TPR>);
+    hipLaunchKernelGGL((layernorm_fwd_kernel<TX, TB, TPR, NCH>), grid, wg, 0, s, p);
     return hipGetLastError();
   }
 };
-template <typename TX, typename TB, int TPR, int NCH> struct Bwd {
+template <typename TX, typename TB, int TPR, int NCH, bool WHOLE> struct Bwd {
   static hipError_t run(const LnTrainBwdParams& p, hipStream_t s) {
-    if (p.n_wg > 0)
-      hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TB, TPR, NCH>), dim3((unsigned)p.n_wg), dim3(kThreads<TPR>), 0, s, p);
+    const dim3 grid((unsigned)p.n_wg), wg(kThreads<TPR>);
+    if (p.n_wg > 0) hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TB, TPR, NCH, WHOLE>), grid, wg, 0, s, p);
     if ((p.dw || p.db) && p.n_wg != 1)
       hipLaunchKernelGGL(layernorm_dw_kernel, dim3((unsigned)((p.C + 31) / 32), 2), dim3(1024), 0, s, p, p.n_wg);
     return hipGetLastError();
   }
 };
 
+template <typename TX, typename TB, bool WHOLE>
+hipError_t bwd_width(int n, const LnTrainBwdParams& p, hipStream_t s) {
+  if (n <= 8) return Bwd<TX, TB, 8, 1, WHOLE>::run(p, s);
+  if (n <= 16) return Bwd<TX, TB, 16, 1, WHOLE>::run(p, s);
+  if (n <= 32) return Bwd<TX, TB, 32, 1, WHOLE>::run(p, s);
+  if (n <= 64) return Bwd<TX, TB, 32, 2, WHOLE>::run(p, s);
+  if (n <= 96) return Bwd<TX, TB, 32, 3, WHOLE>::run(p, s);
+  if (n <= 128) return Bwd<TX, TB, WHOLE ? 32 : 64, WHOLE ? 4 : 2, WHOLE>::run(p, s);
+  if (n <= 192) return Bwd<TX, TB, 64, 3, WHOLE>::run(p, s);
+  if (n <= 256) return Bwd<TX, TB, WHOLE ? 64 : 128, WHOLE ? 4 : 2, WHOLE>::run(p, s);
+  if (n <= 384) return Bwd<TX, TB, 128, 3, WHOLE>::run(p, s);
+  if (n <= 512) return Bwd<TX, TB, 256, 2, WHOLE>::run(p, s);
+  if (n <= 768) return Bwd<TX, TB, 256, 3, WHOLE>::run(p, s);
+  if (n <= 1024) return Bwd<TX, TB, 256, 4, WHOLE>::run(p, s);
+  if (n <= 2048) return Bwd<TX, TB, 1024, 2, WHOLE>::run(p, s);
+  return hipErrorInvalidValue;
+}
+
 template <typename TX, typename TB>
 hipError_t run(const LnTrainParams& p, hipStream_t s) { return fwd_width<TX, TB, Fwd>((p.C + 7) / 8, p, s); }
 template <typename TX, typename TB>
-hipError_t run(const LnTrainBwdParams& p, hipStream_t s) { return bwd_width<TX, TB, Bwd>((p.C + 7) / 8, p, s); }
+hipError_t run(const LnTrainBwdParams& p, hipStream_t s) {
+  return p.C % 8 == 0 ? bwd_width<TX, TB, true>(p.C / 8, p, s) : bwd_width<TX, TB, false>((p.C + 7) / 8, p, s);
+}
 
 template <typename P>
 hipError_t by_types(const P& p, int dtype, int branch, hipStream_t s) {
@@ -361,10 +377,12 @@ int layernorm_row_threads(int C) {
 // second launch (32 x 768: 9 us, 6 + 3 and the gap between in two; 4 x 8192 17 and 9).
 int layernorm_bwd_groups(int64_t rows, int C, int n_cu) {
   const int n = (C + 7) / 8;
-  const int per = n <= 8 ? 32 : (n <= 16 ? 16 : (n <= 128 ? 8 : (n <= 256 ? 4 : 1)));
+  const bool whole = C % 8 == 0;
+  const int waves = n > 1024 ? 16 : n > 384 ? 4 : n > (whole ? 256 : 192) ? 2 : 1;  // of a row that has several
+  const int per = waves > 1 ? 1 : n <= 8 ? 32 : n <= 16 ? 16 : n <= (whole ? 128 : 96) ? 8 : 4;
   const int64_t rounds = (rows + per - 1) / per;
-  if (rounds <= (n <= 256 ? 4 : 1)) return 1;
-  const int64_t most = (int64_t)n_cu * (n <= 1024 ? 2 : 1);
+  if (rounds <= (waves > 1 ? 1 : 4)) return 1;
+  const int64_t most = (int64_t)n_cu * (waves == 2 ? 4 : waves == 16 ? 1 : 2);
   return (int)(rounds < most ? rounds : most);
 }
 
