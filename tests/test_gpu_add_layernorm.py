@@ -1,6 +1,8 @@
 """kernel.add_layernorm against its definition in 64 bits, forward and backward,
 with the float32 error bounds of train_cases.norm_exact and one rounding of each
 result."""
+import math
+
 import pytest
 import torch
 
@@ -54,6 +56,27 @@ def test_widths_and_types(xt, yt, C):
     """Every layout of a row: eight lanes to four waves, 1 to 4 chunks a thread."""
     c = _case(37, C, xt, yt, yt if C % 2 else F32, delta=C % 3 != 0, bias=C % 4 != 0, seed=C)
     _check(**c, dtype=yt)
+
+
+def _among_nans(t, gap):
+    """t's values as rows gap apart, with NaNs between and around them."""
+    R, C = t.shape
+    buf = torch.full((R + 2, C + gap), math.nan, device=DEV, dtype=t.dtype)
+    view = buf[1:-1, gap // 2:gap // 2 + C]
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("xt,yt", [(BF16, BF16), (F32, BF16), (F32, F32)])
+@pytest.mark.parametrize("chunks", [8, 9, 20, 40, 80, 100, 150, 200, 256, 300, 450, 700, 900, 1100])
+def test_last_chunks(xt, yt, chunks):
+    """Every size of a last chunk in every layout, whole ones of the wider layouts too;
+    nothing of what lies around a row gets into it."""
+    for rest in range(8):
+        c = _case(9, 8 * chunks + rest, xt, yt, xt, seed=chunks + rest)
+        for k in ("x", "delta", "dy", "dr"):
+            c[k] = _among_nans(c[k], 5 + rest)
+        _check(**c, dtype=yt)
 
 
 @pytest.mark.parametrize("C", [8193, 16384])
