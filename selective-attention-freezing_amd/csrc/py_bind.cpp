@@ -53,11 +53,15 @@ void check(int rc) {
   TORCH_CHECK(false, last_error());
 }
 
+// dimensions that a descriptor has room for
+constexpr int kMaxDims = sizeof(saf_tensor_t::size) / sizeof(int64_t);
+
 saf_tensor_t desc(const char* what, const at::Tensor& x) {
   saf_tensor_t d{};
   if (!x.defined()) return d;
   const int code = dtype_code(x.scalar_type());
   TORCH_CHECK_NOT_IMPLEMENTED(code >= 0, what, ": unsupported dtype ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() <= kMaxDims, what, ": tensors have at most ", kMaxDims, " dimensions");
   d.data = x.data_ptr();
   d.dtype = code;
   d.ndim = (int32_t)x.dim();
@@ -147,7 +151,7 @@ PyObject* fill(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int code = dtype_code(x.scalar_type());
     if (code < 0)
       return PyErr_Format(PyExc_NotImplementedError, "%s: unsupported dtype %s", what, c10::toString(x.scalar_type()));
-    if (x.dim() > 4) return PyErr_Format(PyExc_ValueError, "%s: tensors have at most 4 dimensions", what);
+    if (x.dim() > kMaxDims) return PyErr_Format(PyExc_ValueError, "%s: tensors have at most %d dimensions", what, kMaxDims);
     if (rows >> i & 1 && !rows_ok(x)) {
       copies |= 1L << i;
       continue;

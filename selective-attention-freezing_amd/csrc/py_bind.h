@@ -31,7 +31,8 @@ bool has_tangent(const at::Tensor& x);
 // The exception of a status, with the library's message.
 void check(int rc);
 
-// saf_tensor_t of a tensor; an undefined one is absent.
+// saf_tensor_t of a tensor; an undefined one is absent, one of more dimensions than
+// a descriptor has is refused.
 saf_tensor_t desc(const char* what, const at::Tensor& x);
 
 // A leaf's autograd node belongs to the stream of the call that made it.  A

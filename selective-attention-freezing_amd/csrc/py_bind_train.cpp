@@ -100,6 +100,9 @@ void same_device(const char* what, const at::Tensor& x, const at::Tensor& as) {
   TORCH_CHECK(as.is_cuda(), what, " runs on HIP devices only (got a CPU tensor)");
   TORCH_CHECK_VALUE(x.device() == as.device(), what, ": a tensor is on ", x.device(), ", expected ", as.device());
 }
+void check_vector(const char* what, const char* name, const at::Tensor& x) {
+  TORCH_CHECK_VALUE(x.dim() == 1, what, ": ", name, " must be a (C,) vector (got ", x.sizes(), ")");
+}
 bool recorded(const at::Tensor& x) { return x.defined() && x.requires_grad() && at::GradMode::is_enabled(); }
 
 // ---- embed_tokens ----------------------------------------------------------------
@@ -339,8 +342,10 @@ PyObject* add_layernorm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   std::optional<at::Tensor> delta, bias;
   if (args[1] != Py_None) delta = tensor(kNorm, args[1]);
   if (args[3] != Py_None) bias = tensor(kNorm, args[3]);
-  same_device(kNorm, weight, x);
   TORCH_CHECK_VALUE(x.dim() >= 1, kNorm, ": x must have channels");
+  check_vector(kNorm, "weight", weight);
+  if (bias) check_vector(kNorm, "bias", *bias);
+  same_device(kNorm, weight, x);
   if (delta) {
     same_device(kNorm, *delta, x);
     TORCH_CHECK_VALUE(delta->sizes() == x.sizes(), kNorm, ": x and delta must share a shape (got ", x.sizes(), " and ",
