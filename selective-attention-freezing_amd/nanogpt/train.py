@@ -9,9 +9,11 @@ embedding, each residual addition fused with the LayerNorm behind it
 (``kernel.add_layernorm``), and the MLPs' activations kept in 8 bits for the
 backward pass (``kernel.mlp_packed``; ``packed=False`` keeps them whole).  Under
 autocast the residual stream has the weights' float32 and the branches the
-autocast dtype.
+autocast dtype.  An MLP that is not the model's own, or has another activation,
+adapted projections or hooks, is called as it is.
 """
 import torch
+import torch.nn as nn
 
 import kernel as _kernel_mod
 from kernel import _ext
@@ -44,9 +46,16 @@ def forward_hidden(model, idx, packed=True):
     return h
 
 
+def _stock(module, kind):
+    """Whether calling module computes kind's forward and nothing else: no subclass, no
+    forward of the instance's own, no hooks."""
+    return (type(module) is kind and "forward" not in vars(module)
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
 def _mlp(mlp, h, packed):
-    # a module of the caller's own, or another activation, runs as it is
-    if not packed or type(mlp) is not MLP or mlp.gelu.approximate != "none":
+    if not (packed and _stock(mlp, MLP) and _stock(mlp.c_fc, nn.Linear) and _stock(mlp.c_proj, nn.Linear)
+            and _stock(mlp.gelu, nn.GELU) and mlp.gelu.approximate == "none"):
         return mlp(h)
     return _kernel_mod.mlp_packed(h, mlp.c_fc.weight, mlp.c_proj.weight, mlp.c_fc.bias, mlp.c_proj.bias)
 

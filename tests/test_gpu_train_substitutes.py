@@ -1,0 +1,37 @@
+"""nanogpt.train with modules of the caller's own in the model against the model's own
+path, on the kernels: float32, the bounds of test_gpu_train_model.test_float32."""
+import pytest
+import torch
+import torch.nn as nn
+
+from nanogpt import train
+from test_gpu_train_model import _batch, _loss_and_grads, _model, _near
+from test_train_substitutes import _Adapter, _hook
+from train_cases import DEV
+
+pytestmark = pytest.mark.gpu
+
+
+def _same(m, packed):
+    idx, nxt = _batch(m)
+    a, ga = _loss_and_grads(m, lambda: m.token_logprobs(idx, nxt).logp)
+    b, gb = _loss_and_grads(m, lambda: train.token_logprobs(m, idx, nxt, packed=packed).logp)
+    assert (a - b).abs().max() <= 6e-4
+    _near(gb, ga, 0.1 if packed else 6e-4)
+    return ga
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_mlps(packed):
+    """One of the two layers stays packed where packed is asked for."""
+    m = _model()
+    m.transformer.h[0].mlp.gelu = nn.SiLU()
+    _same(m, packed)
+    m = _model()
+    mlp = m.transformer.h[1].mlp
+    mlp.c_fc, mlp.c_proj = _Adapter(mlp.c_fc).to(DEV), _Adapter(mlp.c_proj).to(DEV)
+    grads = _same(m, packed)
+    assert sum("down" in n or "up" in n for n in grads) == 4
+    m = _model()
+    m.transformer.h[0].mlp.c_fc.register_forward_hook(_hook)
+    _same(m, packed)

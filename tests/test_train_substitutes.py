@@ -1,0 +1,130 @@
+"""nanogpt.train with modules of the caller's own in the model: what they compute is
+part of the pass, as in GPT.forward_hidden (CPU: the fused operators in plain torch,
+so both paths are the same float32 operations)."""
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+import kernel
+from nanogpt import train
+from test_decode_cache import _model as _bare
+from test_model_substitutes import _Attention
+
+
+def _embed(tokens, weight, scale=1.0, ignore_index=-100, dtype=None):
+    skip, out = tokens == ignore_index, (tokens < 0) | (tokens >= weight.size(0))
+    y = F.embedding(tokens.clamp(0, weight.size(0) - 1), weight) * scale
+    return y.masked_fill(out[..., None], float("nan")).masked_fill(skip[..., None], 0.0)
+
+
+def _norm(x, delta, weight, bias=None, eps=1e-5, dtype=None):
+    r = x if delta is None else x + delta
+    return r, F.layer_norm(r, weight.shape, weight, bias, eps)
+
+
+def _mlp(x, w_fc, w_proj, b_fc=None, b_proj=None):
+    return F.linear(F.gelu(F.linear(x, w_fc, b_fc)), w_proj, b_proj)
+
+
+@pytest.fixture(autouse=True)
+def calls(monkeypatch):
+    """The operators in plain torch; the names of those that ran."""
+    made = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)   # asks for a device
+    for name, f in (("embed_tokens", _embed), ("add_layernorm", _norm), ("mlp_packed", _mlp)):
+        monkeypatch.setattr(kernel, name, lambda *a, _n=name, _f=f, **k: (made.append(_n), _f(*a, **k))[1])
+    return made
+
+
+def _model():
+    m = _bare()
+    torch.manual_seed(7)
+    for blk in m.transformer.h:
+        blk.attn = _Attention(blk.attn)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.add_(torch.randn_like(p) * 0.1)
+    return m
+
+
+IDX = torch.randint(0, 128, (2, 9), generator=torch.Generator().manual_seed(1))
+
+
+def _same(m, packed=True):
+    """Hidden states and every gradient of both paths."""
+    out = []
+    for f in (lambda: m.forward_hidden(IDX), lambda: train.forward_hidden(m, IDX, packed)):
+        m.zero_grad(set_to_none=True)
+        h = f()
+        (h * torch.linspace(-1, 1, h.numel()).view_as(h)).sum().backward()
+        out.append((h.detach(), {n: p.grad for n, p in m.named_parameters() if p.grad is not None}))
+    (a, ga), (b, gb) = out
+    assert torch.equal(a, b)
+    assert ga.keys() == gb.keys()
+    for n in ga:
+        # the same terms, added in another order at most
+        assert (ga[n] - gb[n]).norm() <= 1e-5 * ga[n].norm(), n
+    return ga
+
+
+class _Adapter(nn.Linear):
+    """A linear layer with a low-rank addition."""
+
+    def __init__(self, inner, rank=3):
+        super().__init__(inner.in_features, inner.out_features, inner.bias is not None)
+        self.weight, self.bias = inner.weight, inner.bias
+        self.down = nn.Parameter(torch.randn(rank, inner.in_features) * 0.1)
+        self.up = nn.Parameter(torch.randn(inner.out_features, rank) * 0.1)
+
+    def forward(self, x):
+        return super().forward(x) + x @ self.down.t() @ self.up.t()
+
+
+def _hook(module, args, out):
+    return out * 1.5
+
+
+def _pre_hook(module, args):
+    return (args[0] * 0.5,)
+
+
+def test_plain_model_is_fused(calls):
+    m = _model()
+    _same(m)
+    assert calls == ["embed_tokens"] + ["add_layernorm", "add_layernorm", "mlp_packed"] * 2 + ["add_layernorm"]
+
+
+# ---- inside the MLP ---------------------------------------------------------------
+
+@pytest.mark.parametrize("act", [nn.SiLU(), nn.ReLU(), nn.Identity(), nn.GELU(approximate="tanh")], ids=lambda a: str(a))
+def test_activations(act, calls):
+    m = _model()
+    m.transformer.h[0].mlp.gelu = act
+    _same(m)
+    assert calls.count("mlp_packed") == 1
+
+
+@pytest.mark.parametrize("name", ["c_fc", "c_proj"])
+def test_adapted_projections(name, calls):
+    m = _model()
+    mlp = m.transformer.h[1].mlp
+    setattr(mlp, name, _Adapter(getattr(mlp, name)))
+    grads = _same(m)
+    assert {f"transformer.h.1.mlp.{name}.{p}" for p in ("weight", "down", "up")} <= grads.keys()
+    assert calls.count("mlp_packed") == 1
+
+
+@pytest.mark.parametrize("name", ["", "c_fc", "gelu", "c_proj"])
+def test_hooked_mlps(name, calls):
+    for add in (lambda t: t.register_forward_hook(_hook), lambda t: t.register_forward_pre_hook(_pre_hook),
+                lambda t: t.register_full_backward_hook(lambda *a: (a[1][0] * 2,))):
+        m = _model()
+        add(m.transformer.h[1].mlp.get_submodule(name))
+        _same(m)
+    m = _model()
+    target = m.transformer.h[1].mlp.get_submodule(name)
+    own = target.forward
+    target.forward = lambda x: own(x) * 0.25
+    _same(m)
+    assert calls.count("mlp_packed") == 4
