@@ -9,15 +9,15 @@ embedding, each residual addition fused with the LayerNorm behind it
 (``kernel.add_layernorm``), and the MLPs' activations kept in 8 bits for the
 backward pass (``kernel.mlp_packed``; ``packed=False`` keeps them whole).  Under
 autocast the residual stream has the weights' float32 and the branches the
-autocast dtype.  An MLP that is not the model's own, or has another activation,
-adapted projections or hooks, is called as it is.
+autocast dtype.  A norm or an MLP that is not the model's own, or has hooks, another
+activation or adapted projections, is called as it is.
 """
 import torch
 import torch.nn as nn
 
 import kernel as _kernel_mod
 from kernel import _ext
-from nanogpt.model import MLP
+from nanogpt.model import MLP, LayerNorm
 
 
 def forward_hidden(model, idx, packed=True):
@@ -37,13 +37,12 @@ def forward_hidden(model, idx, packed=True):
         x = x + tr.wpe(torch.arange(T, device=idx.device))
     else:
         rope = model.rotary(T, dtype)
-    ln = tr.h[0].ln_1
-    h = _kernel_mod.add_layernorm(x, None, ln.weight, ln.bias, dtype=dtype)[1]
-    for i, block in enumerate(tr.h):
-        x, h = _kernel_mod.add_layernorm(x, block.attn(h, rope=rope), block.ln_2.weight, block.ln_2.bias)
-        ln = tr.h[i + 1].ln_1 if i + 1 < len(tr.h) else tr.ln_f
-        x, h = _kernel_mod.add_layernorm(x, _mlp(block.mlp, h, packed), ln.weight, ln.bias)
-    return h
+    d = None                                     # what is not yet added to the residual
+    for block in tr.h:
+        x, h = _norm(block.ln_1, x, d, dtype)
+        x, h = _norm(block.ln_2, x, block.attn(h, rope=rope), dtype)
+        d = _mlp(block.mlp, h, packed)
+    return _norm(tr.ln_f, x, d, dtype)[1]
 
 
 def _stock(module, kind):
@@ -51,6 +50,14 @@ def _stock(module, kind):
     forward of the instance's own, no hooks."""
     return (type(module) is kind and "forward" not in vars(module)
             and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
+def _norm(ln, x, d, dtype):
+    """(x + d, ln of it); without d the norm of x in dtype."""
+    if not _stock(ln, LayerNorm):
+        x = x if d is None else x + d
+        return x, ln(x)
+    return _kernel_mod.add_layernorm(x, d, ln.weight, ln.bias, dtype=dtype if d is None else None)
 
 
 def _mlp(mlp, h, packed):

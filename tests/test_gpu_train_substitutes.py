@@ -35,3 +35,30 @@ def test_mlps(packed):
     m = _model()
     m.transformer.h[0].mlp.c_fc.register_forward_hook(_hook)
     _same(m, packed)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_norms(packed):
+    m = _model()
+    m.transformer.h[0].ln_1 = nn.LayerNorm(128, eps=0.5).to(DEV)
+    m.transformer.h[1].ln_2 = nn.LayerNorm(128, eps=0.5).to(DEV)
+    _same(m, packed)
+    m = _model()
+    m.transformer.ln_f = nn.LayerNorm(128, eps=0.5).to(DEV)
+    m.transformer.h[0].ln_2.register_forward_hook(_hook)
+    _same(m, packed)
+
+
+def test_norms_under_autocast():
+    """float32 norms of the caller's own between bf16 branches (the bound of
+    test_gpu_train_model.test_autocast)."""
+    m = _model(frozen=False)
+    m.transformer.h[1].ln_1 = nn.LayerNorm(128, eps=0.5).to(DEV)
+    m.transformer.ln_f = nn.LayerNorm(128, eps=0.5).to(DEV)
+    idx, nxt = _batch(m)
+    a, ga = _loss_and_grads(m, lambda: m.token_logprobs(idx, nxt).logp)
+    with torch.autocast("cuda", torch.bfloat16):
+        _, own = _loss_and_grads(m, lambda: m.token_logprobs(idx, nxt).logp)
+        b, gb = _loss_and_grads(m, lambda: train.token_logprobs(m, idx, nxt, packed=False).logp)
+    assert (a - b).abs().max() <= 10 * 2.0 ** -8 * 4
+    _near(gb, ga, 10 * 2.0 ** -8, own)

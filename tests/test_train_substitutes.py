@@ -128,3 +128,39 @@ def test_hooked_mlps(name, calls):
     target.forward = lambda x: own(x) * 0.25
     _same(m)
     assert calls.count("mlp_packed") == 4
+
+
+# ---- the norms --------------------------------------------------------------------
+
+class _RMSNorm(nn.Module):
+    def __init__(self, n):
+        super().__init__()
+        self.gain = nn.Parameter(torch.linspace(0.5, 1.5, n))
+
+    def forward(self, x):
+        return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-3) * self.gain
+
+
+def _owner(m, name):
+    return m.transformer if name == "ln_f" else m.transformer.h[1]
+
+
+@pytest.mark.parametrize("name", ["ln_1", "ln_2", "ln_f"])
+@pytest.mark.parametrize("other", [lambda: nn.LayerNorm(128, eps=0.5), lambda: _RMSNorm(128),
+                                   lambda: nn.LayerNorm(128, elementwise_affine=False), nn.Identity],
+                         ids=["eps", "rms", "bare", "none"])
+def test_other_norms(name, other, calls):
+    m = _model()
+    _owner(m, name).add_module(name, other())
+    _same(m)
+    assert calls.count("add_layernorm") == 4
+
+
+@pytest.mark.parametrize("name", ["ln_1", "ln_2", "ln_f"])
+def test_hooked_norms(name, calls):
+    for add in (lambda t: t.register_forward_hook(_hook), lambda t: t.register_forward_pre_hook(_pre_hook),
+                lambda t: t.register_full_backward_hook(lambda *a: (a[1][0] * 2,))):
+        m = _model()
+        add(getattr(_owner(m, name), name))
+        _same(m)
+    assert calls.count("add_layernorm") == 12
