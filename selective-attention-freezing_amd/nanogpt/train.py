@@ -9,15 +9,15 @@ embedding, each residual addition fused with the LayerNorm behind it
 (``kernel.add_layernorm``), and the MLPs' activations kept in 8 bits for the
 backward pass (``kernel.mlp_packed``; ``packed=False`` keeps them whole).  Under
 autocast the residual stream has the weights' float32 and the branches the
-autocast dtype.  A norm or an MLP that is not the model's own, or has hooks, another
-activation or adapted projections, is called as it is.
+autocast dtype.  A block, norm or MLP that is not the model's own, or has hooks,
+another activation or adapted projections, is called as it is.
 """
 import torch
 import torch.nn as nn
 
 import kernel as _kernel_mod
 from kernel import _ext
-from nanogpt.model import MLP, LayerNorm
+from nanogpt.model import MLP, Block, LayerNorm
 
 
 def forward_hidden(model, idx, packed=True):
@@ -39,6 +39,9 @@ def forward_hidden(model, idx, packed=True):
         rope = model.rotary(T, dtype)
     d = None                                     # what is not yet added to the residual
     for block in tr.h:
+        if not _stock(block, Block):
+            x, d = block(x if d is None else x + d, rope=rope), None
+            continue
         x, h = _norm(block.ln_1, x, d, dtype)
         x, h = _norm(block.ln_2, x, block.attn(h, rope=rope), dtype)
         d = _mlp(block.mlp, h, packed)

@@ -6,7 +6,7 @@ import torch.nn as nn
 
 from nanogpt import train
 from test_gpu_train_model import _batch, _loss_and_grads, _model, _near
-from test_train_substitutes import _Adapter, _hook
+from test_train_substitutes import _Adapter, _hook, _Scaled, _Wrapper
 from train_cases import DEV
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +62,17 @@ def test_norms_under_autocast():
         b, gb = _loss_and_grads(m, lambda: train.token_logprobs(m, idx, nxt, packed=False).logp)
     assert (a - b).abs().max() <= 10 * 2.0 ** -8 * 4
     _near(gb, ga, 10 * 2.0 ** -8, own)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("kind", [_Scaled, _Wrapper])
+def test_blocks(kind, packed):
+    """A block of the caller's own before and behind one that is fused."""
+    for at in (0, 1):
+        m = _model()
+        blocks = m.transformer.h
+        if kind is _Scaled:
+            blocks[at].__class__ = _Scaled
+        else:
+            blocks[at] = _Wrapper(blocks[at]).to(DEV)
+        _same(m, packed)

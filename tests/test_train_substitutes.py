@@ -8,6 +8,7 @@ import torch.nn.functional as F
 
 import kernel
 from nanogpt import train
+from nanogpt.model import Block
 from test_decode_cache import _model as _bare
 from test_model_substitutes import _Attention
 
@@ -164,3 +165,52 @@ def test_hooked_norms(name, calls):
         add(getattr(_owner(m, name), name))
         _same(m)
     assert calls.count("add_layernorm") == 12
+
+
+# ---- blocks -----------------------------------------------------------------------
+
+class _Scaled(Block):
+    def forward(self, x, rope=None, **sink):
+        return x + 0.5 * (super().forward(x, rope=rope, **sink) - x)
+
+
+class _Wrapper(nn.Module):
+    """A block without the names of Block's parts."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner, self.gain = inner, nn.Parameter(torch.tensor(0.7))
+
+    def forward(self, x, rope=None):
+        return self.inner(x, rope=rope) * self.gain
+
+
+@pytest.mark.parametrize("at", [(0,), (1,), (0, 1)])
+def test_other_blocks(at, calls):
+    def scaled(m, i):
+        m.transformer.h[i].__class__ = _Scaled
+
+    def wrapped(m, i):
+        m.transformer.h[i] = _Wrapper(m.transformer.h[i])
+
+    def hooked(m, i):
+        m.transformer.h[i].register_forward_hook(_hook)
+
+    def own_forward(m, i):
+        blk = m.transformer.h[i]
+        was = blk.forward
+        blk.forward = lambda x, **k: was(x, **k) * 2
+
+    for change in (scaled, wrapped, hooked, own_forward):
+        m = _model()
+        for i in at:
+            change(m, i)
+        grads = _same(m)
+        assert change is not wrapped or {f"transformer.h.{i}.gain" for i in at} <= grads.keys()
+    assert calls.count("mlp_packed") == 4 * (2 - len(at))
+
+
+def test_no_blocks():
+    m = _model()
+    m.transformer.h = nn.ModuleList()
+    _same(m)
