@@ -9,8 +9,9 @@ embedding, each residual addition fused with the LayerNorm behind it
 (``kernel.add_layernorm``), and the MLPs' activations kept in 8 bits for the
 backward pass (``kernel.mlp_packed``; ``packed=False`` keeps them whole).  Under
 autocast the residual stream has the weights' float32 and the branches the
-autocast dtype.  A block, norm or MLP that is not the model's own, or has hooks,
-another activation or adapted projections, is called as it is.
+autocast dtype.  An embedding, block, norm or MLP that is not the model's own, or
+has hooks, other options, another activation or adapted projections, is called as
+it is.
 """
 import torch
 import torch.nn as nn
@@ -27,7 +28,7 @@ def forward_hidden(model, idx, packed=True):
     if T > model.config.block_size:
         raise ValueError(f"sequences of {T} tokens exceed the model's block size {model.config.block_size}")
     tr = model.transformer
-    x = _kernel_mod.embed_tokens(idx, tr.wte.weight)
+    x = _embed(tr.wte, idx)
     if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
         # weights of torch's own operators as well, which would not refuse the capture
         _ext.bind().check_differentiable("nanogpt.train", *model.parameters())
@@ -53,6 +54,13 @@ def _stock(module, kind):
     forward of the instance's own, no hooks."""
     return (type(module) is kind and "forward" not in vars(module)
             and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
+def _embed(wte, idx):
+    if not _stock(wte, nn.Embedding) or wte.padding_idx is not None or wte.max_norm is not None \
+            or wte.scale_grad_by_freq or wte.sparse:
+        return wte(idx)
+    return _kernel_mod.embed_tokens(idx, wte.weight)
 
 
 def _norm(ln, x, d, dtype):

@@ -76,3 +76,16 @@ def test_blocks(kind, packed):
         else:
             blocks[at] = _Wrapper(blocks[at]).to(DEV)
         _same(m, packed)
+
+
+def test_embeddings():
+    m = _model()
+    m.transformer.wte = nn.Sequential(nn.Embedding(211, 16), nn.Linear(16, 128)).to(DEV)
+    _same(m, True)
+    m = _model()
+    m.transformer.wte.weight = nn.Parameter(m.transformer.wte.weight.detach().clone())
+    m.transformer.wte.padding_idx = 5
+    idx, _ = _batch(m)
+    assert (idx == 5).any()
+    grads = _same(m, True)
+    assert not grads["transformer.wte.weight"][5].any()

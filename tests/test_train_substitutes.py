@@ -214,3 +214,54 @@ def test_no_blocks():
     m = _model()
     m.transformer.h = nn.ModuleList()
     _same(m)
+
+
+# ---- the embedding ----------------------------------------------------------------
+
+class _Embedding(nn.Embedding):
+    def forward(self, idx):
+        return super().forward(idx) * 1.5
+
+
+def test_other_embeddings(calls):
+    def subclass(m):
+        m.transformer.wte.__class__ = _Embedding
+
+    def replaced(m):
+        m.transformer.wte = nn.Sequential(nn.Embedding(128, 16), nn.Linear(16, 128))
+
+    def padded(m):
+        m.transformer.wte.padding_idx = int(IDX[0, 3])       # a row without gradient
+
+    def by_frequency(m):
+        m.transformer.wte.scale_grad_by_freq = True
+
+    def hooked(m):
+        m.transformer.wte.register_forward_hook(_hook)
+
+    for change in (subclass, replaced, padded, by_frequency, hooked):
+        m = _model()
+        # beside the head's weight, whose gradient would be the sum of both
+        m.transformer.wte.weight = nn.Parameter(m.transformer.wte.weight.detach().clone())
+        change(m)
+        grads = _same(m)
+        if change is padded:
+            assert not grads["transformer.wte.weight"][int(IDX[0, 3])].any()
+    assert "embed_tokens" not in calls
+
+
+def test_renormalised_embedding(calls):
+    """max_norm changes the weight in place; without a gradient, as nn.Embedding asks."""
+    m = _model()
+    m.transformer.wte.max_norm = 0.25
+    m.transformer.wte.weight.requires_grad_(False)
+    _same(m)
+    assert m.transformer.wte.weight[IDX[0, 0]].norm() <= 0.2501 and "embed_tokens" not in calls
+
+
+def test_sparse_embedding(calls):
+    m = _model()
+    m.transformer.wte.weight = nn.Parameter(m.transformer.wte.weight.detach().clone())
+    m.transformer.wte.sparse = True
+    train.forward_hidden(m, IDX).sum().backward()
+    assert m.transformer.wte.weight.grad.is_sparse and "embed_tokens" not in calls
