@@ -11,14 +11,14 @@ backward pass (``kernel.mlp_packed``; ``packed=False`` keeps them whole).  Under
 autocast the residual stream has the weights' float32 and the branches the
 autocast dtype.  An embedding, block, norm or MLP that is not the model's own, or
 has hooks, other options, another activation or adapted projections, is called as
-it is.
+it is, and so are the model's own methods where a subclass has other ones.
 """
 import torch
 import torch.nn as nn
 
 import kernel as _kernel_mod
 from kernel import _ext
-from nanogpt.model import MLP, Block, LayerNorm
+from nanogpt.model import GPT, MLP, Block, LayerNorm
 
 
 def forward_hidden(model, idx, packed=True):
@@ -27,17 +27,12 @@ def forward_hidden(model, idx, packed=True):
     T = idx.size(1)
     if T > model.config.block_size:
         raise ValueError(f"sequences of {T} tokens exceed the model's block size {model.config.block_size}")
-    tr = model.transformer
-    x = _embed(tr.wte, idx)
     if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
         # weights of torch's own operators as well, which would not refuse the capture
         _ext.bind().check_differentiable("nanogpt.train", *model.parameters())
-    dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
-    rope = None
-    if model.rotary is None:
-        x = x + tr.wpe(torch.arange(T, device=idx.device))
-    else:
-        rope = model.rotary(T, dtype)
+    x, rope = model.prepare_inputs(idx) if _own(model, "prepare_inputs") else _inputs(model, idx)
+    dtype = _branch_dtype(x)
+    tr = model.transformer
     d = None                                     # what is not yet added to the residual
     for block in tr.h:
         if not _stock(block, Block):
@@ -54,6 +49,24 @@ def _stock(module, kind):
     forward of the instance's own, no hooks."""
     return (type(module) is kind and "forward" not in vars(module)
             and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
+def _own(model, name):
+    """Whether a model has a method of its own in place of GPT's."""
+    return name in vars(model) or getattr(type(model), name, None) not in (None, getattr(GPT, name))
+
+
+def _branch_dtype(x):
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+
+
+def _inputs(model, idx):
+    """GPT.prepare_inputs on embed_tokens."""
+    tr, T = model.transformer, idx.size(1)
+    x = _embed(tr.wte, idx)
+    if model.rotary is None:
+        return x + tr.wpe(torch.arange(T, device=idx.device)), None
+    return x, model.rotary(T, _branch_dtype(x))
 
 
 def _embed(wte, idx):
@@ -81,4 +94,8 @@ def _mlp(mlp, h, packed):
 def token_logprobs(model, idx, tokens, packed=True, **kw):
     """Log probabilities of tokens (B, T) as the next tokens of idx (B, T), with
     kernel.token_logprobs' options; -logp.mean() is the training loss."""
-    return _kernel_mod.token_logprobs(model.lm_head(forward_hidden(model, idx, packed)), tokens, **kw)
+    if _own(model, "forward_all_positions"):
+        logits = model.forward_all_positions(idx)
+    else:
+        logits = model.lm_head(model.forward_hidden(idx) if _own(model, "forward_hidden") else forward_hidden(model, idx, packed))
+    return _kernel_mod.token_logprobs(logits, tokens, **kw)

@@ -8,7 +8,7 @@ import torch.nn.functional as F
 
 import kernel
 from nanogpt import train
-from nanogpt.model import Block
+from nanogpt.model import GPT, Block
 from test_decode_cache import _model as _bare
 from test_model_substitutes import _Attention
 
@@ -265,3 +265,43 @@ def test_sparse_embedding(calls):
     m.transformer.wte.sparse = True
     train.forward_hidden(m, IDX).sum().backward()
     assert m.transformer.wte.weight.grad.is_sparse and "embed_tokens" not in calls
+
+
+# ---- the model --------------------------------------------------------------------
+
+class _Inputs(GPT):
+    def prepare_inputs(self, idx):
+        x, rope = super().prepare_inputs(idx)
+        return x * 2, rope
+
+
+class _Hidden(GPT):
+    def forward_hidden(self, idx, sinks=None):
+        return super().forward_hidden(idx, sinks) * 2
+
+
+class _Logits(GPT):
+    def forward_all_positions(self, idx):
+        return super().forward_all_positions(idx) * 2
+
+
+def test_inputs_of_the_model(calls):
+    m = _model()
+    m.__class__ = _Inputs
+    _same(m)
+    assert "embed_tokens" not in calls
+
+
+class _Fused(GPT):
+    """The pass as the model's own hidden states."""
+
+    def forward_hidden(self, idx, sinks=None):
+        return train.forward_hidden(self, idx)
+
+
+@pytest.mark.parametrize("kind", [GPT, _Inputs, _Logits, _Hidden, _Fused])
+def test_logits_of_the_model(kind, monkeypatch):
+    monkeypatch.setattr(kernel, "token_logprobs", lambda logits, tokens, **kw: logits)
+    m = _model()
+    m.__class__ = kind
+    assert torch.equal(train.token_logprobs(m, IDX, IDX), m.token_logprobs(IDX, IDX))
