@@ -23,7 +23,8 @@ from nanogpt.model import GPT, MLP, Block, LayerNorm
 
 def forward_hidden(model, idx, packed=True):
     """Hidden states (B, T, C) of every position behind the last norm,
-    differentiable in every parameter of the model that the tokens reach."""
+    differentiable in every parameter of the model that the tokens reach.  A token
+    outside the vocabulary, -100 included, makes its sequence NaN."""
     T = idx.size(1)
     if T > model.config.block_size:
         raise ValueError(f"sequences of {T} tokens exceed the model's block size {model.config.block_size}")
@@ -73,7 +74,8 @@ def _embed(wte, idx):
     if not _stock(wte, nn.Embedding) or wte.padding_idx is not None or wte.max_norm is not None \
             or wte.scale_grad_by_freq or wte.sparse:
         return wte(idx)
-    return _kernel_mod.embed_tokens(idx, wte.weight)
+    # no token of a batch is padding: one outside the vocabulary gives NaNs, not zeros
+    return _kernel_mod.embed_tokens(idx, wte.weight, ignore_index=-2 ** 63)
 
 
 def _norm(ln, x, d, dtype):

@@ -89,3 +89,17 @@ def test_embeddings():
     assert (idx == 5).any()
     grads = _same(m, True)
     assert not grads["transformer.wte.weight"][5].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+@pytest.mark.parametrize("bad", [-100, 211])
+def test_tokens_outside_the_vocabulary(bad, dtype):
+    """What such a token reaches is NaN, and the loss with it; the other sequences are
+    as they were."""
+    m = _model(frozen=False)
+    idx, nxt = _batch(m)
+    want = train.token_logprobs(m, idx, nxt).logp.detach()
+    idx[1, 60] = bad
+    got = train.token_logprobs(m, idx.to(dtype), nxt).logp.detach()
+    assert got[1, 60:].isnan().all()
+    assert torch.equal(got[::2], want[::2])

@@ -305,3 +305,15 @@ def test_logits_of_the_model(kind, monkeypatch):
     m = _model()
     m.__class__ = kind
     assert torch.equal(train.token_logprobs(m, IDX, IDX), m.token_logprobs(IDX, IDX))
+
+
+# ---- tokens -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("bad", [-100, -1, 128, 1 - 2 ** 63, 2 ** 63 - 1])
+def test_tokens_outside_the_vocabulary(bad):
+    """No row of zeros for any of them: the sequence is NaN and the others as they are."""
+    m = _model()
+    idx = IDX.clone()
+    idx[1, 4] = bad
+    h, want = train.forward_hidden(m, idx), train.forward_hidden(m, IDX)
+    assert h[1, 4].isnan().all() and torch.equal(h[0], want[0])
