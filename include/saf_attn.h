@@ -519,7 +519,8 @@ int saf_act_pack(const saf_tensor_t* x, const saf_tensor_t* q, const saf_tensor_
  * had.  out may have any row stride. */
 int saf_act_unpack(const saf_tensor_t* q, const saf_tensor_t* exp, const saf_tensor_t* out, void* stream);
 
-/* y = x Phi(x) (the exact GELU) and x in 8 bits, in one pass. */
+/* y = x Phi(x) (the exact GELU) and x in 8 bits, in one pass; without q and exp (both
+ * absent) y alone. */
 int saf_gelu_pack_fwd(const saf_tensor_t* x, const saf_tensor_t* y, const saf_tensor_t* q, const saf_tensor_t* exp,
                       void* stream);
 

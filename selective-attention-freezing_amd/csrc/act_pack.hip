@@ -13,7 +13,7 @@
 //   gelu'(h) = Phi(h) + h phi(h), from the held h;  du = dy gelu'(h)
 //
 // The kernels move bytes: per 16-bit element 3 + 1/32 (pack, unpack), 5 + 1/32 (GELU,
-// either way).  A thread has 8 channels, four threads a block: its largest magnitude
+// either way), 4 for the GELU alone, where no backward pass will read the 8 bits.  A thread has 8 channels, four threads a block: its largest magnitude
 // takes two lane exchanges inside the quad.  16384 x 2048 bf16: 18 us to pack, 17 to
 // unpack (5.6 and 6.0 TB/s; a copy reaches 5.2); the GELU of 16384 x 8192 110 to 140
 // us forward, 120 to 150 backward (4.8 to 6.1 and 4.5 to 5.6 TB/s, by where its 700 MB
@@ -142,8 +142,8 @@ __device__ inline void store_q8(int8_t* row, int c, int C, u32x2_any q) {
   }
 }
 
-// Forward: x packed; with GELU also y = gelu(x).
-template <typename T, bool GELU>
+// Forward: x packed (KEEP), y = gelu(x) (GELU).
+template <typename T, bool KEEP, bool GELU>
 __global__ __launch_bounds__(256) void act_pack_kernel(const ActPackParams p) {
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;
   if (i >= p.units) return;  // units is a multiple of four: a quad leaves together
@@ -151,10 +151,12 @@ __global__ __launch_bounds__(256) void act_pack_kernel(const ActPackParams p) {
   const int c = 8 * (int)k, C = p.C;
   float f[8];
   load_row8(reinterpret_cast<const T*>(p.x) + (int64_t)row * p.x_rs, c, C, f);
-  u32x2_any q;
-  const uint32_t byte = pack8(f, q);
-  store_q8(p.q + (int64_t)row * C, c, C, q);
-  if ((k & 3) == 0) p.exp[(int64_t)row * (p.per_row.d >> 2) + (k >> 2)] = (uint8_t)byte;
+  if constexpr (KEEP) {
+    u32x2_any q;
+    const uint32_t byte = pack8(f, q);
+    store_q8(p.q + (int64_t)row * C, c, C, q);
+    if ((k & 3) == 0) p.exp[(int64_t)row * (p.per_row.d >> 2) + (k >> 2)] = (uint8_t)byte;
+  }
   if constexpr (GELU) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -203,9 +205,10 @@ template <typename T>
 hipError_t launch_t(const ActPackParams& p, ActPackOp op, hipStream_t s) {
   const dim3 grid((p.units + 255) / 256), wg(256);
   switch (op) {
-    case ActPackOp::kPack: hipLaunchKernelGGL((act_pack_kernel<T, false>), grid, wg, 0, s, p); break;
+    case ActPackOp::kPack: hipLaunchKernelGGL((act_pack_kernel<T, true, false>), grid, wg, 0, s, p); break;
     case ActPackOp::kUnpack: hipLaunchKernelGGL((act_unpack_kernel<T>), grid, wg, 0, s, p); break;
-    case ActPackOp::kGelu: hipLaunchKernelGGL((act_pack_kernel<T, true>), grid, wg, 0, s, p); break;
+    case ActPackOp::kGelu: hipLaunchKernelGGL((act_pack_kernel<T, true, true>), grid, wg, 0, s, p); break;
+    case ActPackOp::kGeluOnly: hipLaunchKernelGGL((act_pack_kernel<T, false, true>), grid, wg, 0, s, p); break;
     case ActPackOp::kGeluBwd: hipLaunchKernelGGL((gelu_pack_bwd_kernel<T>), grid, wg, 0, s, p); break;
   }
   return hipGetLastError();

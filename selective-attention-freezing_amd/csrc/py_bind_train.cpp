@@ -255,8 +255,10 @@ constexpr const char* kGelu = "gelu_packed";
 struct Packed {
   at::Tensor q, exp;
 };
-Packed packed_like(const at::Tensor& x) {
+void check_channels(const at::Tensor& x) {
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "an activation has at least one channel");
+}
+Packed packed_like(const at::Tensor& x) {
   auto sizes = x.sizes().vec();
   sizes.back() = (sizes.back() + 31) / 32;
   return {at::empty(x.sizes(), plain(x).dtype(at::kChar)), at::empty(sizes, plain(x).dtype(at::kByte))};
@@ -266,9 +268,10 @@ struct GeluOutputs {
   at::Tensor y;
   Packed p;
 };
-GeluOutputs gelu_forward(const at::Tensor& x) {
+GeluOutputs gelu_forward(const at::Tensor& x, bool keep) {
   const c10::hip::HIPGuard guard(x.get_device());
-  GeluOutputs g{at::empty(x.sizes(), plain(x)), packed_like(x)};
+  check_channels(x);
+  GeluOutputs g{at::empty(x.sizes(), plain(x)), keep ? packed_like(x) : Packed{}};
   const at::Tensor x2 = rows(x);
   const saf_tensor_t xd = rows_desc(kGelu, x2), yd = rows_desc(kGelu, g.y), qd = rows_desc(kGelu, g.p.q),
                      ed = rows_desc(kGelu, g.p.exp);
@@ -287,7 +290,7 @@ std::pair<at::Tensor, at::Tensor> gelu_backward(const at::Tensor& q, const at::T
 
 struct GeluPacked : public torch::autograd::Function<GeluPacked> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x) {
-    const GeluOutputs g = gelu_forward(x);
+    const GeluOutputs g = gelu_forward(x, true);
     ctx->save_for_backward({g.p.q, g.p.exp});
     ctx->set_materialize_grads(false);
     return {g.y};
@@ -379,10 +382,10 @@ PyObject* gelu_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   same_device(kGelu, x, x);
   if (PyObject_IsTrue(args[1]) == 1) {
     at::NoGradGuard no_grad;
-    const GeluOutputs g = gelu_forward(x);
+    const GeluOutputs g = gelu_forward(x, true);
     return wrap_all({g.y, g.p.q, g.p.exp});
   }
-  if (!recorded(x)) return wrap(gelu_forward(x).y);
+  if (!recorded(x)) return wrap(gelu_forward(x, false).y);
   refuse_foreign_capture(kGelu, "activations", x);
   return wrap(GeluPacked::apply(x)[0]);
   END_HANDLE_TH_ERRORS
@@ -408,6 +411,7 @@ PyObject* pack_activation(PyObject*, PyObject* const* args, Py_ssize_t n) {
   same_device(what, x, x);
   TORCH_CHECK_NOT_IMPLEMENTED(!recorded(x), what, " has no backward: call it under torch.no_grad()");
   const c10::hip::HIPGuard guard(x.get_device());
+  check_channels(x);
   const Packed p = packed_like(x);
   const at::Tensor x2 = rows(x);
   const saf_tensor_t xd = rows_desc(what, x2), qd = rows_desc(what, p.q), ed = rows_desc(what, p.exp);

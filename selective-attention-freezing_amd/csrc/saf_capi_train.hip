@@ -126,21 +126,23 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int64_t C) {
 // ---- 8-bit activations ------------------------------------------------------------
 
 int pack_params(const char* what, const saf_tensor_t* x, const char* x_name, const saf_tensor_t* q, const saf_tensor_t* exp,
-                ActPackParams& p) {
+                ActPackParams& p, bool held = true) {
   if (int rc = check_float(x, x_name)) return rc;
   if (x->ndim != 2) return fail(SAF_EINVAL, "%s must be 2-D (rows, C)", x_name);
   const int64_t R = x->size[0], C = x->size[1];
   if (C < 1 || C > kMaxC) return fail(SAF_EUNSUPPORTED, "%s: C = %lld is not supported (1 to 2^23)", what, (long long)C);
   if (int rc = check_rows(x, x_name, R, C, false)) return rc;
   const int64_t nb = (C + 31) / 32;
-  if (int rc = check_rows(q, "q", R, C, true)) return rc;
-  if (int rc = check_rows(exp, "exp", R, nb, true)) return rc;
-  if (q->dtype != SAF_I8 || exp->dtype != SAF_U8) return fail(SAF_EINVAL, "q must be int8 and exp uint8");
+  if (held) {
+    if (int rc = check_rows(q, "q", R, C, true)) return rc;
+    if (int rc = check_rows(exp, "exp", R, nb, true)) return rc;
+    if (q->dtype != SAF_I8 || exp->dtype != SAF_U8) return fail(SAF_EINVAL, "q must be int8 and exp uint8");
+    p.q = reinterpret_cast<int8_t*>(q->data);
+    p.exp = reinterpret_cast<uint8_t*>(exp->data);
+  }
   if (int rc = units_of(what, R, 4 * nb, p.per_row, p.units)) return rc;
   p.x = x->data;
   p.x_rs = x->stride[0];
-  p.q = reinterpret_cast<int8_t*>(q->data);
-  p.exp = reinterpret_cast<uint8_t*>(exp->data);
   p.C = (int)C;
   return SAF_OK;
 }
@@ -374,12 +376,13 @@ int saf_act_unpack(const saf_tensor_t* q, const saf_tensor_t* exp, const saf_ten
 int saf_gelu_pack_fwd(const saf_tensor_t* x, const saf_tensor_t* y, const saf_tensor_t* q, const saf_tensor_t* exp,
                       void* stream) {
   ActPackParams p{};
-  if (int rc = pack_params("gelu_pack", x, "x", q, exp, p)) return rc;
+  const bool held = given(q) || given(exp);
+  if (int rc = pack_params("gelu_pack", x, "x", q, exp, p, held)) return rc;
   if (int rc = check_rows(y, "y", x->size[0], x->size[1], true)) return rc;
   if (y->dtype != x->dtype) return fail(SAF_EINVAL, "y must have x's dtype");
   p.y = y->data;
   p.y_rs = x->size[1];
-  return run_pack("gelu_pack", p, x->dtype, ActPackOp::kGelu, stream);
+  return run_pack("gelu_pack", p, x->dtype, held ? ActPackOp::kGelu : ActPackOp::kGeluOnly, stream);
 }
 
 int saf_gelu_pack_bwd(const saf_tensor_t* q, const saf_tensor_t* exp, const saf_tensor_t* dy, const saf_tensor_t* dx,

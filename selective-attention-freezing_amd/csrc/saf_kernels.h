@@ -375,7 +375,7 @@ int layernorm_bwd_groups(int64_t rows, int C, int n_cu);
 struct ActPackParams {
   const void* x;   // the activation; dy in the backward pass
   int64_t x_rs;
-  int8_t* q;
+  int8_t* q;       // q and exp: null for the GELU alone
   uint8_t* exp;
   void* y;         // gelu(x) (contiguous); the unpacked activation; null in the backward pass: not wanted
   int64_t y_rs;
@@ -384,7 +384,7 @@ struct ActPackParams {
   FastDiv per_row;
   uint32_t units;
 };
-enum class ActPackOp { kPack, kUnpack, kGelu, kGeluBwd };
+enum class ActPackOp { kPack, kUnpack, kGelu, kGeluOnly, kGeluBwd };
 
 // Embedding lookup and gradient (embed.hip); a unit is 8 channels of a token, in the
 // backward pass 256 channels of a chunk of at most 64 sorted positions.

@@ -43,7 +43,7 @@ def unpack_activation(p, dtype=None):
 def gelu_packed(x):
     """Exact GELU of x (..., C), float32, bfloat16 or float16.  Its backward is
     dy (Phi(h) + h phi(h)) for the 8-bit h of x (see pack_activation), which is
-    all that it keeps (reverse mode, once)."""
+    all that it keeps (reverse mode, once); without a gradient nothing is packed."""
     return _ext.bind().gelu_packed(x, False)
 
 
@@ -90,7 +90,8 @@ def mlp_packed(x, w_fc, w_proj, b_fc=None, b_proj=None):
     w_proj (C', F), all of one dtype (under autocast they are cast to its); exact
     GELU.  Keeps x and the GELU's input in 8 bits and recomputes the GELU's output
     from them; the gradients of x, the weights and the biases are those of the
-    held activations (reverse mode, once).  The products are library GEMMs."""
+    held activations (reverse mode, once).  Without a gradient nothing is packed.  The
+    products are library GEMMs."""
     x, (w_fc, w_proj, b_fc, b_proj) = _compute_args(x, [w_fc, w_proj, b_fc, b_proj])
     if w_fc.dim() != 2 or w_proj.dim() != 2 or x.size(-1) != w_fc.size(1) or w_proj.size(1) != w_fc.size(0):
         raise ValueError(f"mlp_packed takes x (..., C), w_fc (F, C) and w_proj (C', F) (got {tuple(x.shape)}, "
@@ -98,6 +99,6 @@ def mlp_packed(x, w_fc, w_proj, b_fc=None, b_proj=None):
     if any(t is not None and t.dtype != x.dtype for t in (w_fc, w_proj, b_fc, b_proj)):
         raise ValueError("mlp_packed takes tensors of one dtype")
     _ext.bind().check_differentiable("mlp_packed", x, w_fc, w_proj, b_fc, b_proj)
-    if not torch.is_grad_enabled():
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, w_fc, w_proj, b_fc, b_proj)):
         return F.linear(gelu_packed(F.linear(x, w_fc, b_fc)), w_proj, b_proj)
     return _MlpPacked.apply(x, w_fc, w_proj, b_fc, b_proj)
