@@ -479,9 +479,13 @@ int saf_embed_fwd(const saf_tensor_t* tokens, const saf_tensor_t* weight, float 
                   const saf_tensor_t* out, void* stream);
 
 /* Gradient of saf_embed_fwd: dweight[v] = scale sum of dout[n] over the n with
- * tokens[n] = v, added in the order of n; every row of dweight (V, C) is written,
- * 16-byte aligned.  The workspace (256-byte aligned) is that of N tokens (at most 2^28), V
- * and C. */
+ * tokens[n] = v; every row of dweight (V, C) is written, 16-byte aligned.  The order of
+ * the additions is fixed by N, C and the tokens: that of n up to 64 tokens.  With more, the
+ * positions sorted by token are cut into chunks of 16, 32 or 64 (by N and C); inside a
+ * chunk the order is that of n, and the chunks' parts of a token after its first are
+ * added in 16 runs, every sixteenth part to one, the first part ahead of the first run,
+ * then the runs in order.  The workspace (256-byte aligned) is that of N tokens (at most
+ * 2^28), V and C. */
 int saf_embed_bwd(const saf_tensor_t* tokens, const saf_tensor_t* dout, float scale, int64_t ignore_index,
                   const saf_tensor_t* dweight, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t saf_embed_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t channels);

@@ -12,16 +12,19 @@
 //    (9 bits at most a pass), while the other workgroups of the same launches
 //    clear dW: the sort takes no time of its own as long as it is the shorter.
 //    Up to kEmbedFew tokens nothing is sorted: each workgroup looks for the words of its
-//    rows in the list of tokens.  Up to kEmbedOnce tokens one workgroup sorts in LDS in one launch.  More go tile
-//    by tile, a launch a pass that places every tile's keys; each workgroup counts the
-//    digits of all keys for itself, from kEmbedCounted tokens on a launch before it
-//    counts them once, and past kEmbedScanned tiles another sums the counts up.
+//    rows in the list of tokens.  Up to kEmbedOnce tokens one workgroup sorts in LDS in
+//    one launch.  More go tile by tile, a launch a pass that places every tile's keys;
+//    each workgroup counts the digits of all keys for itself, from kEmbedCounted tokens
+//    on a launch before it counts them once, and past kEmbedScanned tiles another sums
+//    the counts up.
 // 2. The sorted positions are cut into chunks; a wave sums 256 channels over a chunk
 //    and writes the rows whose tokens lie inside it.  A token that crosses chunks
 //    leaves float32 partial sums,
-// 3. which the third launch adds in order.
-// Every sum is in the order of n whatever runs beside it: no atomic touches a
-// gradient, and each run gives the same bits.
+// 3. which the third launch adds: every kLanes-th of them in one run of their order,
+//    the part of the token's first chunk ahead of the first run, then the runs in order.
+// The order is fixed by N and C, which decide the chunks, and by the positions of the
+// token, whatever runs beside it: no atomic touches a gradient, and each run gives the
+// same bits.  It is the order of n inside a chunk only (up to kEmbedFew tokens: in all).
 #include "saf_kernels.h"
 #include "saf_rowio.h"
 
@@ -516,7 +519,8 @@ __global__ __launch_bounds__(kFewThreads) void embed_few_kernel(const EmbedBwdPa
 
 // Words that cross chunks: the workgroups of the chunk where one begins add its
 // partials, kLanes of them at a time for 32 groups of 8 channels, each lane's in
-// order and then the lanes in order.
+// order (every kLanes-th, the first lane's behind the first chunk's) and then the lanes
+// in order.
 constexpr int kLanes = 16;
 
 template <typename TW>

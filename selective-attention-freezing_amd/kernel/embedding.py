@@ -3,9 +3,9 @@
 ``embed_tokens`` is the lookup that starts a forward pass (nn.Embedding of the
 reference's GPT, nanogpt/model.py:1312-1417), with a factor and the activations'
 own dtype (libsafattn.so ``saf_embed_fwd``); its backward sorts the tokens and
-writes the whole gradient once, the rows of each word added in the order of their
-positions (``saf_embed_bwd``), so it is the same in every run, where a scatter
-with atomics is not.
+writes the whole gradient once, the rows of each word added in an order that the
+tokens and the shape alone decide (``saf_embed_bwd``), so it is the same in every
+run, where a scatter with atomics is not.
 """
 from . import _ext
 
