@@ -13,8 +13,9 @@
 //   gelu'(h) = Phi(h) + h phi(h), from the held h;  du = dy gelu'(h)
 //
 // The kernels move bytes: per 16-bit element 3 + 1/32 (pack, unpack), 5 + 1/32 (GELU,
-// either way), 4 for the GELU alone, where no backward pass will read the 8 bits.  A thread has 8 channels, four threads a block: its largest magnitude
-// takes two lane exchanges inside the quad.  16384 x 2048 bf16: 18 us to pack, 17 to
+// either way), 4 for the GELU alone, where no backward pass will read the 8 bits.  A
+// thread has 8 channels, four threads a block: its largest magnitude takes two lane
+// exchanges inside the quad.  16384 x 2048 bf16: 18 us to pack, 17 to
 // unpack (5.6 and 6.0 TB/s; a copy reaches 5.2); the GELU of 16384 x 8192 110 to 140
 // us forward, 120 to 150 backward (4.8 to 6.1 and 4.5 to 5.6 TB/s, by where its 700 MB
 // meet the 256 MB of the last cache).  Past the caches a pass over both took 242 us
@@ -30,11 +31,14 @@ namespace {
 // Phi(u) and exp(-u^2 / 2): for a = |u| the tail Phi(-a) = exp(-a^2 / 2) t P(t),
 // t = 1 / (1 + c a), P fitted to erfcx(a / sqrt 2) / (2 t) for its largest relative
 // error over 0 <= a <= 14.5, so that small results far below zero keep their digits.
-// 16-bit types: degree 5, 9.2e-6 evaluated in float32 (1/50 of half an fp16 step).
-// float32: degree 8, 3.2e-8; the tail is within 12 float32 roundings (2^-24), as what
-// the square and the product lose is given back to the exponential.  With the library's
-// erfc and exp in its place 16384 x 4096 float32 took 146 us forward and 166 backward,
-// 113 and 112 so (5.4 TB/s).
+// 16-bit types: degree 5, 8.9e-6; evaluated in float32, where u^2 is rounded ahead of the
+// exponential, 9.2e-6 up to a = 3, 1.1e-5 up to 8 and 1.4e-5 up to 13 (1/35 of half an
+// fp16 step).
+// float32: degree 8, 5.5e-8 with the coefficients as they are in float32; the tail is
+// within 16 float32 roundings (2^-24) by their count, 6.2 at most in 400001 arguments
+// down to -12.5, as what the square and the product lose is given back to the exponential
+// (125 without).  With the library's erfc and exp in its place 16384 x 4096 float32 took
+// 146 us forward and 166 backward, 113 and 112 so (5.4 TB/s).
 template <bool EXACT>
 __device__ inline float normal_cdf(float u, float& e) {
   if constexpr (EXACT) {
