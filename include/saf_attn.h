@@ -469,8 +469,10 @@ int saf_token_logprobs_bwd(const saf_token_logprobs_args* args, const saf_tensor
  * Embedding, residual LayerNorm and 8-bit activations, forward and backward, in
  * fp32, bf16 and fp16.  2-D operands are rows (R, C) with a unit column stride
  * and any row stride and alignment; what these entry points write is contiguous
- * unless said otherwise.  All arithmetic is fp32, each result rounded once.  The
- * gradients are sums in a fixed order: the same bits in every run. */
+ * unless said otherwise, and overlaps neither what they read nor each other: a row's
+ * last piece may be read behind a neighbour's write.  All arithmetic is fp32, each
+ * result rounded once.  The gradients are sums in a fixed order: the same bits in
+ * every run. */
 
 /* out[n] = scale weight[tokens[n]] for tokens (N,) int32 / int64, weight (V, C),
  * out (N, C) of any of the three types (bf16 with fp16 is refused).  Rows of
