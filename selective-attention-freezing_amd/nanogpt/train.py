@@ -80,8 +80,11 @@ def _embed(wte, idx):
 
 def _norm(ln, x, d, dtype):
     """(x + d, ln of it); without d the norm of x in dtype."""
-    if not _stock(ln, LayerNorm):
-        x = x if d is None else x + d
+    fused = _stock(ln, LayerNorm)
+    # a sum of one shape, and of x's type
+    if d is not None and not (fused and d.shape == x.shape and torch.promote_types(x.dtype, d.dtype) == x.dtype):
+        x, d = x + d, None
+    if not fused:
         return x, ln(x)
     return _kernel_mod.add_layernorm(x, d, ln.weight, ln.bias, dtype=dtype if d is None else None)
 

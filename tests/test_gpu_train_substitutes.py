@@ -1,12 +1,14 @@
 """nanogpt.train with modules of the caller's own in the model against the model's own
 path, on the kernels: float32, the bounds of test_gpu_train_model.test_float32."""
+import copy
+
 import pytest
 import torch
 import torch.nn as nn
 
 from nanogpt import train
 from test_gpu_train_model import _batch, _loss_and_grads, _model, _near
-from test_train_substitutes import _Adapter, _hook, _Scaled, _Wrapper
+from test_train_substitutes import _Adapter, _Branch, _hook, _Scaled, _Wrapper
 from train_cases import DEV
 
 pytestmark = pytest.mark.gpu
@@ -103,3 +105,21 @@ def test_tokens_outside_the_vocabulary(bad, dtype):
     got = train.token_logprobs(m, idx.to(dtype), nxt).logp.detach()
     assert got[1, 60:].isnan().all()
     assert torch.equal(got[::2], want[::2])
+
+
+@pytest.mark.parametrize("lead", [None, (1,), (1, 1)])
+def test_branches_of_another_type_or_shape(lead):
+    """A float32 branch widens a bf16 residual, as torch's sum does (the model's norms
+    take it under autocast).  Against the same weights in float32, with the bounds of
+    test_gpu_train_model.test_bf16_model (this residual has more bits) and, for q and k,
+    what the model's own path shows of the cancellation in their gradients."""
+    m = _model(dtype=torch.bfloat16, frozen=False)
+    m.transformer.h[0].mlp = _Branch(torch.float32, lead).to(DEV)
+    idx, nxt = _batch(m)
+    whole = copy.deepcopy(m).float()
+    a, ga = _loss_and_grads(whole, lambda: whole.token_logprobs(idx, nxt).logp)
+    with torch.autocast("cuda", torch.bfloat16):
+        _, own = _loss_and_grads(m, lambda: m.token_logprobs(idx, nxt).logp)
+        b, gb = _loss_and_grads(m, lambda: train.token_logprobs(m, idx, nxt).logp)
+    assert (a - b).abs().max() <= 20 * 2.0 ** -8 * 4
+    _near(gb, ga, 20 * 2.0 ** -8 + 0.1, own)

@@ -317,3 +317,31 @@ def test_tokens_outside_the_vocabulary(bad):
     idx[1, 4] = bad
     h, want = train.forward_hidden(m, idx), train.forward_hidden(m, IDX)
     assert h[1, 4].isnan().all() and torch.equal(h[0], want[0])
+
+
+# ---- branches that do not meet the residual ------------------------------------------
+
+class _Branch(nn.Module):
+    """An MLP whose result has a dtype or a shape of its own."""
+
+    def __init__(self, dtype=None, lead=None):
+        super().__init__()
+        self.dtype, self.lead, self.gain = dtype, lead, nn.Parameter(torch.tensor(0.3))
+
+    def forward(self, x):
+        y = (x if self.lead is None else x.mean(dim=(0, 1)).view(*self.lead, -1)) * self.gain
+        return y if self.dtype is None else y.to(self.dtype)
+
+
+@pytest.mark.parametrize("lead", [(), (1,), (1, 1)])
+@pytest.mark.parametrize("at", [0, 1])
+def test_broadcast_branches(lead, at, monkeypatch):
+    """Added as torch adds them, ahead of a norm that takes one shape only."""
+    def strict(x, delta, *a, **k):
+        assert delta is None or delta.shape == x.shape
+        return _norm(x, delta, *a, **k)
+
+    monkeypatch.setattr(kernel, "add_layernorm", strict)
+    m = _model()
+    m.transformer.h[at].mlp = _Branch(lead=lead)
+    assert f"transformer.h.{at}.mlp.gain" in _same(m)
